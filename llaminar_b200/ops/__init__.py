@@ -419,3 +419,6 @@ def spec_verify_reject(p_target, p_draft, draft, seeds, step, n_accept, out_toke
 def moe_topk(logits, k, renorm, ids, weights, counts=None) -> None:
     ext().moe_topk(logits, k, renorm, ids, weights, counts)
     _count()
+
+
+from .hybrid import GdnStash, gdn_commit, gdn_prefill, gdn_verify  # noqa: E402,F401

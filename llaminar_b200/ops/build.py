@@ -16,8 +16,8 @@ NAME = "llaminar_b200_ops"
 CSRC = Path(__file__).resolve().parent / "csrc"
 BUILD_DIR = Path(__file__).resolve().parent / "_build"
 # kernels of models with unquantised matrices, built and loaded on their own: shared ones, latent attention, grouped-query attention,
-# mixers with a recurrent state, and experts
-DENSE, LATENT, GROUPED, MIXERS, EXPERTS = (f"llaminar_b200_{n}" for n in ("dense", "latent", "grouped", "mixers", "experts"))
+# mixers with a recurrent state, and experts; and the blocks of the hybrid family
+DENSE, LATENT, GROUPED, MIXERS, EXPERTS, HYBRID = (f"llaminar_b200_{n}" for n in ("dense", "latent", "grouped", "mixers", "experts", "hybrid"))
 SOURCES = {
     NAME: ["binding.cpp", "gemv.cu", "gemv_stream.cu", "gemm_tc.cu", "gemm_tc_small.cu", "gemm_tc_pair.cu", "attention.cu", "attention_tc.cu", "ops.cu", "gdn.cu", "moe_ep.cu", "moe_stream.cu", "no_alloc.cu"],
     DENSE: ["dense_binding.cpp", "dense_ops.cu"],
@@ -25,6 +25,7 @@ SOURCES = {
     GROUPED: ["grouped_binding.cpp", "grouped.cu", "attention.cu", "attention_tc.cu"],
     MIXERS: ["mixers_binding.cpp", "mixers.cu", "linear_tc.cu"],
     EXPERTS: ["experts_binding.cpp", "experts.cu", "experts_tc.cu"],
+    HYBRID: ["hybrid_binding.cpp", "gdn_rows.cu"],
 }
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--expt-relaxed-constexpr", "-Xptxas", "-v"]

@@ -1,4 +1,5 @@
 // Checks and conversions shared by the small Python bindings.  Every tensor is checked on the host before a launch.
+// (Numbers enter messages as text: a stream of the compiler's own library does not find the facets of the one that torch brings along.)
 #pragma once
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
@@ -29,7 +30,7 @@ inline const int* ints(const Tensor& t, const char* name) {
 }
 inline const float* floats(const Tensor& t, int64_t n, const char* name) {
     want(t, torch::kFloat32, name);
-    TORCH_CHECK(t.numel() == n, name, " must hold ", n, " values");
+    TORCH_CHECK(t.numel() == n, name, " must hold ", std::to_string(n), " values");
     return t.data_ptr<float>();
 }
 inline const float2* angle_ptr(const Tensor& t, int64_t rows) {

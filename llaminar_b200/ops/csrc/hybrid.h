@@ -1,0 +1,36 @@
+// Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace llm {
+
+// The gated delta rule over packed rows.  Row r of `in` holds q | k | v in columns [0, C), the gate z from z_off and (alpha | beta) from
+// ab_off; C = (2 n_k + n_v) d.  Rows cu[b] .. cu[b + 1] are sequence b's (cu nullptr: `rows_per_seq` rows each), its state the slot
+// slots[b] of conv [n_slots, C, K - 1] and rec [n_slots, n_v, d, d]; a sequence whose first row has position 0 starts from zeros
+// (positions nullptr: none does).
+struct GdnParams {
+    const __nv_bfloat16* in; size_t in_row;
+    int C, z_off, ab_off, K, n_k, n_v, d, v_head_offset;
+    const float *conv_w, *ssm_a, *dt_bias, *norm_w;          // [C, K], [n_v], [n_v], [d]
+    float *conv, *rec;
+    const int *positions, *cu, *slots;
+    int n_seqs, rows_per_seq, n_slots, n_rows;               // n_rows: rows of `in` and `out`
+    __nv_bfloat16* out; size_t out_row;                      // [rows, n_v d]
+    float eps;
+    // what a pass that leaves the state alone keeps for gdn_commit, all [n_seqs, rows_per_seq, ...]: decay [n_v], key [n_v, d], correction [n_v, d]
+    // and the convolution's inputs [C]
+    float *keep_a, *keep_k, *keep_u;
+    __nv_bfloat16* keep_x;
+};
+// rows one after the other, any number of them; d of 32, 64 or 128.  With keep_*: the state stays as it is.
+cudaError_t launch_gdn_rows(const GdnParams& p, cudaStream_t st);
+// the convolution windows behind the sequences' rows; to run after everything that reads the old ones
+cudaError_t launch_gdn_windows(const GdnParams& p, cudaStream_t st);
+// states and windows advanced by the first accepted[b] of the kept rows (0: as they were)
+cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStream_t st);
+
+int bounds_status_gdn_rows(bool reset);
+
+}  // namespace llm

@@ -1,0 +1,119 @@
+// Python bindings of the hybrid family's blocks: an extension of its own, so that a process that serves another family neither compiles
+// nor loads it.  Every argument is checked on the host before a launch.
+#include <c10/cuda/CUDAGuard.h>
+
+#include "binding_util.h"
+#include "hybrid.h"
+
+namespace {
+using namespace llm_binding;
+
+void same_device(const Tensor& a, const Tensor& b, const char* name) { TORCH_CHECK(b.is_cuda() && b.device() == a.device(), name, " must be on the device of the rows"); }
+
+// Rows whose values lie next to one another, in bf16
+const __nv_bfloat16* bf16_rows(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kBFloat16 && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)), name, " must be bf16 rows on the GPU");
+    return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
+}
+const float* floats_on(const Tensor& like, const Tensor& t, int64_t n, const char* name) {
+    same_device(like, t, name);
+    return floats(t, n, name);
+}
+const int* ints_on(const Tensor& like, const Tensor& t, int64_t n, const char* name) {
+    same_device(like, t, name);
+    TORCH_CHECK(t.numel() == n, name, " must hold ", std::to_string(n), " values");
+    return ints(t, name);
+}
+
+// The state pools and sizes; C counts the channels of q | k | v
+llm::GdnParams gdn_state(const Tensor& conv, const Tensor& rec, int64_t n_k) {
+    llm::GdnParams p = {};
+    want(conv, torch::kFloat32, "conv_state"); want(rec, torch::kFloat32, "rec");
+    TORCH_CHECK(conv.dim() == 3 && rec.dim() == 4 && rec.size(2) == rec.size(3) && conv.size(0) == rec.size(0), "conv_state must be [slots, C, K - 1] and rec [slots, n_v, d, d]");
+    same_device(rec, conv, "conv_state");
+    p.n_slots = rec.size(0); p.n_v = rec.size(1); p.d = rec.size(2); p.n_k = n_k; p.C = conv.size(1); p.K = conv.size(2) + 1;
+    TORCH_CHECK(p.d == 32 || p.d == 64 || p.d == 128, "head size must be 32, 64 or 128");
+    TORCH_CHECK(p.n_k >= 1 && p.n_v >= 1 && p.n_v <= 65535 && p.C == (2 * p.n_k + p.n_v) * p.d, "conv_state must have (2 n_k + n_v) d channels");
+    TORCH_CHECK(p.K >= 2 && p.K <= 16, "the convolution must have 2 to 16 taps");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(rec.data_ptr()) % 16 == 0, "rec must be 16-byte aligned");
+    p.conv = conv.data_ptr<float>(); p.rec = rec.data_ptr<float>();
+    return p;
+}
+
+llm::GdnParams gdn_params(const Tensor& in, int64_t C, int64_t z_off, int64_t ab_off, const Tensor& conv_w, const Tensor& ssm_a, const Tensor& dt_bias, const Tensor& norm_w,
+                          const Tensor& conv, const Tensor& rec, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps) {
+    llm::GdnParams p = gdn_state(conv, rec, n_k);
+    p.in = bf16_rows(in, "in");
+    same_device(in, rec, "rec"); same_device(in, out, "out");
+    TORCH_CHECK(C == p.C && z_off >= 0 && ab_off >= 0 && z_off + (int64_t)p.n_v * p.d <= in.size(1) && ab_off + 2 * (int64_t)p.n_v <= in.size(1) && C <= in.size(1),
+                "in: columns of q | k | v, z or alpha | beta are missing");
+    TORCH_CHECK(in.size(0) <= INT32_MAX && in.stride(0) <= INT32_MAX, "in: too many rows");
+    p.in_row = in.stride(0); p.n_rows = in.size(0); p.z_off = z_off; p.ab_off = ab_off;
+    TORCH_CHECK(conv_w.dim() == 2 && conv_w.size(1) == p.K, "conv_w must be [C, K]");
+    p.conv_w = floats_on(in, conv_w, (int64_t)p.C * p.K, "conv_w");
+    p.ssm_a = floats_on(in, ssm_a, p.n_v, "ssm_a"); p.dt_bias = floats_on(in, dt_bias, p.n_v, "dt_bias"); p.norm_w = floats_on(in, norm_w, p.d, "norm_w");
+    p.n_seqs = slots.numel();
+    TORCH_CHECK(p.n_seqs <= 65535, "more than 65535 sequences");
+    p.slots = ints_on(in, slots, p.n_seqs, "slots");
+    bf16_rows(out, "out");
+    TORCH_CHECK(out.size(0) == in.size(0) && out.size(1) == (int64_t)p.n_v * p.d, "out must be [rows, n_v d]");
+    p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()); p.out_row = out.stride(0);
+    TORCH_CHECK(v_head_offset >= 0 && v_head_offset <= INT32_MAX / 2, "v_head_offset");
+    p.v_head_offset = v_head_offset; p.eps = eps;
+    return p;
+}
+
+int gdn_prefill(const Tensor& in, int64_t C, int64_t z_off, int64_t ab_off, const Tensor& conv_w, const Tensor& ssm_a, const Tensor& dt_bias, const Tensor& norm_w,
+                const Tensor& conv, const Tensor& rec, const Tensor& positions, const Tensor& cu, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps) {
+    llm::GdnParams p = gdn_params(in, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv, rec, slots, out, n_k, v_head_offset, eps);
+    p.positions = ints_on(in, positions, in.size(0), "positions");
+    p.cu = ints_on(in, cu, p.n_seqs + 1, "cu");
+    const c10::cuda::CUDAGuard guard(in.device());
+    check(llm::launch_gdn_rows(p, stream()), "gdn_prefill");
+    check(llm::launch_gdn_windows(p, stream()), "gdn_prefill");
+    return 2;
+}
+
+// keep: decays [B, R, n_v], keys and corrections [B, R, n_v, d], convolution inputs [B, R, C]
+void keep_args(llm::GdnParams& p, const Tensor& like, const std::vector<Tensor>& keep) {
+    TORCH_CHECK(keep.size() == 4 && keep[3].dim() == 3, "keep");
+    const int64_t B = p.n_seqs, R = keep[3].size(1), n = B * R * p.n_v;
+    TORCH_CHECK(keep[3].size(0) == B && keep[3].size(2) == p.C, "kept rows of other sizes");
+    p.rows_per_seq = R;
+    p.keep_a = const_cast<float*>(floats_on(like, keep[0], n, "decays")); p.keep_k = const_cast<float*>(floats_on(like, keep[1], n * p.d, "keys"));
+    p.keep_u = const_cast<float*>(floats_on(like, keep[2], n * p.d, "corrections"));
+    same_device(like, keep[3], "inputs");
+    want(keep[3], torch::kBFloat16, "inputs");
+    p.keep_x = reinterpret_cast<__nv_bfloat16*>(keep[3].data_ptr());
+}
+
+int gdn_verify(const Tensor& in, int64_t C, int64_t z_off, int64_t ab_off, const Tensor& conv_w, const Tensor& ssm_a, const Tensor& dt_bias, const Tensor& norm_w,
+               const Tensor& conv, const Tensor& rec, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps, const std::vector<Tensor>& keep) {
+    llm::GdnParams p = gdn_params(in, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv, rec, slots, out, n_k, v_head_offset, eps);
+    keep_args(p, in, keep);
+    TORCH_CHECK(in.size(0) == (int64_t)p.n_seqs * p.rows_per_seq, "in must have the same number of rows for every sequence");
+    const c10::cuda::CUDAGuard guard(in.device());
+    check(llm::launch_gdn_rows(p, stream()), "gdn_verify");
+    check(llm::launch_gdn_windows(p, stream()), "gdn_verify");
+    return 2;
+}
+
+void gdn_commit(const std::vector<Tensor>& keep, const Tensor& accepted, const Tensor& conv, const Tensor& rec, const Tensor& slots, int64_t n_k) {
+    llm::GdnParams p = gdn_state(conv, rec, n_k);
+    p.n_seqs = slots.numel();
+    TORCH_CHECK(p.n_seqs <= 65535, "more than 65535 sequences");
+    p.slots = ints_on(rec, slots, p.n_seqs, "slots");
+    keep_args(p, rec, keep);
+    const int* n = ints_on(rec, accepted, p.n_seqs, "n_rows");
+    const c10::cuda::CUDAGuard guard(rec.device());
+    check(llm::launch_gdn_commit(p, n, stream()), "gdn_commit");
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("gdn_prefill", &gdn_prefill);
+    m.def("gdn_verify", &gdn_verify);
+    m.def("gdn_commit", &gdn_commit);
+    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset); });
+}

@@ -1,0 +1,67 @@
+"""Python surface of the hybrid extension (csrc/gdn_rows.cu): the blocks of the Gated-DeltaNet family where
+a step has more than one new row per sequence.
+
+As in :mod:`llaminar_b200.ops`, every call launches hand-written CUDA on the current stream; there is no fallback.  Arguments are checked
+on the host, indices that lie on the device (slots, page ids, row ranges) are the caller's promise.  The PyTorch form of the
+recurrence is in :mod:`llaminar_b200.models.gdn`.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _count
+from . import build as _build
+
+
+def ext():
+    return _build.load(_build.HYBRID)
+
+
+def gdn_prefill(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torch.Tensor, ssm_a: torch.Tensor, dt_bias: torch.Tensor,
+                norm_w: torch.Tensor, conv_state: torch.Tensor, rec: torch.Tensor, positions: torch.Tensor, cu: torch.Tensor,
+                slots: torch.Tensor, out: torch.Tensor, n_k: int, v_head_offset: int, eps: float) -> None:
+    """A Gated-DeltaNet block between its input and output projections for the new rows of a packed batch (arguments as in `gdn_step`).
+    Rows cu[b] .. cu[b + 1] of ``inp`` and ``out`` are sequence b's; its state, the slot slots[b] of the layer's fp32 pools conv_state
+    [slots, C, K - 1] and rec [slots, n_v, d, d], is advanced in place.  A sequence whose first row has position 0 starts from zeros, whatever
+    its slot holds.  Sequences have slots of their own; one without rows keeps its state, and rows outside of all sequences are left as
+    they are.  d is 32, 64 or 128; ssm_a is not positive, so that no decay grows."""
+    _count(ext().gdn_prefill(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, positions, cu, slots, out, n_k, v_head_offset, eps))
+
+
+@dataclass
+class GdnStash:
+    """What `gdn_verify` keeps for `gdn_commit`: decay, key and correction of every row and head, and the convolution's inputs."""
+    decay: torch.Tensor            # [B, R, n_v]
+    key: torch.Tensor              # [B, R, n_v, d]
+    correction: torch.Tensor       # [B, R, n_v, d]
+    inputs: torch.Tensor           # [B, R, C] bf16
+    slots: torch.Tensor            # [B]
+    n_k: int
+
+
+def gdn_verify(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torch.Tensor, ssm_a: torch.Tensor, dt_bias: torch.Tensor,
+               norm_w: torch.Tensor, conv_state: torch.Tensor, rec: torch.Tensor, slots: torch.Tensor, out: torch.Tensor, n_k: int,
+               v_head_offset: int, eps: float) -> GdnStash:
+    """The same for R drafted rows of every sequence (``inp`` [B * R, ...]) with the state left alone: the outputs are those of feeding
+    the rows one by one, and `gdn_commit` advances the states once it is known how many of them are accepted."""
+    B = slots.numel()
+    if B == 0 or inp.shape[0] % B:
+        raise ValueError(f"{inp.shape[0]} rows cannot be shared out evenly between {B} sequences")
+    R, n_v, d = inp.shape[0] // B, rec.shape[1], rec.shape[2]
+    f = lambda *s: torch.empty(*s, dtype=torch.float32, device=inp.device)
+    st = GdnStash(f(B, R, n_v), f(B, R, n_v, d), f(B, R, n_v, d), torch.empty(B, R, C, dtype=torch.bfloat16, device=inp.device), slots, n_k)
+    _count(ext().gdn_verify(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, slots, out, n_k, v_head_offset, eps,
+                            [st.decay, st.key, st.correction, st.inputs]))
+    return st
+
+
+def gdn_commit(stash: GdnStash, n_rows: torch.Tensor, conv_state: torch.Tensor, rec: torch.Tensor) -> None:
+    """Advance the state of every sequence of ``stash`` by its first n_rows[b] rows (int32 on the device; 0 leaves it as it is)."""
+    ext().gdn_commit([stash.decay, stash.key, stash.correction, stash.inputs], n_rows, conv_state, rec, stash.slots, stash.n_k)
+    _count()
+
+
+def bounds_status(reset: bool = True) -> int:
+    return int(ext().bounds_status(bool(reset)))
