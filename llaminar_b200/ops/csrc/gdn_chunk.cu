@@ -1,0 +1,758 @@
+// The gated delta rule over prompts, chunk-parallel on the 5th-generation tensor cores (d = 128).
+//
+// A sequence is cut into chunks of 64 rows.  With G_t the running sum of the log decays inside a chunk, M[t, i] = e^(G_t - G_i) for i <= t, and S the state
+// in front of the chunk, the corrections of a chunk solve a triangular system, and everything else is matrix products:
+//
+//     (I + A) U = R       A[t, i] = b_t M[t, i] k_t.k_i  (i < t)      R_t = b_t (v_t - e^(G_t) S^T k_t)
+//     o_t = e^(G_t) S^T q_t + sum_{i<=t} M[t, i] (q_t.k_i) u_i        S' = e^(G_C) S + sum_i e^(G_C - G_i) k_i u_i^T
+//
+// Every exponent is <= 0.  Two launches:
+//
+//   gdn_chunk_prep   per chunk and key head: convolutions, norms, gates, k.k and q.k (mma.sync), then per value head the inverse T = (I + A)^-1 by
+//                    forward substitution (a thread per column) and P[t, i] = M[t, i] q_t.k_i.  All chunks at once.
+//   gdn_chunk_scan   per sequence and value head, chunk after chunk:  S^T k, S^T q, U = T R, P U and the state's sum as tcgen05.mma with M = 128 value
+//                    columns, the left operand (S, R, U) in tensor memory and T, P, K, Q in shared memory.  A thread has one value column: what it reads
+//                    from an accumulator it scales, splits and writes back as the next product's operand without leaving its lane.
+//
+// Everything stays at 32-bit accuracy: each operand is split into two fp16 numbers (22 bits), which takes three products.  The range comes from
+// powers of two: k, T and q, P are bounded by 1 in magnitude and have fixed factors (a row's update is a contraction, so no entry of T exceeds 1); S,
+// R and U are scaled per value column, to 2^13 .. 2^14 at the largest.  (With q, P and the S and U that only the output sees as single fp16 numbers an output whose
+// sum cancels was 2^-7 off behind the gated norm.)  G is summed in 64 bits: differences of sums near -100 would cost a 32-bit one 2^-17.
+//
+// What bounds it: the scan's chain of three products and three passes through registers per chunk.  Every mbarrier wait is bounded; on a timeout the kernel
+// raises the status word and tears down.
+//
+// (reference: the chunk kernels of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu.)
+#include <cuda_fp16.h>
+
+#include "hybrid.h"
+#include "launch.h"
+#include "tc_tile.cuh"
+
+namespace llm {
+namespace gdc {
+using namespace tc5;
+
+constexpr int D = 128, C = 64;
+// one chunk of a key head: K and Q as two fp16 numbers each, [2 halves of d][64 rows][128 bytes], swizzled as the products read them
+constexpr int IMG = C * D * 2;                              // 16 KB
+constexpr int OFF_KHI = 0, OFF_KLO = IMG, OFF_QHI = 2 * IMG, OFF_QLO = 3 * IMG, KEY_BYTES = 4 * IMG;
+// one chunk of a value head: T and P likewise [64 rows][128 bytes], b v transposed [128 columns][64 rows] fp32, four vectors
+constexpr int TRI = C * C * 2;                              // 8 KB
+constexpr int OFF_THI = 0, OFF_TLO = TRI, OFF_PHI = 2 * TRI, OFF_PLO = 3 * TRI, OFF_V = 4 * TRI, VALS = C * D * 4, OFF_VEC = OFF_V + VALS, VEC_BYTES = 4 * C * 4, HEAD_BYTES = OFF_VEC + VEC_BYTES;
+static_assert(KEY_BYTES % 1024 == 0 && HEAD_BYTES % 1024 == 0, "tiles start on swizzle atoms");
+enum Vec { V_BE = 0, V_EG = C, V_EL = 2 * C, V_ALL = 3 * C };               // b e^G, e^G, e^(G_C - G), e^G_C
+constexpr float SK = 4096.f, SQ = 16384.f;                  // factors of k, T and of q, P
+
+LLM_DEVICE int rows_of(const GdnParams& p, int b, int& first) {
+    first = max(0, min(p.cu[b], p.n_rows));
+    return max(0, min(p.cu[b + 1], p.n_rows) - first);
+}
+// chunks of the sequences in front of sequence `b` (whole warp)
+LLM_DEVICE int chunks_before(const GdnParams& p, int b) {
+    int n = 0, first;
+    for (int i = threadIdx.x & 31; i < b; i += 32) n += (rows_of(p, i, first) + C - 1) / C;
+    return __reduce_add_sync(0xffffffffu, n);
+}
+// the sequence that chunk `u` of the batch belongs to, and that sequence's first chunk (whole warp); -1: none
+LLM_DEVICE int sequence_of(const GdnParams& p, int u, int& at) {
+    const int lane = threadIdx.x & 31;
+    at = 0;
+    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+        int first;
+        const int n = b0 + lane < p.n_seqs ? (rows_of(p, b0 + lane, first) + C - 1) / C : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, at + sum > u);
+        if (m) {
+            const int l = __ffs(m) - 1;
+            at += __shfl_sync(0xffffffffu, sum - n, l);
+            return b0 + l;
+        }
+        at += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return -1;
+}
+
+struct Chunk {                                              // rows [row0, row0 + n) of a sequence that starts at `first`
+    int first, row0, n, slot;
+    bool fresh;
+};
+
+LLM_DEVICE float4 four(const __nv_bfloat16* x, bool aligned) {
+    if (aligned) {
+        const uint2 v = *reinterpret_cast<const uint2*>(x);
+        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+    }
+    return make_float4(__bfloat162float(x[0]), __bfloat162float(x[1]), __bfloat162float(x[2]), __bfloat162float(x[3]));
+}
+LLM_DEVICE void add_tap(float4& y, const float4& w, const float4& x) { y.x += w.x * x.x; y.y += w.y * x.y; y.z += w.z * x.z; y.w += w.w * x.w; }
+LLM_DEVICE float silu_of(float x) { return x / (1.f + __expf(-x)); }
+
+// ROWS rows from t0 of the chunk, channels c .. c + 3: convolution and SiLU; zeros behind the chunk's rows.  K4: four taps, each row loaded once.
+template <int ROWS, bool K4>
+LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, float4 (&y)[ROWS]) {
+    const int K = K4 ? 4 : p.K;
+    auto tap = [&](int w) {
+        const float* x = p.conv_w + (size_t)c * K + w;
+        return make_float4(x[0], x[K], x[2 * K], x[3 * K]);
+    };
+    auto input = [&](int t) -> float4 {                     // row t of the chunk, before its first one: of the sequence, then of the window
+        if (t >= ch.n) return make_float4(0.f, 0.f, 0.f, 0.f);
+        const int r = ch.row0 + t;
+        if (r >= ch.first) return four(p.in + (size_t)r * p.in_row + c, aligned);
+        if (ch.fresh) return make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* w = p.conv + ((size_t)ch.slot * p.C + c) * (K - 1) + (K - 1 + r - ch.first);
+        return make_float4(w[0], w[K - 1], w[2 * (K - 1)], w[3 * (K - 1)]);
+    };
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (K4) {
+        const float4 w0 = tap(0), w1 = tap(1), w2 = tap(2), w3 = tap(3);
+        float4 x[ROWS + 3];
+#pragma unroll
+        for (int i = 0; i < ROWS + 3; ++i) x[i] = input(t0 + i - 3);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) { add_tap(y[i], w0, x[i]); add_tap(y[i], w1, x[i + 1]); add_tap(y[i], w2, x[i + 2]); add_tap(y[i], w3, x[i + 3]); }
+    } else {
+        for (int w = 0; w < K; ++w) {
+            const float4 f = tap(w);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) add_tap(y[i], f, input(t0 + i + w - (K - 1)));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (t0 + i < ch.n) y[i] = make_float4(silu_of(y[i].x), silu_of(y[i].y), silu_of(y[i].z), silu_of(y[i].w));
+        else y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+
+LLM_DEVICE uint32_t pack_half(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+LLM_DEVICE float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+// two numbers as fp16 and what that leaves of them as fp16
+LLM_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack_half(a, b);
+    const float2 h = unpack_half(hi);
+    lo = pack_half(a - h.x, b - h.y);
+}
+
+LLM_DEVICE void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+LLM_DEVICE void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// byte of 16-byte unit u (0 .. 15) of row t in an image of K or Q
+LLM_DEVICE int img_at(int t, int u) { return (u >> 3) * (IMG / 2) + t * 128 + (((u ^ t) & 7) << 4); }
+
+constexpr int PREP_HEADS = 3;                               // value heads whose triangular systems are solved at the same time
+constexpr int PREP_A = 2 * C * C * 4, PREP_SMEM = PREP_A + PREP_HEADS * C * C * 4;        // k.k and q.k, then the matrices A, all where the images were
+static_assert(PREP_SMEM >= KEY_BYTES, "the images");
+constexpr int PREP_THREADS = 256;
+
+struct ChunkParams {
+    GdnParams g;
+    uint8_t* ws;                                            // [units][n_ks] chunks of key heads, then [units][n_v] of value heads
+    int n_ks, u0, units;                                    // key heads in use, first chunk of this pass, chunks of it
+    int* status;
+    int in_aligned, out_aligned;
+};
+LLM_DEVICE uint8_t* key_chunk(const ChunkParams& p, int u, int ks) { return p.ws + ((size_t)u * p.n_ks + ks) * KEY_BYTES; }
+LLM_DEVICE uint8_t* head_chunk(const ChunkParams& p, int u, int h) { return p.ws + (size_t)p.units * p.n_ks * KEY_BYTES + ((size_t)u * p.g.n_v + h) * HEAD_BYTES; }
+
+template <bool K4>
+__global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const ChunkParams cp) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ double s_G[PREP_HEADS][C];
+    __shared__ float s_b[PREP_HEADS][C];
+    __shared__ int s_chunk[5];
+    const GdnParams& p = cp.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ks = blockIdx.x, u = blockIdx.y;              // value heads ks, ks + n_k, ... read this key head
+    if (warp == 0) {
+        int at;
+        const int b = sequence_of(p, cp.u0 + u, at);
+        if (lane == 0) {
+            s_chunk[0] = b;
+            if (b >= 0) {
+                int first;
+                const int n = rows_of(p, b, first), row0 = first + (cp.u0 + u - at) * C;
+                s_chunk[1] = first; s_chunk[2] = row0; s_chunk[3] = min(C, first + n - row0);
+                s_chunk[4] = LLM_CHECK_INDEX(p.slots[b], p.n_slots);
+            }
+        }
+    }
+    __syncthreads();
+    if (s_chunk[0] < 0) return;
+    Chunk ch = {s_chunk[1], s_chunk[2], s_chunk[3], s_chunk[4], false};
+    ch.fresh = p.positions[ch.first] == 0;
+    const bool aligned = cp.in_aligned;
+    const int kh = (ks + p.v_head_offset) % p.n_k;
+    const uint32_t sm = smem_u32(smem);
+
+    // ---- q and k: a warp has eight rows, a lane four channels ----
+    {
+        uint8_t* img = key_chunk(cp, u, ks);
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {              // 0: q, 1: k
+            float4 y[8];
+            conv_rows<8, K4>(p, ch, warp * 8, part * p.n_k * D + kh * D + lane * 4, aligned, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = warp * 8 + i;
+                const float ss = warp_sum(y[i].x * y[i].x + y[i].y * y[i].y + y[i].z * y[i].z + y[i].w * y[i].w);
+                const float r = 1.f / sqrtf(ss + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
+                uint2 hi, lo;
+                split2(y[i].x * r, y[i].y * r, hi.x, lo.x);
+                split2(y[i].z * r, y[i].w * r, hi.y, lo.y);
+                const int at = img_at(t, lane >> 1) + (lane & 1) * 8;
+                const int at_hi = (part ? OFF_KHI : OFF_QHI) + at, at_lo = (part ? OFF_KLO : OFF_QLO) + at;
+                *reinterpret_cast<uint2*>(smem + at_hi) = hi; *reinterpret_cast<uint2*>(img + at_hi) = hi;
+                *reinterpret_cast<uint2*>(smem + at_lo) = lo; *reinterpret_cast<uint2*>(img + at_lo) = lo;
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- k.k (warps 0 - 3) and q.k (warps 4 - 7), 16 rows a warp, up to the diagonal ----
+    {
+        const int w = warp & 3, mat = lane >> 3, r8 = lane & 7;
+        const bool kk = warp < 4;
+        float acc[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll 1
+        for (int s = 0; s < 8; ++s) {
+            uint32_t ah[4], al[4];
+            const int a_at = img_at(16 * w + (lane & 15), 2 * s + (lane >> 4));
+            ldsm4(sm + (kk ? OFF_KHI : OFF_QHI) + a_at, ah);
+            ldsm4(sm + (kk ? OFF_KLO : OFF_QLO) + a_at, al);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (n > w) break;
+                uint32_t bh[4], bl[4];
+                const int b_at = img_at(16 * n + (mat >> 1) * 8 + r8, 2 * s + (mat & 1));
+                ldsm4(sm + OFF_KHI + b_at, bh);
+                ldsm4(sm + OFF_KLO + b_at, bl);
+                mma16(acc[2 * n], ah, bh[0], bh[1]);
+                mma16(acc[2 * n + 1], ah, bh[2], bh[3]);
+                mma16(acc[2 * n], al, bh[0], bh[1]);
+                mma16(acc[2 * n + 1], al, bh[2], bh[3]);
+                mma16(acc[2 * n], ah, bl[0], bl[1]);
+                mma16(acc[2 * n + 1], ah, bl[2], bl[3]);
+            }
+        }
+        __syncthreads();                                    // the images have been read: the products take their place
+        float* dst = reinterpret_cast<float*>(smem) + (kk ? 0 : C * C);
+        const float f = kk ? 1.f / (SK * SK) : 1.f / SK;    // q.k keeps its factor SQ
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            if (n > 2 * w + 1) break;
+            const int t = 16 * w + (lane >> 2), i = 8 * n + (lane & 3) * 2;
+            *reinterpret_cast<float2*>(dst + t * C + i) = make_float2(acc[n][0] * f, acc[n][1] * f);
+            *reinterpret_cast<float2*>(dst + (t + 8) * C + i) = make_float2(acc[n][2] * f, acc[n][3] * f);
+        }
+    }
+    const float* s_kk = reinterpret_cast<const float*>(smem);
+    const float* s_qk = s_kk + C * C;
+
+    for (int h0 = ks; h0 < p.n_v; h0 += PREP_HEADS * p.n_k) {
+        const int nh = min(PREP_HEADS, (p.n_v - h0 + p.n_k - 1) / p.n_k);
+        __syncthreads();
+        // ---- gates: a warp per head, two rows a lane ----
+        if (warp < nh) {
+            const int h = h0 + warp * p.n_k;
+            const float a = p.ssm_a[h], dt = p.dt_bias[h];
+            float g[2], b[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int t = 2 * lane + e;
+                g[e] = b[e] = 0.f;
+                if (t < ch.n) {
+                    const __nv_bfloat16* ab = p.in + (size_t)(ch.row0 + t) * p.in_row + p.ab_off;
+                    const float x = __bfloat162float(ab[h]) + dt;
+                    g[e] = a * (x > 20.f ? x : log1pf(expf(x)));
+                    b[e] = 1.f / (1.f + expf(-__bfloat162float(ab[p.n_v + h])));
+                }
+            }
+            double sum = (double)g[0] + (double)g[1];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const double G1 = sum, G0 = sum - (double)g[1], all = __shfl_sync(0xffffffffu, sum, 31);
+            s_G[warp][2 * lane] = G0; s_G[warp][2 * lane + 1] = G1;
+            s_b[warp][2 * lane] = b[0]; s_b[warp][2 * lane + 1] = b[1];
+            float2* vec = reinterpret_cast<float2*>(head_chunk(cp, u, h) + OFF_VEC);
+            const float e0 = expf((float)G0), e1 = expf((float)G1), ea = expf((float)all);
+            vec[V_BE / 2 + lane] = make_float2(b[0] * e0, b[1] * e1);
+            vec[V_EG / 2 + lane] = make_float2(e0, e1);
+            vec[V_EL / 2 + lane] = make_float2(expf((float)(all - G0)), expf((float)(all - G1)));
+            vec[V_ALL / 2 + lane] = make_float2(ea, ea);
+        }
+        __syncthreads();
+        // ---- A and P; b v, transposed ----
+#pragma unroll 1
+        for (int hi = 0; hi < nh; ++hi) {
+            const int h = h0 + hi * p.n_k;
+            uint8_t* dst = head_chunk(cp, u, h);
+            float* A = reinterpret_cast<float*>(smem + PREP_A) + hi * C * C;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int item = tid + r * PREP_THREADS, t = item >> 3, unit = item & 7;
+                const double Gt = s_G[hi][t];
+                const float b = s_b[hi][t];
+                float a8[8], p8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = unit * 8 + e;
+                    a8[e] = p8[e] = 0.f;
+                    if (i <= t) {
+                        const float m = expf((float)(Gt - s_G[hi][i]));
+                        p8[e] = m * s_qk[t * C + i];
+                        if (i < t) a8[e] = b * m * s_kk[t * C + i];
+                    }
+                }
+                *reinterpret_cast<float4*>(A + t * C + unit * 8) = make_float4(a8[0], a8[1], a8[2], a8[3]);
+                *reinterpret_cast<float4*>(A + t * C + unit * 8 + 4) = make_float4(a8[4], a8[5], a8[6], a8[7]);
+                uint4 ph, pl;
+                split2(p8[0], p8[1], ph.x, pl.x); split2(p8[2], p8[3], ph.y, pl.y); split2(p8[4], p8[5], ph.z, pl.z); split2(p8[6], p8[7], ph.w, pl.w);
+                const int at = t * 128 + (((unit ^ t) & 7) << 4);
+                *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
+                *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
+            }
+            float4 y[8];
+            conv_rows<8, K4>(p, ch, warp * 8, 2 * p.n_k * D + h * D + lane * 4, aligned, y);
+            float v[4][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float b = s_b[hi][warp * 8 + i];
+                v[0][i] = b * y[i].x; v[1][i] = b * y[i].y; v[2][i] = b * y[i].z; v[3][i] = b * y[i].w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int col = lane * 4 + e;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    *reinterpret_cast<float4*>(dst + OFF_V + col * 256 + (((2 * warp + q) ^ (col & 7)) << 4)) = make_float4(v[e][4 * q], v[e][4 * q + 1], v[e][4 * q + 2], v[e][4 * q + 3]);
+            }
+        }
+        __syncthreads();
+        // ---- T: column j of (I + A)^-1 by forward substitution, 64 threads a head ----
+        if (tid < nh * C) {
+            const int hi = tid / C, j = tid % C;
+            const float* A = reinterpret_cast<const float*>(smem + PREP_A) + hi * C * C;
+            uint8_t* dst = head_chunk(cp, u, h0 + hi * p.n_k);
+            float x[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                float s[4] = {i == j ? 1.f : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int m = 0; m < i; m += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(A + i * C + m);       // zeros from column i on
+                    s[0] -= a.x * x[m];
+                    if (m + 1 < i) s[1] -= a.y * x[m + 1];
+                    if (m + 2 < i) s[2] -= a.z * x[m + 2];
+                    if (m + 3 < i) s[3] -= a.w * x[m + 3];
+                }
+                x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+                const float f = x[i] * SK;
+                const __half h = __float2half_rn(f), l = __float2half_rn(f - __half2float(h));
+                const int at = i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 7) * 2;
+                *reinterpret_cast<__half*>(dst + OFF_THI + at) = h;
+                *reinterpret_cast<__half*>(dst + OFF_TLO + at) = l;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// scan
+// ------------------------------------------------------------------------------------------------
+// Warps 0-3 and 4-7 are the two math groups: a thread has a value column (== TMEM lane), the groups share out a row's columns.  Warps 8-11 write the output,
+// warp 12 copies, warp 13 allocates tensor memory and issues the products.
+constexpr int THREADS = 512;
+constexpr int REGS_MATH = 176, REGS_OUT = 88, REGS_REST = 72, REGS_LAUNCH = 128;
+static_assert(2 * REGS_MATH + REGS_OUT + REGS_REST <= 4 * REGS_LAUNCH, "a warpgroup would wait for registers that nobody gives back");
+// shared memory: K, T and the vectors in two stages; V, Q and P, which are free again while their chunk is still at work, once; the output's rows
+constexpr int ST_T = 2 * IMG, ST_VEC = ST_T + 2 * TRI, STAGE_BYTES = ST_VEC + VEC_BYTES;
+constexpr int SM_V = 2 * STAGE_BYTES, SM_Q = SM_V + VALS, SM_P = SM_Q + 2 * IMG, SM_O = SM_P + 2 * TRI, SCAN_SMEM = SM_O + C * D * 4 + 1024;
+static_assert(STAGE_BYTES % 1024 == 0 && SM_Q % 1024 == 0 && SM_P % 1024 == 0, "tiles start on swizzle atoms");
+static_assert(SCAN_SMEM <= 227 * 1024, "shared memory of a CTA");
+// tensor memory columns; the state's sum takes the columns of the state operand, U those of S^T k, U' those of R
+constexpr uint32_t T_SHI = 0, T_SLO = 64, T_DS = 0, T_KS = 128, T_QS = 192, T_PU = 256, T_RHI = 320, T_RLO = 352, T_UHI = 384, T_ULO = 416;
+__host__ __device__ constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }     // fp16 x fp16 -> fp32, M = 128
+
+enum Bar { IN_FULL = 0, IN_EMPTY = 2, V_FULL = 4, V_EMPTY, Q_FULL, Q_EMPTY, P_FULL, P_EMPTY, S_RDY, KS_DONE, R_RDY, U_DONE, U_RDY, DS_DONE, O_DONE, O_FREE, N_BARS };
+
+// the power of two that brings `top` into [2^13, 2^14), and its inverse
+LLM_DEVICE void scale_for(float top, float& s, float& inv) {
+    const int e = (int)(__float_as_uint(top) >> 23);        // 0 .. 255: top >= 0
+    const int b = min(253, 267 - e);
+    s = __uint_as_float((uint32_t)b << 23);
+    inv = __uint_as_float((uint32_t)(254 - b) << 23);
+}
+LLM_DEVICE void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+LLM_DEVICE float4 lds4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+
+__global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkParams cp) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[N_BARS];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort[2];                              // [1] stays 0 here (tc_common.cuh: restarts the wait clock when set)
+    __shared__ int s_first[3];
+    __shared__ float s_top[3][2][D];                        // largest magnitudes of a column, per math group
+    __shared__ float s_inv[2][2][D];                        // inverse scales of S and U, by parity of the chunk
+    const GdnParams& p = cp.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.x, b = blockIdx.y;
+    if (warp == 0) {
+        const int before = chunks_before(p, b);
+        if (lane == 0) s_first[0] = before;
+    }
+    __syncthreads();
+    int first;
+    const int n_rows = rows_of(p, b, first), u_first = s_first[0];
+    const int c0 = max(0, cp.u0 - u_first), c1 = min((n_rows + C - 1) / C, cp.u0 + cp.units - u_first);
+    if (c0 >= c1) return;                                   // uniform for the CTA, before any barrier or allocation
+    const int nc = c1 - c0, u_ws = u_first + c0 - cp.u0;    // chunks of this pass, the first one's place in the workspace
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = smem_u32(s_bars);
+    auto bar = [&](int i) { return bars + i * 8; };
+    if (tid == 0) {
+        s_abort[0] = 0; s_abort[1] = 0;
+        for (int i = 0; i < N_BARS; ++i) {
+            int n = 1;
+            if (i == IN_EMPTY || i == IN_EMPTY + 1) n = 1 + 8 + 4;                   // the products, the math and the output warps
+            if (i == S_RDY || i == R_RDY || i == U_RDY || i == V_EMPTY) n = 8;
+            if (i == O_FREE) n = 4;
+            mbar_init(bar(i), n);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    volatile int* abort_flag = s_abort;
+    auto stage = [&](int c) { return base + (c & 1) * STAGE_BYTES; };
+    auto phase = [](int c) { return (uint32_t)((c >> 1) & 1); };               // of a stage's barriers
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MATH));
+        const int w = warp >> 2, col = tid & 127;
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const bool fresh = c0 == 0 && p.positions[first] == 0;
+        const int slot = LLM_CHECK_INDEX(p.slots[b], p.n_slots);
+        float* state = p.rec + ((size_t)slot * p.n_v + h) * (D * D) + (size_t)w * 64 * D + col;
+        float S[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) S[i] = fresh ? 0.f : state[(size_t)i * D];
+        // largest magnitude of the column over both groups
+        auto column_top = [&](int which, float mine) {
+            s_top[which][w][col] = mine;
+            tc_fence_before();
+            bar_sync(1, 256);
+            tc_fence_after();
+            return fmaxf(mine, s_top[which][w ^ 1][col]);
+        };
+        bool ok = true;
+        for (int c = 0; c < nc; ++c) {
+            const uint32_t vec = stage(c) + ST_VEC, vals = base + SM_V + col * 256;
+            float s, inv;
+            // ---- the state as an operand ----
+            {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(S[i]));
+                scale_for(column_top(0, top), s, inv);
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) split2(S[2 * i] * s, S[2 * i + 1] * s, hi[i], lo[i]);
+                tmem_st32(t_lane + T_SHI + w * 32, hi);
+                tmem_st32(t_lane + T_SLO + w * 32, lo);
+                if (w == 0) s_inv[c & 1][0][col] = inv;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                mbar_arrive_if(bar(S_RDY), lane == 0);
+            }
+            // ---- R = b v - b e^G S^T k ----
+            ok = mbar_wait_warp(bar(IN_FULL + (c & 1)), phase(c), abort_flag) && mbar_wait_warp(bar(V_FULL), c & 1, abort_flag) && mbar_wait_warp(bar(KS_DONE), c & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            {
+                uint32_t x[32];
+                tmem_ld_n<32>(t_lane + T_KS + w * 32, x);
+                const float f = -inv * (1.f / SK);
+                float r[32], top = 0.f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 v = lds4(vals + (((8 * w + q) ^ (col & 7)) << 4)), be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
+                    r[4 * q] = fmaf(be.x * f, __uint_as_float(x[4 * q]), v.x);
+                    r[4 * q + 1] = fmaf(be.y * f, __uint_as_float(x[4 * q + 1]), v.y);
+                    r[4 * q + 2] = fmaf(be.z * f, __uint_as_float(x[4 * q + 2]), v.z);
+                    r[4 * q + 3] = fmaf(be.w * f, __uint_as_float(x[4 * q + 3]), v.w);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(r[i]));
+                scale_for(column_top(1, top), s, inv);
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) split2(r[2 * i] * s, r[2 * i + 1] * s, hi[i], lo[i]);
+                tmem_st_n<16>(t_lane + T_RHI + w * 16, hi);
+                tmem_st_n<16>(t_lane + T_RLO + w * 16, lo);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                mbar_arrive_if(bar(R_RDY), lane == 0);
+                mbar_arrive_if(bar(V_EMPTY), lane == 0);
+            }
+            // ---- U = T R; U e^(G_C - G) for the state ----
+            ok = mbar_wait_warp(bar(U_DONE), c & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const float decay = lds4(vec + V_ALL * 4).x;
+            {
+                uint32_t x[32];
+                tmem_ld_n<32>(t_lane + T_KS + w * 32, x);
+                const float f = inv * (1.f / SK);
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(__uint_as_float(x[i])));
+                scale_for(column_top(2, top), s, inv);       // of the accumulator as it is: its own factor f goes into the inverse
+                uint32_t uh[16], ul[16], hi[16], lo[16];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 el = lds4(vec + (V_EL + 32 * w + 4 * q) * 4);
+                    const float a = __uint_as_float(x[4 * q]) * s, bb = __uint_as_float(x[4 * q + 1]) * s, cc = __uint_as_float(x[4 * q + 2]) * s, d = __uint_as_float(x[4 * q + 3]) * s;
+                    split2(a, bb, uh[2 * q], ul[2 * q]);
+                    split2(cc, d, uh[2 * q + 1], ul[2 * q + 1]);
+                    split2(a * el.x, bb * el.y, hi[2 * q], lo[2 * q]);
+                    split2(cc * el.z, d * el.w, hi[2 * q + 1], lo[2 * q + 1]);
+                }
+                inv *= f;
+                tmem_st_n<16>(t_lane + T_RHI + w * 16, hi);
+                tmem_st_n<16>(t_lane + T_RLO + w * 16, lo);
+                tmem_st_n<16>(t_lane + T_UHI + w * 16, uh);
+                tmem_st_n<16>(t_lane + T_ULO + w * 16, ul);
+                if (w == 0) s_inv[c & 1][1][col] = inv;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                mbar_arrive_if(bar(U_RDY), lane == 0);
+                mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
+            }
+            // ---- S = e^G_C S + sum ----
+            ok = mbar_wait_warp(bar(DS_DONE), c & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const float f = inv * (1.f / SK);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t x[32];
+                tmem_ld_n<32>(t_lane + T_DS + w * 64 + half * 32, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) S[half * 32 + i] = fmaf(f, __uint_as_float(x[i]), decay * S[half * 32 + i]);
+            }
+        }
+        if (ok) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) state[(size_t)i * D] = S[i];
+        }
+    } else if (warp < 12) {
+        // ------------------------------ output: o, gated norm ------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OUT));
+        const int ow = warp - 8, col = tid & 127;
+        const uint32_t t_lane = tmem + ((uint32_t)(ow * 32) << 16);
+        const float4 gain = make_float4(p.norm_w[lane * 4], p.norm_w[lane * 4 + 1], p.norm_w[lane * 4 + 2], p.norm_w[lane * 4 + 3]);
+        const bool in_aligned = cp.in_aligned, out_aligned = cp.out_aligned;
+        for (int c = 0; c < nc; ++c) {
+            if (!mbar_wait_warp(bar(O_DONE), c & 1, abort_flag)) break;
+            tc_fence_after();
+            bar_sync(2, 128);                               // the last chunk's rows have been read
+            const uint32_t vec = stage(c) + ST_VEC, rows = base + SM_O;
+            const float fs = s_inv[c & 1][0][col] * (1.f / SQ), fu = s_inv[c & 1][1][col] * (1.f / SQ);
+#pragma unroll
+            for (int part = 0; part < 4; ++part) {
+                uint32_t a[16], e[16];
+                tmem_ld_n<16>(t_lane + T_QS + part * 16, a);
+                tmem_ld_n<16>(t_lane + T_PU + part * 16, e);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 eg = lds4(vec + (V_EG + part * 16 + q * 4) * 4);
+                    const float g[4] = {eg.x, eg.y, eg.z, eg.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float o = fmaf(g[k] * fs, __uint_as_float(a[4 * q + k]), fu * __uint_as_float(e[4 * q + k]));
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows + (part * 16 + q * 4 + k) * (D * 4) + col * 4), "f"(o) : "memory");
+                    }
+                }
+            }
+            tc_fence_before();
+            bar_sync(2, 128);
+            mbar_arrive_if(bar(O_FREE), lane == 0);
+            mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
+            const int row0 = first + (c0 + c) * C, n = min(C, first + n_rows - row0);
+#pragma unroll 4
+            for (int i = 0; i < C / 4; ++i) {
+                const int t = i * 4 + ow;
+                if (t >= n) break;
+                const float4 o = lds4(rows + t * (D * 4) + lane * 16);
+                const float4 z = four(p.in + (size_t)(row0 + t) * p.in_row + p.z_off + h * D + lane * 4, in_aligned);
+                const float ss = warp_sum(o.x * o.x + o.y * o.y + o.z * o.z + o.w * o.w);
+                const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                const uint32_t lo = pack_bf16(o.x * r * gain.x * silu_of(z.x), o.y * r * gain.y * silu_of(z.y)), hi = pack_bf16(o.z * r * gain.z * silu_of(z.z), o.w * r * gain.w * silu_of(z.w));
+                __nv_bfloat16* dst = p.out + (size_t)(row0 + t) * p.out_row + h * D + lane * 4;
+                if (out_aligned) {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+                } else {
+                    dst[0] = __ushort_as_bfloat16(lo & 0xffff); dst[1] = __ushort_as_bfloat16(lo >> 16);
+                    dst[2] = __ushort_as_bfloat16(hi & 0xffff); dst[3] = __ushort_as_bfloat16(hi >> 16);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
+        if (warp == 12 && elect_one()) {
+            // ------------------------------ copies ------------------------------
+            const int ks = h % p.n_k;
+            auto load = [&](int full, int empty, uint32_t parity, int bytes) {
+                if (!mbar_wait(bar(empty), parity ^ 1, abort_flag)) return false;
+                mbar_arrive_expect_tx(bar(full), bytes);
+                return true;
+            };
+            for (int c = 0; c < nc; ++c) {
+                const uint8_t *key = key_chunk(cp, u_ws + c, ks), *head = head_chunk(cp, u_ws + c, h);
+                const int in = IN_FULL + (c & 1);
+                if (!load(in, IN_EMPTY + (c & 1), phase(c), STAGE_BYTES)) break;
+                bulk_load(stage(c), key + OFF_KHI, 2 * IMG, bar(in));
+                bulk_load(stage(c) + ST_T, head + OFF_THI, 2 * TRI, bar(in));
+                bulk_load(stage(c) + ST_VEC, head + OFF_VEC, VEC_BYTES, bar(in));
+                if (!load(V_FULL, V_EMPTY, c & 1, VALS)) break;
+                bulk_load(base + SM_V, head + OFF_V, VALS, bar(V_FULL));
+                if (!load(Q_FULL, Q_EMPTY, c & 1, 2 * IMG)) break;
+                bulk_load(base + SM_Q, key + OFF_QHI, 2 * IMG, bar(Q_FULL));
+                if (!load(P_FULL, P_EMPTY, c & 1, 2 * TRI)) break;
+                bulk_load(base + SM_P, head + OFF_PHI, 2 * TRI, bar(P_FULL));
+            }
+        } else if (warp == 13 && elect_one()) {
+            // ------------------------------ products ------------------------------
+            constexpr uint32_t MN = 1u << 16;               // right operand with its rows along K
+            for (int c = 0; c < nc; ++c) {
+                const uint32_t key = stage(c), tri = key + ST_T, q = base + SM_Q, pt = base + SM_P;
+                if (!mbar_wait(bar(IN_FULL + (c & 1)), phase(c), abort_flag) || !mbar_wait(bar(S_RDY), c & 1, abort_flag)) break;
+                tc_fence_after();
+                auto with_rows = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {      // [128 columns x d] [64 rows x d]^T
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_f16_ts(tmem + d, tmem + a + k * 8, smem_desc_sw128(img + (k >> 2) * (IMG / 2)) + 2 * (k & 3), idesc(C), !first_one || k > 0 ? 1u : 0u);
+                };
+                auto with_tri = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {       // [128 columns x 64 rows] times a lower triangle's transpose
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)             // columns in front of the diagonal's block are zero
+                        mma_f16_ts(tmem + d + 16 * k, tmem + a + k * 8, smem_desc_sw128(img + 16 * k * 128) + 2 * k, idesc(C - 16 * k), !first_one || k > 0 ? 1u : 0u);
+                };
+                auto with_keys = [&](uint32_t a, uint32_t img, bool first_one) {                  // [128 columns x 64 rows] [64 rows x d]
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16_ts(tmem + T_DS, tmem + a + k * 8, smem_desc_mn_sw128(img + 16 * k * 128, IMG / 2), idesc(D) | MN, !first_one || k > 0 ? 1u : 0u);
+                };
+                with_rows(T_KS, T_SHI, key, true);
+                with_rows(T_KS, T_SLO, key, false);
+                with_rows(T_KS, T_SHI, key + IMG, false);
+                mma_commit(bar(KS_DONE));
+                if (!mbar_wait(bar(Q_FULL), c & 1, abort_flag) || (c > 0 && !mbar_wait(bar(O_FREE), (c - 1) & 1, abort_flag))) break;
+                tc_fence_after();
+                with_rows(T_QS, T_SHI, q, true);
+                with_rows(T_QS, T_SLO, q, false);
+                with_rows(T_QS, T_SHI, q + IMG, false);
+                mma_commit(bar(Q_EMPTY));
+                if (!mbar_wait(bar(R_RDY), c & 1, abort_flag)) break;
+                tc_fence_after();
+                with_tri(T_KS, T_RHI, tri, true);
+                with_tri(T_KS, T_RLO, tri, false);
+                with_tri(T_KS, T_RHI, tri + TRI, false);
+                mma_commit(bar(U_DONE));
+                if (!mbar_wait(bar(P_FULL), c & 1, abort_flag) || !mbar_wait(bar(U_RDY), c & 1, abort_flag)) break;
+                tc_fence_after();
+                with_keys(T_RHI, key, true);
+                with_keys(T_RLO, key, false);
+                with_keys(T_RHI, key + IMG, false);
+                mma_commit(bar(DS_DONE));
+                with_tri(T_PU, T_UHI, pt, true);
+                with_tri(T_PU, T_ULO, pt, false);
+                with_tri(T_PU, T_UHI, pt + TRI, false);
+                mma_commit(bar(IN_EMPTY + (c & 1)));
+                mma_commit(bar(P_EMPTY));
+                mma_commit(bar(O_DONE));
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    teardown(abort_flag, tid, cp.status);
+    if (warp == 13) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+}  // namespace gdc
+
+// Bytes of workspace that a pass over `units` chunks takes
+size_t gdn_chunk_bytes(int units, int n_k, int n_v) {
+    return (size_t)units * ((size_t)(n_k < n_v ? n_k : n_v) * gdc::KEY_BYTES + (size_t)n_v * gdc::HEAD_BYTES);
+}
+
+cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, int* status, int& launches, cudaStream_t st) {
+    launches = 0;
+    if (g.n_seqs == 0 || g.n_rows == 0) return cudaSuccess;
+    if (g.d != gdc::D || (reinterpret_cast<uintptr_t>(workspace) & 1023)) return cudaErrorInvalidValue;
+    const int total = g.n_rows / gdc::C + g.n_seqs;         // no fewer than the sequences' chunks
+    const size_t most = bytes / gdn_chunk_bytes(1, g.n_k, g.n_v);
+    if (most < 1) return cudaErrorInvalidValue;
+    gdc::ChunkParams p = {};
+    p.g = g; p.ws = static_cast<uint8_t*>(workspace); p.status = status;
+    p.n_ks = g.n_k < g.n_v ? g.n_k : g.n_v;
+    auto fits = [](const void* x, size_t row, int off) { return (reinterpret_cast<uintptr_t>(x) & 7) == 0 && row % 4 == 0 && off % 4 == 0; };
+    p.in_aligned = fits(g.in, g.in_row, g.z_off);
+    p.out_aligned = fits(g.out, g.out_row, 0);
+    const auto prep = g.K == 4 ? gdc::gdn_chunk_prep_kernel<true> : gdc::gdn_chunk_prep_kernel<false>;
+    cudaError_t e = tc5::raise_smem(prep, gdc::PREP_SMEM);
+    if (e == cudaSuccess) e = tc5::raise_smem(gdc::gdn_chunk_scan_kernel, gdc::SCAN_SMEM);
+    if (e != cudaSuccess) return e;
+    for (int u0 = 0; u0 < total; u0 += p.units) {           // as many chunks at a time as the workspace holds
+        p.u0 = u0;
+        p.units = (int)((size_t)(total - u0) < most ? (size_t)(total - u0) : most);
+        if (p.units > 65535) p.units = 65535;
+        prep<<<dim3(p.n_ks, p.units), gdc::PREP_THREADS, gdc::PREP_SMEM, st>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        gdc::gdn_chunk_scan_kernel<<<dim3(g.n_v, g.n_seqs), gdc::THREADS, gdc::SCAN_SMEM, st>>>(p);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        launches += 2;
+    }
+    return cudaSuccess;
+}
+
+LLM_DEFINE_BOUNDS_STATUS_READER(bounds_status_gdn_chunk)
+
+}  // namespace llm

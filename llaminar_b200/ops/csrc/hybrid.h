@@ -1,4 +1,4 @@
-// Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu).
+// Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu, gdn_chunk.cu).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -31,6 +31,12 @@ cudaError_t launch_gdn_windows(const GdnParams& p, cudaStream_t st);
 // states and windows advanced by the first accepted[b] of the kept rows (0: as they were)
 cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStream_t st);
 
+// the same for prompts, chunk-parallel on the tensor cores; d = 128.  `workspace` (1024-byte aligned) holds as many chunks as it has room for, at
+// least one; `status` receives STATUS_TIMEOUT if a wait gave up.  (Windows are left to launch_gdn_windows here too.)
+size_t gdn_chunk_bytes(int units, int n_k, int n_v);
+cudaError_t launch_gdn_chunk(const GdnParams& p, void* workspace, size_t bytes, int* status, int& launches, cudaStream_t st);
+
 int bounds_status_gdn_rows(bool reset);
+int bounds_status_gdn_chunk(bool reset);
 
 }  // namespace llm

@@ -64,14 +64,27 @@ llm::GdnParams gdn_params(const Tensor& in, int64_t C, int64_t z_off, int64_t ab
 }
 
 int gdn_prefill(const Tensor& in, int64_t C, int64_t z_off, int64_t ab_off, const Tensor& conv_w, const Tensor& ssm_a, const Tensor& dt_bias, const Tensor& norm_w,
-                const Tensor& conv, const Tensor& rec, const Tensor& positions, const Tensor& cu, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps) {
+                const Tensor& conv, const Tensor& rec, const Tensor& positions, const Tensor& cu, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps,
+                const OptTensor& workspace, const OptTensor& status) {
     llm::GdnParams p = gdn_params(in, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv, rec, slots, out, n_k, v_head_offset, eps);
     p.positions = ints_on(in, positions, in.size(0), "positions");
     p.cu = ints_on(in, cu, p.n_seqs + 1, "cu");
     const c10::cuda::CUDAGuard guard(in.device());
-    check(llm::launch_gdn_rows(p, stream()), "gdn_prefill");
+    int launches = 1;
+    if (workspace) {
+        same_device(in, *workspace, "workspace");
+        want(*workspace, torch::kUInt8, "workspace");
+        TORCH_CHECK(status.has_value(), "the chunk form takes a status word");
+        same_device(in, *status, "status");
+        want(*status, torch::kInt32, "status");
+        const uintptr_t at = reinterpret_cast<uintptr_t>(workspace->data_ptr()), first = (at + 1023) & ~(uintptr_t)1023;
+        TORCH_CHECK(workspace->numel() >= (int64_t)(first - at + llm::gdn_chunk_bytes(1, p.n_k, p.n_v)), "workspace too small");
+        check(llm::launch_gdn_chunk(p, reinterpret_cast<void*>(first), workspace->numel() - (first - at), status->data_ptr<int>(), launches, stream()), "gdn_prefill");
+    } else {
+        check(llm::launch_gdn_rows(p, stream()), "gdn_prefill");
+    }
     check(llm::launch_gdn_windows(p, stream()), "gdn_prefill");
-    return 2;
+    return launches + 1;
 }
 
 // keep: decays [B, R, n_v], keys and corrections [B, R, n_v, d], convolution inputs [B, R, C]
@@ -115,5 +128,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gdn_prefill", &gdn_prefill);
     m.def("gdn_verify", &gdn_verify);
     m.def("gdn_commit", &gdn_commit);
-    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset); });
+    m.def("gdn_chunk_bytes", &llm::gdn_chunk_bytes);
+    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset) | llm::bounds_status_gdn_chunk(reset); });
 }

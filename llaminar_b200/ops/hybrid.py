@@ -1,4 +1,4 @@
-"""Python surface of the hybrid extension (csrc/gdn_rows.cu): the blocks of the Gated-DeltaNet family where
+"""Python surface of the hybrid extension (csrc/gdn_rows.cu, gdn_chunk.cu): the blocks of the Gated-DeltaNet family where
 a step has more than one new row per sequence.
 
 As in :mod:`llaminar_b200.ops`, every call launches hand-written CUDA on the current stream; there is no fallback.  Arguments are checked
@@ -11,12 +11,26 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _count
+from . import _count, scratch_for
 from . import build as _build
 
 
 def ext():
     return _build.load(_build.HYBRID)
+
+
+GDN_CHUNK = 64                 # rows of a chunk
+GDN_CHUNK_MIN_ROWS = 8         # rows per sequence, on average, from which the chunk form is taken
+GDN_WORKSPACE = 256 << 20      # bytes that a pass of the chunk form may hold; longer prompts take several passes
+
+
+def _gdn_workspace(inp: torch.Tensor, n_seqs: int, n_k: int, n_v: int, d: int):
+    """Workspace of the chunk form, or None where the rows go one after the other."""
+    if d != 128 or n_seqs == 0 or inp.shape[0] < GDN_CHUNK_MIN_ROWS * n_seqs:
+        return None
+    one = ext().gdn_chunk_bytes(1, n_k, n_v)
+    units = max(1, min(inp.shape[0] // GDN_CHUNK + n_seqs, GDN_WORKSPACE // one))
+    return torch.empty(units * one + 1024, dtype=torch.uint8, device=inp.device)
 
 
 def gdn_prefill(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torch.Tensor, ssm_a: torch.Tensor, dt_bias: torch.Tensor,
@@ -27,7 +41,9 @@ def gdn_prefill(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torc
     [slots, C, K - 1] and rec [slots, n_v, d, d], is advanced in place.  A sequence whose first row has position 0 starts from zeros, whatever
     its slot holds.  Sequences have slots of their own; one without rows keeps its state, and rows outside of all sequences are left as
     they are.  d is 32, 64 or 128; ssm_a is not positive, so that no decay grows."""
-    _count(ext().gdn_prefill(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, positions, cu, slots, out, n_k, v_head_offset, eps))
+    ws = _gdn_workspace(inp, slots.numel(), n_k, rec.shape[1], rec.shape[-1]) if inp.is_cuda else None
+    _count(ext().gdn_prefill(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, positions, cu, slots, out, n_k, v_head_offset, eps,
+                             ws, scratch_for(inp.device).status if ws is not None else None))
 
 
 @dataclass
