@@ -8,8 +8,9 @@
 //
 // Every exponent is <= 0.  Two launches:
 //
-//   gdn_chunk_prep   per chunk and key head: convolutions, norms, gates, k.k and q.k (mma.sync), then per value head the inverse T = (I + A)^-1 by
-//                    forward substitution (a thread per column) and P[t, i] = M[t, i] q_t.k_i.  All chunks at once.
+//   gdn_chunk_prep   per chunk and key head: convolutions, norms, gates, k.k and q.k (mma.sync), then per value head P[t, i] = M[t, i] q_t.k_i and the inverse
+//                    T = (I + A)^-1: blocks of 16 rows on the diagonal by forward substitution (a thread per column), the others from them by products,
+//                    T_ij = -T_ii sum_k A_ik T_kj, a warp per column of blocks.  All chunks at once.
 //   gdn_chunk_scan   per sequence and value head, chunk after chunk:  S^T k, S^T q, U = T R, P U and the state's sum as tcgen05.mma with M = 128 value
 //                    columns, the left operand (S, R, U) in tensor memory and T, P, K, Q in shared memory.  A thread has one value column: what it reads
 //                    from an accumulator it scales, splits and writes back as the next product's operand without leaving its lane.
@@ -39,7 +40,7 @@ constexpr int IMG = C * D * 2;                              // 16 KB
 constexpr int OFF_KHI = 0, OFF_KLO = IMG, OFF_QHI = 2 * IMG, OFF_QLO = 3 * IMG, KEY_BYTES = 4 * IMG;
 // one chunk of a value head: T and P likewise [64 rows][128 bytes], b v transposed [128 columns][64 rows] fp32, four vectors
 constexpr int TRI = C * C * 2;                              // 8 KB
-constexpr int OFF_THI = 0, OFF_TLO = TRI, OFF_PHI = 2 * TRI, OFF_PLO = 3 * TRI, OFF_V = 4 * TRI, VALS = C * D * 4, OFF_VEC = OFF_V + VALS, VEC_BYTES = 4 * C * 4, HEAD_BYTES = OFF_VEC + VEC_BYTES;
+constexpr int OFF_THI = 0, OFF_PHI = 2 * TRI, OFF_PLO = 3 * TRI, OFF_V = 4 * TRI, VALS = C * D * 4, OFF_VEC = OFF_V + VALS, VEC_BYTES = 4 * C * 4, HEAD_BYTES = OFF_VEC + VEC_BYTES;
 static_assert(KEY_BYTES % 1024 == 0 && HEAD_BYTES % 1024 == 0, "tiles start on swizzle atoms");
 enum Vec { V_BE = 0, V_EG = C, V_EL = 2 * C, V_ALL = 3 * C };               // b e^G, e^G, e^(G_C - G), e^G_C
 constexpr float SK = 4096.f, SQ = 16384.f;                  // factors of k, T and of q, P
@@ -83,17 +84,16 @@ struct Chunk {                                              // rows [row0, row0 
     bool fresh;
 };
 
-LLM_DEVICE float4 four(const __nv_bfloat16* x, bool aligned) {
-    if (aligned) {
-        const uint2 v = *reinterpret_cast<const uint2*>(x);
-        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
-    }
-    return make_float4(__bfloat162float(x[0]), __bfloat162float(x[1]), __bfloat162float(x[2]), __bfloat162float(x[3]));
+// four neighbours as they lie; the host says whether 8-byte loads may be used
+LLM_DEVICE uint2 four(const __nv_bfloat16* x, bool aligned) {
+    if (aligned) return *reinterpret_cast<const uint2*>(x);
+    return make_uint2(__bfloat16_as_ushort(x[0]) | (uint32_t)__bfloat16_as_ushort(x[1]) << 16, __bfloat16_as_ushort(x[2]) | (uint32_t)__bfloat16_as_ushort(x[3]) << 16);
 }
 LLM_DEVICE void add_tap(float4& y, const float4& w, const float4& x) { y.x += w.x * x.x; y.y += w.y * x.y; y.z += w.z * x.z; y.w += w.w * x.w; }
-LLM_DEVICE float silu_of(float x) { return x / (1.f + __expf(-x)); }
 
 // ROWS rows from t0 of the chunk, channels c .. c + 3: convolution and SiLU; zeros behind the chunk's rows.  K4: four taps, each row loaded once.
+// Rows are loaded without a branch, from places inside of the sequence, so that all of them are on their way together; then zeros take the place of what is
+// not there and the window that of what lies before the sequence's first row.
 template <int ROWS, bool K4>
 LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, float4 (&y)[ROWS]) {
     const int K = K4 ? 4 : p.K;
@@ -101,33 +101,54 @@ LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bo
         const float* x = p.conv_w + (size_t)c * K + w;
         return make_float4(x[0], x[K], x[2 * K], x[3 * K]);
     };
-    auto input = [&](int t) -> float4 {                     // row t of the chunk, before its first one: of the sequence, then of the window
+    auto row = [&](int t) { return p.in + (size_t)min(max(ch.row0 + t, ch.first), ch.row0 + ch.n - 1) * p.in_row + c; };
+    auto value = [&](const uint2& x, int t) {
         if (t >= ch.n) return make_float4(0.f, 0.f, 0.f, 0.f);
-        const int r = ch.row0 + t;
-        if (r >= ch.first) return four(p.in + (size_t)r * p.in_row + c, aligned);
-        if (ch.fresh) return make_float4(0.f, 0.f, 0.f, 0.f);
-        const float* w = p.conv + ((size_t)ch.slot * p.C + c) * (K - 1) + (K - 1 + r - ch.first);
-        return make_float4(w[0], w[K - 1], w[2 * (K - 1)], w[3 * (K - 1)]);
+        return make_float4(bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y));
     };
+    auto before = [&](float4& x, int t) {                   // r < 0: of the window
+        const int r = ch.row0 + t - ch.first;
+        if (r >= 0) return;
+        const float* w = p.conv + ((size_t)ch.slot * p.C + c) * (K - 1) + (K - 1 + r);
+        x = ch.fresh ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(w[0], w[K - 1], w[2 * (K - 1)], w[3 * (K - 1)]);
+    };
+    const bool edge = ch.row0 + t0 - (K - 1) < ch.first;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (K4) {
+        uint2 raw[ROWS + 3];
+        if (aligned) {
+#pragma unroll
+            for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row(t0 + i - 3), true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row(t0 + i - 3), false);
+        }
         const float4 w0 = tap(0), w1 = tap(1), w2 = tap(2), w3 = tap(3);
         float4 x[ROWS + 3];
 #pragma unroll
-        for (int i = 0; i < ROWS + 3; ++i) x[i] = input(t0 + i - 3);
+        for (int i = 0; i < ROWS + 3; ++i) x[i] = value(raw[i], t0 + i - 3);
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) before(x[i], t0 + i - 3);
+        }
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) { add_tap(y[i], w0, x[i]); add_tap(y[i], w1, x[i + 1]); add_tap(y[i], w2, x[i + 2]); add_tap(y[i], w3, x[i + 3]); }
     } else {
         for (int w = 0; w < K; ++w) {
             const float4 f = tap(w);
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) add_tap(y[i], f, input(t0 + i + w - (K - 1)));
+            for (int i = 0; i < ROWS; ++i) {
+                const int t = t0 + i + w - (K - 1);
+                float4 x = value(four(row(t), aligned), t);
+                if (edge) before(x, t);
+                add_tap(y[i], f, x);
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        if (t0 + i < ch.n) y[i] = make_float4(silu_of(y[i].x), silu_of(y[i].y), silu_of(y[i].z), silu_of(y[i].w));
+        if (t0 + i < ch.n) y[i] = make_float4(silu(y[i].x), silu(y[i].y), silu(y[i].z), silu(y[i].w));
         else y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
 }
@@ -144,6 +165,39 @@ LLM_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     lo = pack_half(a - h.x, b - h.y);
 }
 
+// two numbers at a time
+typedef unsigned long long f32x2;
+LLM_DEVICE f32x2 pair(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+LLM_DEVICE float2 both(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+LLM_DEVICE void split2(f32x2 v, uint32_t& hi, uint32_t& lo) {
+    const float2 x = both(v);
+    hi = pack_half(x.x, x.y);
+    const float2 h = unpack_half(hi), l = both(fma2(pair(h.x, h.y), pair(-1.f, -1.f), v));
+    lo = pack_half(l.x, l.y);
+}
+LLM_DEVICE float top2(float t, f32x2 v) {
+    const float2 x = both(v);
+    return fmaxf(t, fmaxf(fabsf(x.x), fabsf(x.y)));
+}
+
 LLM_DEVICE void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -155,8 +209,10 @@ LLM_DEVICE void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
 LLM_DEVICE int img_at(int t, int u) { return (u >> 3) * (IMG / 2) + t * 128 + (((u ^ t) & 7) << 4); }
 
 constexpr int PREP_HEADS = 3;                               // value heads whose triangular systems are solved at the same time
-constexpr int PREP_A = 2 * C * C * 4, PREP_SMEM = PREP_A + PREP_HEADS * C * C * 4;        // k.k and q.k, then the matrices A, all where the images were
-static_assert(PREP_SMEM >= KEY_BYTES, "the images");
+constexpr int PREP_A = 2 * C * C * 4, PREP_DIAG = PREP_A + PREP_HEADS * 2 * TRI;           // k.k and q.k, then the matrices A (as two fp16 numbers), all where the images were
+constexpr int PREP_SMEM = PREP_DIAG + PREP_HEADS * C * 16 * 4;                              // and their diagonal blocks in fp32
+static_assert(PREP_DIAG >= KEY_BYTES, "the images");
+constexpr float SX = 1024.f;                                // factor of sum_k A_ik T_kj = -(I + A_ii) T_ij, at most 17
 constexpr int PREP_THREADS = 256;
 
 struct ChunkParams {
@@ -210,7 +266,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             for (int i = 0; i < 8; ++i) {
                 const int t = warp * 8 + i;
                 const float ss = warp_sum(y[i].x * y[i].x + y[i].y * y[i].y + y[i].z * y[i].z + y[i].w * y[i].w);
-                const float r = 1.f / sqrtf(ss + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
+                const float r = rsqrtf(ss + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
                 uint2 hi, lo;
                 split2(y[i].x * r, y[i].y * r, hi.x, lo.x);
                 split2(y[i].z * r, y[i].w * r, hi.y, lo.y);
@@ -286,20 +342,22 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                     b[e] = 1.f / (1.f + expf(-__bfloat162float(ab[p.n_v + h])));
                 }
             }
-            double sum = (double)g[0] + (double)g[1];
+            // sums in units of ln 2, as exp2 takes them
+            const double l0 = (double)g[0] * 1.4426950408889634, l1 = (double)g[1] * 1.4426950408889634;
+            double sum = l0 + l1;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double x = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += x;
             }
-            const double G1 = sum, G0 = sum - (double)g[1], all = __shfl_sync(0xffffffffu, sum, 31);
+            const double G1 = sum, G0 = sum - l1, all = __shfl_sync(0xffffffffu, sum, 31);
             s_G[warp][2 * lane] = G0; s_G[warp][2 * lane + 1] = G1;
             s_b[warp][2 * lane] = b[0]; s_b[warp][2 * lane + 1] = b[1];
             float2* vec = reinterpret_cast<float2*>(head_chunk(cp, u, h) + OFF_VEC);
-            const float e0 = expf((float)G0), e1 = expf((float)G1), ea = expf((float)all);
+            const float e0 = ex2((float)G0), e1 = ex2((float)G1), ea = ex2((float)all);
             vec[V_BE / 2 + lane] = make_float2(b[0] * e0, b[1] * e1);
             vec[V_EG / 2 + lane] = make_float2(e0, e1);
-            vec[V_EL / 2 + lane] = make_float2(expf((float)(all - G0)), expf((float)(all - G1)));
+            vec[V_EL / 2 + lane] = make_float2(ex2((float)(all - G0)), ex2((float)(all - G1)));
             vec[V_ALL / 2 + lane] = make_float2(ea, ea);
         }
         __syncthreads();
@@ -308,7 +366,8 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
         for (int hi = 0; hi < nh; ++hi) {
             const int h = h0 + hi * p.n_k;
             uint8_t* dst = head_chunk(cp, u, h);
-            float* A = reinterpret_cast<float*>(smem + PREP_A) + hi * C * C;
+            uint8_t* A = smem + PREP_A + hi * 2 * TRI;
+            float* diag = reinterpret_cast<float*>(smem + PREP_DIAG) + hi * C * 16;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int item = tid + r * PREP_THREADS, t = item >> 3, unit = item & 7;
@@ -320,16 +379,23 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                     const int i = unit * 8 + e;
                     a8[e] = p8[e] = 0.f;
                     if (i <= t) {
-                        const float m = expf((float)(Gt - s_G[hi][i]));
+                        const float m = ex2((float)(Gt - s_G[hi][i]));
                         p8[e] = m * s_qk[t * C + i];
                         if (i < t) a8[e] = b * m * s_kk[t * C + i];
                     }
                 }
-                *reinterpret_cast<float4*>(A + t * C + unit * 8) = make_float4(a8[0], a8[1], a8[2], a8[3]);
-                *reinterpret_cast<float4*>(A + t * C + unit * 8 + 4) = make_float4(a8[4], a8[5], a8[6], a8[7]);
-                uint4 ph, pl;
+                if (unit >> 1 == t >> 4) {
+                    *reinterpret_cast<float4*>(diag + t * 16 + (unit & 1) * 8) = make_float4(a8[0], a8[1], a8[2], a8[3]);
+                    *reinterpret_cast<float4*>(diag + t * 16 + (unit & 1) * 8 + 4) = make_float4(a8[4], a8[5], a8[6], a8[7]);
+                }
+                uint4 ph, pl, ah, al;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a8[e] *= SK;
+                split2(a8[0], a8[1], ah.x, al.x); split2(a8[2], a8[3], ah.y, al.y); split2(a8[4], a8[5], ah.z, al.z); split2(a8[6], a8[7], ah.w, al.w);
                 split2(p8[0], p8[1], ph.x, pl.x); split2(p8[2], p8[3], ph.y, pl.y); split2(p8[4], p8[5], ph.z, pl.z); split2(p8[6], p8[7], ph.w, pl.w);
                 const int at = t * 128 + (((unit ^ t) & 7) << 4);
+                *reinterpret_cast<uint4*>(A + at) = ah;
+                *reinterpret_cast<uint4*>(A + TRI + at) = al;
                 *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
                 *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
             }
@@ -350,30 +416,109 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             }
         }
         __syncthreads();
-        // ---- T: column j of (I + A)^-1 by forward substitution, 64 threads a head ----
+        // ---- the diagonal's blocks of T, in the place of A's: a thread per column ----
         if (tid < nh * C) {
-            const int hi = tid / C, j = tid % C;
-            const float* A = reinterpret_cast<const float*>(smem + PREP_A) + hi * C * C;
-            uint8_t* dst = head_chunk(cp, u, h0 + hi * p.n_k);
-            float x[C];
+            const int hi = tid / C, j = tid % C, at = j & 15;
+            const float* diag = reinterpret_cast<const float*>(smem + PREP_DIAG) + hi * C * 16 + (j & ~15) * 16;
+            float x[16];
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                float s[4] = {i == j ? 1.f : 0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 16; ++i) {
+                float sum = i == at ? 1.f : 0.f;
 #pragma unroll
                 for (int m = 0; m < i; m += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(A + i * C + m);       // zeros from column i on
-                    s[0] -= a.x * x[m];
-                    if (m + 1 < i) s[1] -= a.y * x[m + 1];
-                    if (m + 2 < i) s[2] -= a.z * x[m + 2];
-                    if (m + 3 < i) s[3] -= a.w * x[m + 3];
+                    const float4 a = *reinterpret_cast<const float4*>(diag + i * 16 + m);       // zeros from column i on
+                    sum -= a.x * x[m];
+                    if (m + 1 < i) sum -= a.y * x[m + 1];
+                    if (m + 2 < i) sum -= a.z * x[m + 2];
+                    if (m + 3 < i) sum -= a.w * x[m + 3];
                 }
-                x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+                x[i] = sum;
+            }
+            uint8_t* T = smem + PREP_A + hi * 2 * TRI + (j & 7) * 2;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
                 const float f = x[i] * SK;
                 const __half h = __float2half_rn(f), l = __float2half_rn(f - __half2float(h));
-                const int at = i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 7) * 2;
-                *reinterpret_cast<__half*>(dst + OFF_THI + at) = h;
-                *reinterpret_cast<__half*>(dst + OFF_TLO + at) = l;
+                const int t = (j & ~15) + i, row = t * 128 + (((j >> 3) ^ (t & 7)) << 4);
+                *reinterpret_cast<__half*>(T + row) = h;
+                *reinterpret_cast<__half*>(T + TRI + row) = l;
             }
+        }
+        __syncthreads();
+        // ---- the other blocks, T_ij transposed at (j, i): a left operand of the next product as it comes out ----
+#pragma unroll 1
+        for (int item = warp; item < nh * 3; item += PREP_THREADS / 32) {
+            const int hi = item % nh, j = item / nh, mat = lane >> 3, r8 = lane & 7;
+            const uint32_t A = sm + PREP_A + hi * 2 * TRI;
+            // 16 x 16 block (bi, bj) as the right operand of a product with its transpose
+            auto right = [&](int bi, int bj, uint32_t (&h)[4], uint32_t (&l)[4]) {
+                const int row = 16 * bi + (mat >> 1) * 8 + r8;
+                const uint32_t at = A + row * 128 + (((2 * bj + (mat & 1)) ^ (row & 7)) << 4);
+                ldsm4(at, h);
+                ldsm4(at + TRI, l);
+            };
+            auto product = [&](float (&acc)[2][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const uint32_t (&bh)[4], const uint32_t (&bl)[4]) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16(acc[n], ah, bh[2 * n], bh[2 * n + 1]);
+                    mma16(acc[n], al, bh[2 * n], bh[2 * n + 1]);
+                    mma16(acc[n], ah, bl[2 * n], bl[2 * n + 1]);
+                }
+            };
+            auto left = [&](const float (&acc)[2][4], float f, uint32_t (&h)[4], uint32_t (&l)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split2(acc[e >> 1][2 * (e & 1)] * f, acc[e >> 1][2 * (e & 1) + 1] * f, h[e], l[e]);
+            };
+            uint32_t th[4][4], tl[4][4];                    // T_kj transposed, k = j, j + 1, ... (from place 0 on)
+            {
+                const int row = 16 * j + (mat >> 1) * 8 + r8;
+                const uint32_t at = A + row * 128 + (((2 * j + (mat & 1)) ^ (row & 7)) << 4);
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(th[0][0]), "=r"(th[0][1]), "=r"(th[0][2]), "=r"(th[0][3]) : "r"(at));
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(tl[0][0]), "=r"(tl[0][1]), "=r"(tl[0][2]), "=r"(tl[0][3]) : "r"(at + TRI));
+            }
+#pragma unroll
+            for (int step = 1; step < 4; ++step) {
+                const int i = j + step;
+                if (i > 3) break;
+                float acc[2][4] = {};
+                uint32_t bh[4], bl[4], xh[4], xl[4];
+#pragma unroll
+                for (int k = 0; k < step; ++k) {
+                    right(i, j + k, bh, bl);
+                    product(acc, th[k], tl[k], bh, bl);
+                }
+                left(acc, SX / (SK * SK), xh, xl);
+                float out[2][4] = {};
+                right(i, i, bh, bl);
+                product(out, xh, xl, bh, bl);
+                left(out, -1.f / SX, th[step], tl[step]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {               // rows lane / 4 (+ 8), columns of the 8-value unit e / 2
+                    const int row = 16 * j + (lane >> 2) + (e & 1) * 8;
+                    uint8_t* at = smem + PREP_A + hi * 2 * TRI + row * 128 + (((2 * i + (e >> 1)) ^ (row & 7)) << 4) + (lane & 3) * 4;
+                    *reinterpret_cast<uint32_t*>(at) = th[step][e];
+                    *reinterpret_cast<uint32_t*>(at + TRI) = tl[step][e];
+                }
+            }
+        }
+        __syncthreads();
+        // ---- T as the scan reads it ----
+#pragma unroll 1
+        for (int item = tid; item < nh * 2 * C * 8; item += PREP_THREADS) {
+            const int hi = item / (2 * C * 8), half = item / (C * 8) & 1, t = item / 8 % C, unit = item & 7;
+            const uint8_t* T = smem + PREP_A + hi * 2 * TRI + half * TRI;
+            const int to = t * 128 + (((unit ^ t) & 7) << 4);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (unit >> 1 == t >> 4) {
+                v = *reinterpret_cast<const uint4*>(T + to);
+            } else if (unit >> 1 < t >> 4) {
+                uint32_t x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = *reinterpret_cast<const unsigned short*>(T + (unit * 8 + e) * 128 + (((t >> 3) ^ e) << 4) + (t & 7) * 2);
+                v = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+            }
+            *reinterpret_cast<uint4*>(head_chunk(cp, u, h0 + hi * p.n_k) + OFF_THI + half * TRI + to) = v;
         }
     }
 }
@@ -384,7 +529,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
 // Warps 0-3 and 4-7 are the two math groups: a thread has a value column (== TMEM lane), the groups share out a row's columns.  Warps 8-11 write the output,
 // warp 12 copies, warp 13 allocates tensor memory and issues the products.
 constexpr int THREADS = 512;
-constexpr int REGS_MATH = 176, REGS_OUT = 88, REGS_REST = 72, REGS_LAUNCH = 128;
+constexpr int REGS_MATH = 176, REGS_OUT = 104, REGS_REST = 56, REGS_LAUNCH = 128;
 static_assert(2 * REGS_MATH + REGS_OUT + REGS_REST <= 4 * REGS_LAUNCH, "a warpgroup would wait for registers that nobody gives back");
 // shared memory: K, T and the vectors in two stages; V, Q and P, which are free again while their chunk is still at work, once; the output's rows
 constexpr int ST_T = 2 * IMG, ST_VEC = ST_T + 2 * TRI, STAGE_BYTES = ST_VEC + VEC_BYTES;
@@ -404,6 +549,16 @@ LLM_DEVICE void scale_for(float top, float& s, float& inv) {
     s = __uint_as_float((uint32_t)b << 23);
     inv = __uint_as_float((uint32_t)(254 - b) << 23);
 }
+LLM_DEVICE void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {       // readable behind the next wait, and `keep`
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+}
+template <int N> LLM_DEVICE void keep(uint32_t (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+LLM_DEVICE f32x2 pair_of(uint32_t a, uint32_t b) { return pair(__uint_as_float(a), __uint_as_float(b)); }
 LLM_DEVICE void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 LLM_DEVICE float4 lds4(uint32_t a) {
     float4 v;
@@ -466,9 +621,9 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
         const bool fresh = c0 == 0 && p.positions[first] == 0;
         const int slot = LLM_CHECK_INDEX(p.slots[b], p.n_slots);
         float* state = p.rec + ((size_t)slot * p.n_v + h) * (D * D) + (size_t)w * 64 * D + col;
-        float S[64];
+        f32x2 S[32];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) S[i] = fresh ? 0.f : state[(size_t)i * D];
+        for (int i = 0; i < 32; ++i) S[i] = fresh ? pair(0.f, 0.f) : pair(state[(size_t)(2 * i) * D], state[(size_t)(2 * i + 1) * D]);
         // largest magnitude of the column over both groups
         auto column_top = [&](int which, float mine) {
             s_top[which][w][col] = mine;
@@ -485,11 +640,11 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             {
                 float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(S[i]));
+                for (int i = 0; i < 32; ++i) top = top2(top, S[i]);
                 scale_for(column_top(0, top), s, inv);
                 uint32_t hi[32], lo[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) split2(S[2 * i] * s, S[2 * i + 1] * s, hi[i], lo[i]);
+                for (int i = 0; i < 32; ++i) split2(mul2(S[i], pair(s, s)), hi[i], lo[i]);
                 tmem_st32(t_lane + T_SHI + w * 32, hi);
                 tmem_st32(t_lane + T_SLO + w * 32, lo);
                 if (w == 0) s_inv[c & 1][0][col] = inv;
@@ -506,21 +661,21 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 uint32_t x[32];
                 tmem_ld_n<32>(t_lane + T_KS + w * 32, x);
                 const float f = -inv * (1.f / SK);
-                float r[32], top = 0.f;
+                const f32x2 f2 = pair(f, f);
+                f32x2 r[16];
+                float top = 0.f;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const float4 v = lds4(vals + (((8 * w + q) ^ (col & 7)) << 4)), be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
-                    r[4 * q] = fmaf(be.x * f, __uint_as_float(x[4 * q]), v.x);
-                    r[4 * q + 1] = fmaf(be.y * f, __uint_as_float(x[4 * q + 1]), v.y);
-                    r[4 * q + 2] = fmaf(be.z * f, __uint_as_float(x[4 * q + 2]), v.z);
-                    r[4 * q + 3] = fmaf(be.w * f, __uint_as_float(x[4 * q + 3]), v.w);
+                    r[2 * q] = fma2(mul2(pair(be.x, be.y), f2), pair_of(x[4 * q], x[4 * q + 1]), pair(v.x, v.y));
+                    r[2 * q + 1] = fma2(mul2(pair(be.z, be.w), f2), pair_of(x[4 * q + 2], x[4 * q + 3]), pair(v.z, v.w));
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(r[i]));
+                for (int i = 0; i < 16; ++i) top = top2(top, r[i]);
                 scale_for(column_top(1, top), s, inv);
                 uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) split2(r[2 * i] * s, r[2 * i + 1] * s, hi[i], lo[i]);
+                for (int i = 0; i < 16; ++i) split2(mul2(r[i], pair(s, s)), hi[i], lo[i]);
                 tmem_st_n<16>(t_lane + T_RHI + w * 16, hi);
                 tmem_st_n<16>(t_lane + T_RLO + w * 16, lo);
                 tmem_wait_st();
@@ -546,11 +701,11 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const float4 el = lds4(vec + (V_EL + 32 * w + 4 * q) * 4);
-                    const float a = __uint_as_float(x[4 * q]) * s, bb = __uint_as_float(x[4 * q + 1]) * s, cc = __uint_as_float(x[4 * q + 2]) * s, d = __uint_as_float(x[4 * q + 3]) * s;
-                    split2(a, bb, uh[2 * q], ul[2 * q]);
-                    split2(cc, d, uh[2 * q + 1], ul[2 * q + 1]);
-                    split2(a * el.x, bb * el.y, hi[2 * q], lo[2 * q]);
-                    split2(cc * el.z, d * el.w, hi[2 * q + 1], lo[2 * q + 1]);
+                    const f32x2 a = mul2(pair_of(x[4 * q], x[4 * q + 1]), pair(s, s)), e = mul2(pair_of(x[4 * q + 2], x[4 * q + 3]), pair(s, s));
+                    split2(a, uh[2 * q], ul[2 * q]);
+                    split2(e, uh[2 * q + 1], ul[2 * q + 1]);
+                    split2(mul2(a, pair(el.x, el.y)), hi[2 * q], lo[2 * q]);
+                    split2(mul2(e, pair(el.z, el.w)), hi[2 * q + 1], lo[2 * q + 1]);
                 }
                 inv *= f;
                 tmem_st_n<16>(t_lane + T_RHI + w * 16, hi);
@@ -574,12 +729,16 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 uint32_t x[32];
                 tmem_ld_n<32>(t_lane + T_DS + w * 64 + half * 32, x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) S[half * 32 + i] = fmaf(f, __uint_as_float(x[i]), decay * S[half * 32 + i]);
+                for (int i = 0; i < 16; ++i) S[half * 16 + i] = fma2(pair(f, f), pair_of(x[2 * i], x[2 * i + 1]), mul2(pair(decay, decay), S[half * 16 + i]));
             }
         }
         if (ok) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) state[(size_t)i * D] = S[i];
+            for (int i = 0; i < 32; ++i) {
+                const float2 x = both(S[i]);
+                state[(size_t)(2 * i) * D] = x.x;
+                state[(size_t)(2 * i + 1) * D] = x.y;
+            }
         }
     } else if (warp < 12) {
         // ------------------------------ output: o, gated norm ------------------------------
@@ -589,6 +748,13 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
         const float4 gain = make_float4(p.norm_w[lane * 4], p.norm_w[lane * 4 + 1], p.norm_w[lane * 4 + 2], p.norm_w[lane * 4 + 3]);
         const bool in_aligned = cp.in_aligned, out_aligned = cp.out_aligned;
         for (int c = 0; c < nc; ++c) {
+            const int row0 = first + (c0 + c) * C, n = min(C, first + n_rows - row0);
+            uint2 z[C / 4];                                 // the rows' gates, on their way while the chunk is at work
+#pragma unroll
+            for (int i = 0; i < C / 4; ++i) {
+                const __nv_bfloat16* x = p.in + (size_t)(row0 + min(i * 4 + ow, n - 1)) * p.in_row + p.z_off + h * D + lane * 4;
+                z[i] = four(x, in_aligned);
+            }
             if (!mbar_wait_warp(bar(O_DONE), c & 1, abort_flag)) break;
             tc_fence_after();
             bar_sync(2, 128);                               // the last chunk's rows have been read
@@ -597,8 +763,9 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
 #pragma unroll
             for (int part = 0; part < 4; ++part) {
                 uint32_t a[16], e[16];
-                tmem_ld_n<16>(t_lane + T_QS + part * 16, a);
+                tmem_ld16_issue(t_lane + T_QS + part * 16, a);
                 tmem_ld_n<16>(t_lane + T_PU + part * 16, e);
+                keep(a);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float4 eg = lds4(vec + (V_EG + part * 16 + q * 4) * 4);
@@ -614,22 +781,36 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             bar_sync(2, 128);
             mbar_arrive_if(bar(O_FREE), lane == 0);
             mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
-            const int row0 = first + (c0 + c) * C, n = min(C, first + n_rows - row0);
-#pragma unroll 4
-            for (int i = 0; i < C / 4; ++i) {
-                const int t = i * 4 + ow;
-                if (t >= n) break;
-                const float4 o = lds4(rows + t * (D * 4) + lane * 16);
-                const float4 z = four(p.in + (size_t)(row0 + t) * p.in_row + p.z_off + h * D + lane * 4, in_aligned);
-                const float ss = warp_sum(o.x * o.x + o.y * o.y + o.z * o.z + o.w * o.w);
-                const float r = rsqrtf(ss * (1.f / D) + p.eps);
-                const uint32_t lo = pack_bf16(o.x * r * gain.x * silu_of(z.x), o.y * r * gain.y * silu_of(z.y)), hi = pack_bf16(o.z * r * gain.z * silu_of(z.z), o.w * r * gain.w * silu_of(z.w));
-                __nv_bfloat16* dst = p.out + (size_t)(row0 + t) * p.out_row + h * D + lane * 4;
-                if (out_aligned) {
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-                } else {
-                    dst[0] = __ushort_as_bfloat16(lo & 0xffff); dst[1] = __ushort_as_bfloat16(lo >> 16);
-                    dst[2] = __ushort_as_bfloat16(hi & 0xffff); dst[3] = __ushort_as_bfloat16(hi >> 16);
+#pragma unroll
+            for (int i0 = 0; i0 < C / 4; i0 += 4) {         // four rows at a time: their sums go through the lanes together
+                float4 o[4];
+                float ss[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    o[k] = lds4(rows + ((i0 + k) * 4 + ow) * (D * 4) + lane * 16);
+                    ss[k] = o[k].x * o[k].x + o[k].y * o[k].y + o[k].z * o[k].z + o[k].w * o[k].w;
+                }
+#pragma unroll
+                for (int off = 16; off; off >>= 1)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) ss[k] += __shfl_xor_sync(0xffffffffu, ss[k], off);
+                uint2 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint2 g = z[i0 + k];
+                    const float r = rsqrtf(ss[k] * (1.f / D) + p.eps);
+                    v[k].x = pack_bf16(o[k].x * r * gain.x * silu(bf16_lo(g.x)), o[k].y * r * gain.y * silu(bf16_hi(g.x)));
+                    v[k].y = pack_bf16(o[k].z * r * gain.z * silu(bf16_lo(g.y)), o[k].w * r * gain.w * silu(bf16_hi(g.y)));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = (i0 + k) * 4 + ow;
+                    __nv_bfloat16* dst = p.out + (size_t)(row0 + t) * p.out_row + h * D + lane * 4;
+                    if (t < n && out_aligned) *reinterpret_cast<uint2*>(dst) = v[k];
+                    if (t < n && !out_aligned) {
+                        dst[0] = __ushort_as_bfloat16(v[k].x & 0xffff); dst[1] = __ushort_as_bfloat16(v[k].x >> 16);
+                        dst[2] = __ushort_as_bfloat16(v[k].y & 0xffff); dst[3] = __ushort_as_bfloat16(v[k].y >> 16);
+                    }
                 }
             }
         }
@@ -661,23 +842,29 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             // ------------------------------ products ------------------------------
             constexpr uint32_t MN = 1u << 16;               // right operand with its rows along K
             for (int c = 0; c < nc; ++c) {
-                const uint32_t key = stage(c), tri = key + ST_T, q = base + SM_Q, pt = base + SM_P;
+                uint32_t tm = tmem, sm = base;
+                asm volatile("" : "+r"(tm), "+r"(sm));      // addresses are added up where they are used, not kept from one chunk to the next
+                const uint32_t key = sm + (c & 1) * STAGE_BYTES, tri = key + ST_T, q = sm + SM_Q, pt = sm + SM_P;
                 if (!mbar_wait(bar(IN_FULL + (c & 1)), phase(c), abort_flag) || !mbar_wait(bar(S_RDY), c & 1, abort_flag)) break;
                 tc_fence_after();
+                // (a descriptor counts 16 bytes: what lies in one image is reached by addition)
                 auto with_rows = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {      // [128 columns x d] [64 rows x d]^T
+                    const uint64_t desc = smem_desc_sw128(img);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        mma_f16_ts(tmem + d, tmem + a + k * 8, smem_desc_sw128(img + (k >> 2) * (IMG / 2)) + 2 * (k & 3), idesc(C), !first_one || k > 0 ? 1u : 0u);
+                        mma_f16_ts(tm + d, tm + a + k * 8, desc + (k >> 2) * (IMG / 2 / 16) + 2 * (k & 3), idesc(C), !first_one || k > 0 ? 1u : 0u);
                 };
                 auto with_tri = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {       // [128 columns x 64 rows] times a lower triangle's transpose
+                    const uint64_t desc = smem_desc_sw128(img);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)             // columns in front of the diagonal's block are zero
-                        mma_f16_ts(tmem + d + 16 * k, tmem + a + k * 8, smem_desc_sw128(img + 16 * k * 128) + 2 * k, idesc(C - 16 * k), !first_one || k > 0 ? 1u : 0u);
+                        mma_f16_ts(tm + d + 16 * k, tm + a + k * 8, desc + k * (16 * 128 / 16) + 2 * k, idesc(C - 16 * k), !first_one || k > 0 ? 1u : 0u);
                 };
                 auto with_keys = [&](uint32_t a, uint32_t img, bool first_one) {                  // [128 columns x 64 rows] [64 rows x d]
+                    const uint64_t desc = smem_desc_mn_sw128(img, IMG / 2);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_f16_ts(tmem + T_DS, tmem + a + k * 8, smem_desc_mn_sw128(img + 16 * k * 128, IMG / 2), idesc(D) | MN, !first_one || k > 0 ? 1u : 0u);
+                        mma_f16_ts(tm + T_DS, tm + a + k * 8, desc + k * (16 * 128 / 16), idesc(D) | MN, !first_one || k > 0 ? 1u : 0u);
                 };
                 with_rows(T_KS, T_SHI, key, true);
                 with_rows(T_KS, T_SLO, key, false);
