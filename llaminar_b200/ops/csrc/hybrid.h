@@ -1,4 +1,5 @@
-// Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu, gdn_chunk.cu).
+// Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu, gdn_chunk.cu),
+// the rotation of a part of every head with the append to the paged cache (rope_part.cu).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -36,6 +37,27 @@ cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStrea
 size_t gdn_chunk_bytes(int units, int n_k, int n_v);
 cudaError_t launch_gdn_chunk(const GdnParams& p, void* workspace, size_t bytes, int* status, int& launches, cudaStream_t st);
 
+// Rows [(query, gate) per head | keys | values] -> normed and rotated queries, and the tokens' entries of the paged cache (bf16: [n_pages, 2, n_kv_heads, 64, head_dim];
+// 8-bit: as in AttnDecodeParams, ops.h)
+struct RopePartParams {
+    const __nv_bfloat16* rows; size_t row;                   // first row, values from one to the next
+    int whole;                                               // a lane's values may be loaded at once
+    int q_stride;                                            // values from a query head to the next: head_dim, or twice that with gates
+    const float *q_norm, *k_norm;                            // [head_dim] or nullptr
+    const double* freqs;                                     // [rot / 2], angle per position
+    float magnitude;
+    int rot, interleaved;
+    const int *positions, *seq_ids, *block_table;
+    int n_tokens, n_heads, n_kv_heads, head_dim, max_pages, n_seqs, n_pages;
+    __nv_bfloat16* q_out;                                    // [n_tokens, n_heads, head_dim]
+    uint8_t* kv; size_t page_bytes, scale_off;
+    int q8;
+    float eps;
+    int parts;                                               // warps that share a token (the launcher's choice)
+};
+cudaError_t launch_rope_part(const RopePartParams& p, cudaStream_t st);
+
+int bounds_status_rope_part(bool reset);
 int bounds_status_gdn_rows(bool reset);
 int bounds_status_gdn_chunk(bool reset);
 

@@ -4,6 +4,7 @@
 
 #include "binding_util.h"
 #include "hybrid.h"
+#include "launch.h"
 
 namespace {
 using namespace llm_binding;
@@ -122,6 +123,58 @@ void gdn_commit(const std::vector<Tensor>& keep, const Tensor& accepted, const T
     check(llm::launch_gdn_commit(p, n, stream()), "gdn_commit");
 }
 
+// A layer of the paged cache, bf16 or (`q8`) 8-bit
+void cache_args(const Tensor& like, const Tensor& kv, int64_t kv_heads, int64_t head_dim, uint8_t*& at, int& n_pages, size_t& page_bytes, size_t& scale_off, int& q8) {
+    same_device(like, kv, "kv");
+    TORCH_CHECK(kv.is_contiguous() && reinterpret_cast<uintptr_t>(kv.data_ptr()) % 16 == 0, "kv must be contiguous and 16-byte aligned");
+    scale_off = (size_t)2 * kv_heads * 64 * head_dim;
+    q8 = kv.scalar_type() == torch::kUInt8;
+    if (q8) {
+        page_bytes = scale_off + scale_off / 16;
+        TORCH_CHECK(kv.dim() == 2 && (size_t)kv.size(1) == page_bytes, "an 8-bit cache layer is [n_pages, bytes of a page of these heads]");
+    } else {
+        page_bytes = 2 * scale_off;
+        TORCH_CHECK(kv.scalar_type() == torch::kBFloat16, "the cache must be bf16 or 8-bit");
+        TORCH_CHECK(kv.dim() == 5 && kv.size(1) == 2 && kv.size(2) == kv_heads && kv.size(3) == 64 && kv.size(4) == head_dim, "a cache layer is [n_pages, 2, kv heads, 64, head size]");
+    }
+    at = static_cast<uint8_t*>(kv.data_ptr()); n_pages = kv.size(0);
+}
+const int* table_arg(const Tensor& like, const Tensor& t, int& n_seqs, int& max_pages) {
+    same_device(like, t, "block_table");
+    TORCH_CHECK(t.dim() == 2, "block_table must be [sequences, pages]");
+    n_seqs = t.size(0); max_pages = t.size(1);
+    return ints(t, "block_table");
+}
+
+void rope_part_kv(const Tensor& rows, const Tensor& q_out, const Tensor& kv, const OptTensor& q_norm, const OptTensor& k_norm, const Tensor& freqs, double magnitude,
+                  const Tensor& positions, const Tensor& seq_ids, const Tensor& block_table, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, double eps, bool gated, bool interleaved) {
+    llm::RopePartParams p = {};
+    p.rows = bf16_rows(rows, "rows");
+    TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head size must be 64, 128 or 256");
+    TORCH_CHECK(n_heads >= 1 && n_kv_heads >= 1 && n_heads <= 4096 && n_kv_heads <= 4096, "heads");
+    TORCH_CHECK(rows.size(1) == (n_heads * (gated ? 2 : 1) + 2 * n_kv_heads) * head_dim, "rows must be [query (and gate) per head | keys | values]");
+    const int64_t T = rows.size(0), lane = head_dim / 32;
+    TORCH_CHECK(T <= INT32_MAX, "too many rows");
+    p.row = rows.stride(0); p.q_stride = (gated ? 2 : 1) * head_dim;
+    p.whole = reinterpret_cast<uintptr_t>(rows.data_ptr()) % (2 * lane) == 0 && (T <= 1 || rows.stride(0) % lane == 0);
+    if (q_norm) p.q_norm = floats_on(rows, *q_norm, head_dim, "q_norm");
+    if (k_norm) p.k_norm = floats_on(rows, *k_norm, head_dim, "k_norm");
+    same_device(rows, freqs, "freqs");
+    want(freqs, torch::kFloat64, "freqs");
+    TORCH_CHECK(freqs.numel() * 2 <= head_dim, "more frequencies than a head has pairs");
+    p.freqs = freqs.data_ptr<double>(); p.rot = 2 * freqs.numel(); p.magnitude = magnitude; p.interleaved = interleaved;
+    p.positions = ints_on(rows, positions, T, "positions"); p.seq_ids = ints_on(rows, seq_ids, T, "seq_ids");
+    p.block_table = table_arg(rows, block_table, p.n_seqs, p.max_pages);
+    p.n_tokens = T; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.head_dim = head_dim; p.eps = eps;
+    same_device(rows, q_out, "q_out");
+    want(q_out, torch::kBFloat16, "q_out");
+    TORCH_CHECK(q_out.numel() == T * n_heads * head_dim && reinterpret_cast<uintptr_t>(q_out.data_ptr()) % 16 == 0, "q_out must be [rows, heads, head size], 16-byte aligned");
+    p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr());
+    cache_args(rows, kv, n_kv_heads, head_dim, p.kv, p.n_pages, p.page_bytes, p.scale_off, p.q8);
+    const c10::cuda::CUDAGuard guard(rows.device());
+    check(llm::launch_rope_part(p, stream()), "rope_part_kv");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -129,5 +182,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gdn_verify", &gdn_verify);
     m.def("gdn_commit", &gdn_commit);
     m.def("gdn_chunk_bytes", &llm::gdn_chunk_bytes);
-    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset) | llm::bounds_status_gdn_chunk(reset); });
+    m.def("rope_part_kv", &rope_part_kv);
+    m.def("set_pdl", [](bool on) { llm::pdl_enabled() = on; });
+    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset) | llm::bounds_status_gdn_chunk(reset) | llm::bounds_status_rope_part(reset); });
 }

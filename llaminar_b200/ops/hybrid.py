@@ -1,4 +1,4 @@
-"""Python surface of the hybrid extension (csrc/gdn_rows.cu, gdn_chunk.cu): the blocks of the Gated-DeltaNet family where
+"""Python surface of the hybrid extension (csrc/gdn_rows.cu, gdn_chunk.cu, rope_part.cu): the blocks of the Gated-DeltaNet family where
 a step has more than one new row per sequence.
 
 As in :mod:`llaminar_b200.ops`, every call launches hand-written CUDA on the current stream; there is no fallback.  Arguments are checked
@@ -15,8 +15,17 @@ from . import _count, scratch_for
 from . import build as _build
 
 
+_ready = False
+
+
 def ext():
-    return _build.load(_build.HYBRID)
+    global _ready
+    mod = _build.load(_build.HYBRID)
+    if not _ready:
+        from ..utils.env import debug_env
+        mod.set_pdl(bool(debug_env().pdl))
+        _ready = True
+    return mod
 
 
 GDN_CHUNK = 64                 # rows of a chunk
@@ -76,6 +85,19 @@ def gdn_verify(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torch
 def gdn_commit(stash: GdnStash, n_rows: torch.Tensor, conv_state: torch.Tensor, rec: torch.Tensor) -> None:
     """Advance the state of every sequence of ``stash`` by its first n_rows[b] rows (int32 on the device; 0 leaves it as it is)."""
     ext().gdn_commit([stash.decay, stash.key, stash.correction, stash.inputs], n_rows, conv_state, rec, stash.slots, stash.n_k)
+    _count()
+
+
+def rope_part_kv(rows: torch.Tensor, q_out: torch.Tensor, kv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor | None, freqs: torch.Tensor,
+                 magnitude: float, positions: torch.Tensor, seq_ids: torch.Tensor, block_table: torch.Tensor, n_heads: int, n_kv_heads: int,
+                 head_dim: int, eps: float, *, gated: bool = False, interleaved: bool = False) -> None:
+    """Projected rows [query per head | keys | values], with ``gated`` [(query, gate) per head | keys | values] -> queries q_out [tokens, heads, head size] and the
+    tokens' entries of the paged cache ``kv`` (bf16, or 8-bit as in `rope_kv`).  Queries and keys are RMS-normed per head (gains of a head, or None: as they
+    are), then the first 2 len(freqs) values turn by position x freqs (float64, on the device; `Rotary.frequencies` has them for plain and
+    scaled rotations), pairs (i, i + len(freqs)) or, ``interleaved``, (2i, 2i + 1), times ``magnitude``; the rest passes.  Head sizes 64, 128 and 256;
+    positions are not negative and their page is in block_table[seq_ids[t]]."""
+    ext().rope_part_kv(rows, q_out, kv, q_norm, k_norm, freqs, float(magnitude), positions, seq_ids, block_table, n_heads, n_kv_heads, head_dim, eps,
+                       bool(gated), bool(interleaved))
     _count()
 
 

@@ -38,3 +38,27 @@ def gdn_rows(inp, first, rows, start_conv, start_rec, conv_w, ssm_a, dt_bias, no
             out[t, h * d:(h + 1) * d] = o / math.sqrt(float((o * o).mean()) + eps) * g * gate / (1 + torch.exp(-gate))
         states.append((win.clone(), S.clone()))
     return out, states
+
+
+def rope_part(rows, n_heads, n_kv_heads, D, q_norm, k_norm, freqs, magnitude, positions, eps, gated, interleaved):
+    """Rows -> (queries [T, H, D], keys [T, Hk, D], values [T, Hk, D])."""
+    T, per = rows.shape[0], 2 if gated else 1
+    x = rows.to(F64).reshape(T, n_heads * per + 2 * n_kv_heads, D)
+    q, k, v = x[:, :n_heads * per:per], x[:, n_heads * per:n_heads * per + n_kv_heads], x[:, n_heads * per + n_kv_heads:]
+    n = freqs.numel()
+
+    def turn(h, gain):
+        h = h.clone()
+        if gain is not None:
+            h = h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * gain.to(F64)
+        out = h.clone()
+        for t in range(T):
+            for i in range(n):
+                a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + n)
+                ang = float(positions[t]) * float(freqs[i])
+                c, s = magnitude * math.cos(ang), magnitude * math.sin(ang)
+                out[t, :, a] = h[t, :, a] * c - h[t, :, b] * s
+                out[t, :, b] = h[t, :, b] * c + h[t, :, a] * s
+        return out
+
+    return turn(q, q_norm), turn(k, k_norm), v

@@ -193,3 +193,117 @@ def test_gdn_calls_refuse_what_they_cannot_take():
     ops.gdn_prefill(**{**good, "inp": good["inp"][:0], "out": good["out"][:0], "positions": good["positions"][:0], "cu": it([0, 0])})
     ops.gdn_prefill(**{**good, "cu": it([0]), "slots": it([])})
     torch.cuda.synchronize()
+
+
+# -- rotation of a part of every head with the append ---------------------------------------------------------------------
+
+ROPE = [
+    # heads, kv heads, head size, pairs, gated, interleaved, norms, tokens per sequence, first positions
+    (6, 2, 64, 8, True, False, True, [1], [0]),
+    (4, 1, 64, 32, False, True, False, [5, 70], [0, 63]),
+    (8, 8, 128, 64, False, False, True, [3, 1, 130], [200000, 7, 100]),
+    (7, 1, 128, 16, True, True, True, [64], [64]),
+    (24, 4, 256, 32, True, False, True, [1] * 9, [131071, 0, 1, 62, 63, 64, 65, 999, 262143]),
+    (3, 1, 256, 128, False, False, True, [2], [50]),
+    (2, 2, 256, 5, True, False, True, [9], [120]),             # halves that end inside a lane's values
+    (5, 1, 128, 3, False, False, False, [3], [61]),
+    (2, 1, 64, 0, False, False, True, [4], [10]),              # nothing turns
+    (16, 2, 256, 32, True, False, True, [2500], [30]),         # a warp per token
+]
+
+
+@pytest.mark.parametrize("H,Hk,D,n,gated,interleaved,norms,lens,first", ROPE)
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("odd_rows", [False, True])
+def test_rope_part_kv_follows_the_definition(H, Hk, D, n, gated, interleaved, norms, lens, first, q8, odd_rows):
+    """Queries and bf16 entries: half a step, 2^-8 of the value, behind sums of D squares and a few products in 32 bits (an angle is 2^-22 off at most).  8-bit
+    entries: half a step of the scale, which is the largest of 32 values / 127 rounded up by up to 2^-7."""
+    from llaminar_b200 import ops
+    if sum(lens) > 300 and odd_rows:
+        pytest.skip("one form of the long case")
+    g = torch.Generator().manual_seed(H * D + n)
+    T, B = sum(lens), len(lens)
+    width = (H * (2 if gated else 1) + 2 * Hk) * D
+    buf = torch.randn(T, width + (1 if odd_rows else 0), generator=g).to(torch.bfloat16)
+    q_norm, k_norm = (torch.rand(D, generator=g) + 0.5, torch.rand(D, generator=g) + 0.5) if norms else (None, None)
+    freqs, magnitude = 1e6 ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)), 1.25
+    pos = [f + t for f, k in zip(first, lens) for t in range(k)]
+    sid = [b for b, k in enumerate(lens) for _ in range(k)]
+    used = sorted({(b, p // 64) for b, p in zip(sid, pos)})
+    table = torch.zeros(B, max(p for _, p in used) + 1, dtype=torch.int32)
+    ids = (torch.randperm(len(used), generator=g) + 1).tolist()
+    for (b, p), i in zip(used, ids):
+        table[b, p] = i
+    n_pages = len(used) + 1
+    kv = torch.zeros(n_pages, 2, Hk, 64, D, dtype=torch.bfloat16, device=DEV) if not q8 else torch.zeros(n_pages, 2 * Hk * 64 * D * 17 // 16, dtype=torch.uint8, device=DEV)
+    q_out = torch.zeros(T, H, D, dtype=torch.bfloat16, device=DEV)
+    dev = lambda x: None if x is None else x.to(DEV)
+    ops.rope_part_kv(buf.to(DEV)[:, :width], q_out, kv, dev(q_norm), dev(k_norm), freqs.to(DEV), magnitude, torch.tensor(pos, dtype=torch.int32, device=DEV),
+                     torch.tensor(sid, dtype=torch.int32, device=DEV), table.to(DEV), H, Hk, D, EPS, gated=gated, interleaved=interleaved)
+    torch.cuda.synchronize()
+    if T > 300:                                                  # the oracle goes pair by pair: the first, the last and some between
+        some = [0, 1, 77, 1300, T - 1]
+    else:
+        some = list(range(T))
+    q, k, v = oracle.rope_part(buf[some][:, :width], H, Hk, D, q_norm, k_norm, freqs, magnitude, [pos[t] for t in some], EPS, gated, interleaved)
+    close = lambda got, want: ((got.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 64 * 2.0 ** -24 * want.abs().amax(-1, keepdim=True) + 1e-30).all()
+    assert close(q_out[some], q)
+    page = torch.tensor([int(table[sid[t], pos[t] // 64]) for t in some])
+    off = torch.tensor([pos[t] % 64 for t in some])
+    if not q8:
+        assert close(kv[page.to(DEV), 0, :, off.to(DEV)], k) and close(kv[page.to(DEV), 1, :, off.to(DEV)], v)
+        mask = torch.zeros(n_pages, 64, dtype=torch.bool)
+        for t in range(T):
+            mask[int(table[sid[t], pos[t] // 64]), pos[t] % 64] = True
+        assert (kv.cpu().permute(0, 3, 1, 2, 4)[~mask] == 0).all()       # nothing else was written
+    else:
+        raw = kv.cpu()
+        data = raw[:, :2 * Hk * 64 * D].contiguous().view(torch.int8).view(n_pages, 2, Hk, 64, D)[page, :, :, off].double()
+        sc = raw[:, 2 * Hk * 64 * D:].contiguous().view(torch.float16).view(n_pages, 2, Hk, 64, D // 32)[page, :, :, off].double()
+        for i, want in enumerate((k, v)):
+            blocks = want.unflatten(-1, (-1, 32))
+            top = blocks.abs().amax(-1) / 127
+            assert (sc[:, i] >= top * (1 - 2.0 ** -11) - 2.0 ** -24).all() and (sc[:, i] <= top * (1 + 2.0 ** -6) + 2.0 ** -24).all()
+            err = (data[:, i].unflatten(-1, (-1, 32)) * sc[:, i, ..., None] - blocks).abs()
+            assert (err <= sc[:, i, ..., None] * (0.5 + 2.0 ** -10)).all()
+
+
+def test_rope_part_kv_writes_what_rope_kv_writes_for_whole_heads():
+    """Both pages and queries of whole, plain rotations agree with the operator beside it to a step of the type (its angles are 32-bit)."""
+    from llaminar_b200 import ops
+    H, Hk, D, T = 8, 2, 128, 100
+    g = torch.Generator(device=DEV).manual_seed(5)
+    qkv = torch.randn(T, (H + 2 * Hk) * D, device=DEV, generator=g).to(torch.bfloat16)
+    norm = torch.rand(D, device=DEV, generator=g) + 0.5
+    pos, sid = torch.arange(T, dtype=torch.int32, device=DEV), torch.zeros(T, dtype=torch.int32, device=DEV)
+    table = torch.tensor([[2, 1]], dtype=torch.int32, device=DEV)
+    got = []
+    for kv in (torch.zeros(3, 2, Hk, 64, D, dtype=torch.bfloat16, device=DEV), torch.zeros(3, 2, Hk, 64, D, dtype=torch.bfloat16, device=DEV)):
+        q = torch.zeros(T, H, D, dtype=torch.bfloat16, device=DEV)
+        if not got:
+            ops.rope_kv(qkv, q, kv, norm, norm, pos, sid, table, H, Hk, D, 1e6, EPS)
+        else:
+            ops.rope_part_kv(qkv, q, kv, norm, norm, 1e6 ** (-torch.arange(0, D, 2, dtype=torch.float64, device=DEV) / D), 1.0, pos, sid, table, H, Hk, D, EPS)
+        got.append((q.float(), kv.float()))
+    for a, b in zip(*got):
+        assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 2.0 ** -12).all()
+
+
+def test_rope_part_kv_refuses_what_it_cannot_take():
+    from llaminar_b200 import ops
+    H, Hk, D, T = 2, 1, 64, 3
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    good = dict(rows=torch.zeros(T, 4 * D, dtype=torch.bfloat16, device=DEV), q_out=torch.zeros(T, H, D, dtype=torch.bfloat16, device=DEV),
+                kv=torch.zeros(2, 2, Hk, 64, D, dtype=torch.bfloat16, device=DEV), q_norm=torch.ones(D, device=DEV), k_norm=None,
+                freqs=torch.ones(8, dtype=torch.float64, device=DEV), magnitude=1.0, positions=it([0, 1, 2]), seq_ids=it([0, 0, 0]), block_table=it([[1]]),
+                n_heads=H, n_kv_heads=Hk, head_dim=D, eps=EPS)
+    ops.rope_part_kv(**good)
+    for change in (dict(rows=good["rows"].float()), dict(rows=good["rows"][:, :-1]), dict(rows=good["rows"].cpu()), dict(gated=True), dict(q_out=good["q_out"][:2]),
+                   dict(q_out=good["q_out"].transpose(0, 1)), dict(kv=good["kv"].half()), dict(kv=good["kv"][:, :, :, :32]), dict(kv=torch.zeros(2, 100, dtype=torch.uint8, device=DEV)),
+                   dict(q_norm=torch.ones(D - 1, device=DEV)), dict(k_norm=torch.ones(D, device=DEV, dtype=torch.float64)), dict(freqs=good["freqs"].float()),
+                   dict(freqs=torch.ones(33, dtype=torch.float64, device=DEV)), dict(positions=it([0, 1])), dict(seq_ids=good["seq_ids"].long()), dict(block_table=it([1])),
+                   dict(n_heads=0), dict(head_dim=48), dict(n_kv_heads=2)):
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.rope_part_kv(**{**good, **change})
+    ops.rope_part_kv(**{**good, "rows": good["rows"][:0], "q_out": good["q_out"][:0], "positions": it([]), "seq_ids": it([])})
+    torch.cuda.synchronize()
