@@ -18,8 +18,34 @@ namespace llm {
 
 constexpr int PAGE = 64, WARPS = 4;
 
+// two numbers at a time
+typedef unsigned long long f32x2;
+LLM_DEVICE f32x2 pair(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+LLM_DEVICE float2 both(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
 // N bf16 values as they lie in memory (N = 2, 4, 8)
-template <int N> struct Raw { uint32_t w[N / 2]; };
+template <int N> struct Raw {
+    uint32_t w[N / 2];
+    LLM_DEVICE f32x2 two(int i) const { return pair(bf16_lo(w[i]), bf16_hi(w[i])); }
+};
 template <int N> LLM_DEVICE Raw<N> load_raw(const __nv_bfloat16* x, bool whole) {
     Raw<N> r;
     if (!whole) {
@@ -36,19 +62,39 @@ template <int N> LLM_DEVICE Raw<N> load_raw(const __nv_bfloat16* x, bool whole) 
     }
     return r;
 }
-template <int N> LLM_DEVICE void store_raw(__nv_bfloat16* x, const float (&v)[N]) {        // aligned: the caches and the queries are dense
-    uint32_t w[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (N == 8) *reinterpret_cast<uint4*>(x) = make_uint4(w[0], w[1 % (N / 2)], w[2 % (N / 2)], w[3 % (N / 2)]);
-    else if (N == 4) *reinterpret_cast<uint2*>(x) = make_uint2(w[0], w[1 % (N / 2)]);
-    else *reinterpret_cast<uint32_t*>(x) = w[0];
+template <int N> LLM_DEVICE void store_raw(__nv_bfloat16* x, const Raw<N>& r) {            // aligned: the caches and the queries are dense
+    if (N == 8) *reinterpret_cast<uint4*>(x) = make_uint4(r.w[0], r.w[1 % (N / 2)], r.w[2 % (N / 2)], r.w[3 % (N / 2)]);
+    else if (N == 4) *reinterpret_cast<uint2*>(x) = make_uint2(r.w[0], r.w[1 % (N / 2)]);
+    else *reinterpret_cast<uint32_t*>(x) = r.w[0];
 }
 
-// D / 32 values a lane, BATCH heads at a time
-template <int D, int BATCH>
-__global__ void __launch_bounds__(32 * WARPS) rope_part_kernel(const RopePartParams p) {
+// sums of B values over a warp, as reciprocal roots of their means.  Four go through the lanes together: each step halves what a lane carries
+// on, so that four sums take 10 exchanges and one root instead of 20 and four.
+template <int B> LLM_DEVICE void roots(float (&ss)[B], float scale, float eps) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (B == 4) {
+        const bool up = lane & 16, up2 = lane & 8;
+        const float x0 = (up ? ss[2] : ss[0]) + __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[2], 16), x1 = (up ? ss[3] : ss[1]) + __shfl_xor_sync(0xffffffffu, up ? ss[1] : ss[3], 16);
+        float z = (up2 ? x1 : x0) + __shfl_xor_sync(0xffffffffu, up2 ? x0 : x1, 8);
+        z += __shfl_xor_sync(0xffffffffu, z, 4);
+        z += __shfl_xor_sync(0xffffffffu, z, 2);
+        z += __shfl_xor_sync(0xffffffffu, z, 1);
+        const float r = rsqrtf(z * scale + eps);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss[j] = __shfl_sync(0xffffffffu, r, (j >> 1) * 16 + (j & 1) * 8);
+    } else {
+#pragma unroll
+        for (int j = 0; j < B; ++j) ss[j] = rsqrtf(warp_sum(ss[j]) * scale + eps);
+    }
+}
+
+// One value becomes own * gain * cos +- partner * gain of the partner * sin, all times the head's reciprocal root: gains and angles are multiplied once per
+// token, and the partners come as they were loaded, two values a word.  D / 32 values a lane, BATCH heads at a time, the next ones on their way.
+// ODD: halves that end inside a lane's values.
+template <int D, int BATCH, bool ODD>
+__global__ void __launch_bounds__(32 * WARPS, ODD ? 1 : D == 256 ? 4 : 6) rope_part_kernel(const RopePartParams p) {
     constexpr int N = D / 32;
+    __shared__ float2 s_angles[WARPS][D / 2];
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, item = blockIdx.x * WARPS + (threadIdx.x >> 5);
@@ -56,21 +102,38 @@ __global__ void __launch_bounds__(32 * WARPS) rope_part_kernel(const RopePartPar
     const int t = item / p.parts, part = item - t * p.parts;
     const int heads = p.n_heads + 2 * p.n_kv_heads, per = (heads + p.parts - 1) / p.parts;
     const int h0 = part * per, h1 = min(heads, h0 + per);
+    if (h0 >= h1) return;
     const int pos = p.positions[t], half = p.rot / 2, i0 = lane * N;
     const __nv_bfloat16* row = p.rows + (size_t)t * p.row + i0;
     auto source = [&](int h) { return row + (size_t)(h < p.n_heads ? h * p.q_stride : p.n_heads * p.q_stride + (h - p.n_heads) * D); };
-    float cs[N], sn[N];
+    Raw<N> next[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) next[j] = load_raw<N>(source(min(h0 + j, h1 - 1)), p.whole);
+    float cs[N], sn[N];                                      // with the sign that the partner has
+    uint32_t turns[N / 2];                                   // the words' values that turn, as a mask
+    auto partner_of = [&](int i) { return i >= p.rot ? i : p.interleaved ? i ^ 1 : i < half ? i + half : i - half; };
     if (h0 < p.n_heads + p.n_kv_heads) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int i = i0 + e, pair = p.interleaved ? i >> 1 : i < half ? i : i - half;
-            cs[e] = 1.f; sn[e] = 0.f;
-            if (i >= p.rot) continue;
-            if (p.interleaved && (e & 1)) { cs[e] = cs[e - 1]; sn[e] = sn[e - 1]; continue; }
-            const double turns = (double)pos * p.freqs[pair] * 0.15915494309189533577;
+        for (int k = 0; k < N / 2; ++k) {                    // a lane forms the angles of every 32nd pair
+            const int i = k * 32 + lane;
+            if (i >= half) break;
+            const double x = (double)pos * p.freqs[i] * 0.15915494309189533577;       // in turns
             float s, c;
-            sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-            cs[e] = c * p.magnitude; sn[e] = s * p.magnitude;
+            sincospif(2.f * (float)(x - rint(x)), &s, &c);
+            s_angles[threadIdx.x >> 5][i] = make_float2(c * p.magnitude, s * p.magnitude);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int i = i0 + e;
+            const bool first = p.interleaved ? !(e & 1) : i < half;
+            const int index = p.interleaved ? i >> 1 : first ? i : i - half;
+            cs[e] = 1.f; sn[e] = 0.f;
+            if (e % 2 == 0) turns[e / 2] = 0;
+            if (i >= p.rot) continue;
+            turns[e / 2] |= e % 2 ? 0xffff0000u : 0xffffu;
+            const float2 x = s_angles[threadIdx.x >> 5][index];
+            cs[e] = x.x; sn[e] = first ? -x.y : x.y;
         }
     }
     uint8_t* page = nullptr;
@@ -78,99 +141,141 @@ __global__ void __launch_bounds__(32 * WARPS) rope_part_kernel(const RopePartPar
         const int seq = LLM_CHECK_INDEX(p.seq_ids[t], p.n_seqs), slot = LLM_CHECK_INDEX(pos / PAGE, p.max_pages);
         page = p.kv + (size_t)LLM_CHECK_INDEX(p.block_table[(size_t)seq * p.max_pages + slot], p.n_pages) * p.page_bytes;
     }
-    for (int b0 = h0; b0 < h1; b0 += BATCH) {
-        Raw<N> raw[BATCH];
+
+    // heads [a, b) of one kind (0: queries, 1: keys, 2: values); the first batch is in `next`, the last one leaves what comes behind b there
+    auto heads_of = [&](int a, int b, int kind) {
+        const float* gain = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
+        f32x2 own[N / 2], partner[N / 2];
+        if (kind < 2) {
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) raw[j] = load_raw<N>(source(min(b0 + j, h1 - 1)), p.whole);
+            for (int e = 0; e < N; e += 2) {
+                own[e / 2] = pair(cs[e] * (gain ? gain[i0 + e] : 1.f), cs[e + 1] * (gain ? gain[i0 + e + 1] : 1.f));
+                partner[e / 2] = pair(sn[e] * (gain ? gain[partner_of(i0 + e)] : 1.f), sn[e + 1] * (gain ? gain[partner_of(i0 + e + 1)] : 1.f));
+            }
+        }
+        for (int b0 = a; b0 < b; b0 += BATCH) {
+            Raw<N> raw[BATCH];
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            const int h = b0 + j;
-            if (h >= h1) break;
-            const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv_heads;
-            float x[N];
+            for (int j = 0; j < BATCH; ++j) raw[j] = next[j];
+            const int n0 = min(b0 + BATCH, b);               // kinds begin a batch of their own
+            if (n0 < h1) {
 #pragma unroll
-            for (int e = 0; e < N; e += 2) { x[e] = bf16_lo(raw[j].w[e / 2]); x[e + 1] = bf16_hi(raw[j].w[e / 2]); }
-            if (is_q || is_k) {
-                const float* gain = is_q ? p.q_norm : p.k_norm;
-                if (gain) {
-                    float ss = 0.f;
+                for (int j = 0; j < BATCH; ++j) next[j] = load_raw<N>(source(min(n0 + j, h1 - 1)), p.whole);
+            }
+            float r[BATCH];
+            if (gain) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) ss += x[e] * x[e];
-                    const float r = rsqrtf(warp_sum(ss) / D + p.eps);
+                for (int j = 0; j < BATCH; ++j) {
+                    f32x2 ss = pair(0.f, 0.f);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) x[e] *= r * gain[i0 + e];
+                    for (int e = 0; e < N / 2; ++e) ss = fma2(raw[j].two(e), raw[j].two(e), ss);
+                    const float2 x = both(ss);
+                    r[j] = x.x + x.y;
                 }
-                float y[N];                                  // the partners
-                if (p.interleaved) {
+                roots<BATCH>(r, 1.f / D, p.eps);
+            }
 #pragma unroll
-                    for (int e = 0; e < N; e += 2) { y[e] = -x[e + 1]; y[e + 1] = x[e]; }
-                } else if (half % N == 0) {
-                    const int from = i0 < half ? lane + half / N : lane - half / N;
+            for (int j = 0; j < BATCH; ++j) {
+                const int h = b0 + j;
+                if (h >= b) break;
+                f32x2 y[N / 2];
+                if (kind < 2) {
+                    Raw<N> x;
+                    if (p.interleaved) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float v = __shfl_sync(0xffffffffu, x[e], from & 31);
-                        y[e] = i0 < half ? -v : v;
-                    }
-                } else {                                     // a part whose halves end inside a lane's values
+                        for (int e = 0; e < N / 2; ++e) x.w[e] = __byte_perm(raw[j].w[e], 0, 0x1032);
+                    } else if (!ODD) {                       // a lane's partners are the neighbours of one another
+                        const int lane_of = partner_of(i0) / N;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const int i = i0 + e, from = i < half ? i + half : i - half;
-                        y[e] = 0.f;
+                        for (int e = 0; e < N / 2; ++e) x.w[e] = __shfl_sync(0xffffffffu, raw[j].w[e], lane_of);
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < N; ++k) {
-                            const float v = __shfl_sync(0xffffffffu, x[k], (from / N) & 31);
-                            if (from % N == k) y[e] = i < half ? -v : v;
+                        for (int e = 0; e < N; ++e) {
+                            const int from = partner_of(i0 + e);
+                            uint32_t v = 0;
+#pragma unroll
+                            for (int k = 0; k < N / 2; ++k) {
+                                const uint32_t w = __shfl_sync(0xffffffffu, raw[j].w[k], from / N);
+                                if (from % N / 2 == k) v = w;
+                            }
+                            v = from & 1 ? v >> 16 : v & 0xffffu;
+                            x.w[e / 2] = e & 1 ? x.w[e / 2] | v << 16 : v;
                         }
                     }
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) {
+                        x.w[e] &= turns[e];                  // what passes meets no partner (an infinity times 0 is not 0)
+                        y[e] = fma2(x.two(e), partner[e], mul2(raw[j].two(e), own[e]));
+                        if (gain) y[e] = mul2(y[e], pair(r[j], r[j]));
+                    }
+                    if (kind == 0 || !p.q8) {
+#pragma unroll
+                        for (int e = 0; e < N / 2; ++e) {
+                            const float2 v = both(y[e]);
+                            raw[j].w[e] = pack_bf16(v.x, v.y);
+                        }
+                    }
+                } else if (p.q8) {
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) y[e] = raw[j].two(e);
+                }
+                if (kind == 0) {
+                    store_raw<N>(p.q_out + ((size_t)t * p.n_heads + h) * D + i0, raw[j]);
+                    continue;
+                }
+                const size_t at = ((size_t)(kind - 1) * p.n_kv_heads + (h - p.n_heads - (kind - 1) * p.n_kv_heads)) * PAGE + pos % PAGE;
+                if (!p.q8) {
+                    store_raw<N>(reinterpret_cast<__nv_bfloat16*>(page) + at * D + i0, raw[j]);
+                    continue;
+                }
+                // 8-bit: largest magnitude of the 32 values / 127, rounded up to seven bits behind the point (no value clips; see rope_kv for why seven)
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e) {
+                    const float2 v = both(y[e]);
+                    top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (i0 + e < p.rot) x[e] = x[e] * cs[e] + y[e] * sn[e];
-            }
-            if (is_q) {
-                store_raw<N>(p.q_out + ((size_t)t * p.n_heads + h) * D + i0, x);
-                continue;
-            }
-            const size_t at = ((size_t)(is_k ? 0 : 1) * p.n_kv_heads + (is_k ? h - p.n_heads : h - p.n_heads - p.n_kv_heads)) * PAGE + pos % PAGE;
-            if (!p.q8) {
-                store_raw<N>(reinterpret_cast<__nv_bfloat16*>(page) + at * D + i0, x);
-                continue;
-            }
-            // 8-bit: largest magnitude of the 32 values / 127, rounded up to seven bits behind the point (no value clips; see rope_kv for why seven)
-            float top = 0.f;
+                for (int o = 1; o < 32 / N; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const __half hs = __float2half_rn(__uint_as_float((__float_as_uint(top * (1.0f / 127.0f)) + 0xFFFFu) & 0xFFFF0000u));
+                const float s = __half2float(hs), inv = s > 0.f ? 1.0f / s : 0.f;
+                uint32_t w[2] = {0u, 0u};
 #pragma unroll
-            for (int e = 0; e < N; ++e) top = fmaxf(top, fabsf(x[e]));
-#pragma unroll
-            for (int o = 1; o < 32 / N; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const __half hs = __float2half_rn(__uint_as_float((__float_as_uint(top * (1.0f / 127.0f)) + 0xFFFFu) & 0xFFFF0000u));
-            const float s = __half2float(hs), inv = s > 0.f ? 1.0f / s : 0.f;
-            uint32_t w[2] = {0u, 0u};
-#pragma unroll
-            for (int e = 0; e < N; ++e) w[e / 4] |= (uint32_t)(uint8_t)(int8_t)max(-127, min(127, __float2int_rn(x[e] * inv))) << (8 * (e & 3));
-            uint8_t* d8 = page + at * D + i0;
-            if (N == 8) *reinterpret_cast<uint2*>(d8) = make_uint2(w[0], w[1]);
-            else if (N == 4) *reinterpret_cast<uint32_t*>(d8) = w[0];
-            else *reinterpret_cast<unsigned short*>(d8) = (unsigned short)w[0];
-            if ((lane & (32 / N - 1)) == 0) reinterpret_cast<__half*>(page + p.scale_off)[at * (D / 32) + i0 / 32] = hs;
+                for (int e = 0; e < N; ++e) {
+                    const float2 v = both(y[e / 2]);
+                    w[e / 4] |= (uint32_t)(uint8_t)(int8_t)max(-127, min(127, __float2int_rn((e & 1 ? v.y : v.x) * inv))) << (8 * (e & 3));
+                }
+                uint8_t* d8 = page + at * D + i0;
+                if (N == 8) *reinterpret_cast<uint2*>(d8) = make_uint2(w[0], w[1]);
+                else if (N == 4) *reinterpret_cast<uint32_t*>(d8) = w[0];
+                else *reinterpret_cast<unsigned short*>(d8) = (unsigned short)w[0];
+                if ((lane & (32 / N - 1)) == 0) reinterpret_cast<__half*>(page + p.scale_off)[at * (D / 32) + i0 / 32] = hs;
+            }
         }
-    }
+    };
+    const int q1 = min(h1, p.n_heads), k1 = min(h1, p.n_heads + p.n_kv_heads);
+    if (h0 < q1) heads_of(h0, q1, 0);
+    if (max(h0, q1) < k1) heads_of(max(h0, q1), k1, 1);
+    if (max(h0, k1) < h1) heads_of(max(h0, k1), h1, 2);
 }
 
 cudaError_t launch_rope_part(const RopePartParams& args, cudaStream_t st) {
     RopePartParams p = args;
     if (p.n_tokens == 0) return cudaSuccess;
     const int heads = p.n_heads + 2 * p.n_kv_heads;
-    // a warp takes all heads of a token where the tokens fill the GPU's warps, else the heads are shared out
+    // A warp takes all heads of a token where the tokens give every SM `per_sm` warps, else the heads are shared out; up to eight heads go one at a time.
+    const int per_sm = p.head_dim == 256 ? 8 : 16;
     p.parts = 1;
-    while ((long long)p.n_tokens * p.parts < 148 * 16 && p.parts < heads) p.parts *= 2;
+    while ((long long)p.n_tokens * p.parts < 148 * per_sm && p.parts < heads) p.parts *= 2;
     if (p.parts > heads) p.parts = heads;
     const long long ctas = ((long long)p.n_tokens * p.parts + WARPS - 1) / WARPS;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-    const bool few = (heads + p.parts - 1) / p.parts < 4;
-    auto go = [&](auto one, auto many) { return launch_pdl(few ? one : many, dim3((unsigned)ctas), dim3(32 * WARPS), 0, st, p); };
-    if (p.head_dim == 64) return go(rope_part_kernel<64, 1>, rope_part_kernel<64, 4>);
-    if (p.head_dim == 128) return go(rope_part_kernel<128, 1>, rope_part_kernel<128, 4>);
-    if (p.head_dim == 256) return go(rope_part_kernel<256, 1>, rope_part_kernel<256, 4>);
+    const bool few = (heads + p.parts - 1) / p.parts <= 8;
+    const bool odd = !p.interleaved && p.rot / 2 % (p.head_dim / 32);
+    auto go = [&](auto one, auto many, auto any) { return launch_pdl(odd ? any : few ? one : many, dim3((unsigned)ctas), dim3(32 * WARPS), 0, st, p); };
+    if (p.head_dim == 64) return go(rope_part_kernel<64, 1, false>, rope_part_kernel<64, 4, false>, rope_part_kernel<64, 1, true>);
+    if (p.head_dim == 128) return go(rope_part_kernel<128, 1, false>, rope_part_kernel<128, 4, false>, rope_part_kernel<128, 1, true>);
+    if (p.head_dim == 256) return go(rope_part_kernel<256, 1, false>, rope_part_kernel<256, 4, false>, rope_part_kernel<256, 1, true>);
     return cudaErrorInvalidValue;
 }
 
