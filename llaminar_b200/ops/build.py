@@ -25,7 +25,7 @@ SOURCES = {
     GROUPED: ["grouped_binding.cpp", "grouped.cu", "attention.cu", "attention_tc.cu"],
     MIXERS: ["mixers_binding.cpp", "mixers.cu", "linear_tc.cu"],
     EXPERTS: ["experts_binding.cpp", "experts.cu", "experts_tc.cu"],
-    HYBRID: ["hybrid_binding.cpp", "gdn_rows.cu", "gdn_chunk.cu", "rope_part.cu"],
+    HYBRID: ["hybrid_binding.cpp", "gdn_rows.cu", "gdn_chunk.cu", "rope_part.cu", "attn_shared.cu"],
 }
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--expt-relaxed-constexpr", "-Xptxas", "-v"]

@@ -1,5 +1,6 @@
 // Launchers of the hybrid family's blocks: the gated delta rule over several rows of every sequence (gdn_rows.cu, gdn_chunk.cu),
-// the rotation of a part of every head with the append to the paged cache (rope_part.cu).
+// the rotation of a part of every head with the append to the paged cache (rope_part.cu); and decode attention of a batch behind a shared prefix
+// (attn_shared.cu).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -57,6 +58,23 @@ struct RopePartParams {
 };
 cudaError_t launch_rope_part(const RopePartParams& p, cudaStream_t st);
 
+struct AttnSharedParams {
+    const __nv_bfloat16 *q, *kv;   // [n_seqs * rows_per_seq, n_heads, head_dim], [n_pages, 2, n_kv_heads, 64, head_dim]
+    __nv_bfloat16* out;            // as q
+    const int *block_table, *seq_lens, *shared_len;          // [n_seqs, max_pages], [n_seqs], one number
+    int n_seqs, rows_per_seq, n_heads, n_kv_heads, head_dim, max_pages, n_pages;
+    int prefix_row;                // row of block_table whose first pages are the prefix
+    float scale;
+    const __nv_bfloat16* gate; size_t gate_token, gate_head;         // optional: values from a token / a head to the next
+    int splits, tail_splits;       // parts of the prefix's keys (0: no prefix) and of a tail's
+    float *part_o, *part_ml, *tail_o, *tail_ml;              // rows of the plan: head_dim values; maximum and sum
+    unsigned* tickets;             // [n_seqs * n_kv_heads], zero between calls (more than one part)
+};
+struct AttnSharedPlan { int splits, tail_splits; long long prefix_rows, tail_rows; };
+AttnSharedPlan attn_shared_plan(int n_seqs, int rows_per_seq, int n_heads, int n_kv_heads, int head_dim, int max_shared, int max_tail, int max_tickets);
+cudaError_t launch_attn_shared(const AttnSharedParams& p, int* status, cudaStream_t st);
+
+int bounds_status_attn_shared(bool reset);
 int bounds_status_rope_part(bool reset);
 int bounds_status_gdn_rows(bool reset);
 int bounds_status_gdn_chunk(bool reset);

@@ -175,6 +175,58 @@ void rope_part_kv(const Tensor& rows, const Tensor& q_out, const Tensor& kv, con
     check(llm::launch_rope_part(p, stream()), "rope_part_kv");
 }
 
+// Returns the number of launches
+int attn_decode_shared(const Tensor& q, const Tensor& kv, const Tensor& out, const Tensor& block_table, const Tensor& seq_lens, const Tensor& shared_len, int64_t n_heads, int64_t n_kv_heads,
+                       int64_t head_dim, int64_t rows_per_seq, double scale, const OptTensor& gate, int64_t max_shared, int64_t max_tail, int64_t prefix_row, const Tensor& tickets, const Tensor& status) {
+    llm::AttnSharedParams p = {};
+    want(q, torch::kBFloat16, "q");
+    TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head size must be 64, 128 or 256");
+    TORCH_CHECK(n_kv_heads >= 1 && n_heads >= 1 && n_heads <= 65535 && n_heads % n_kv_heads == 0, "query heads must be a multiple of K/V heads");
+    TORCH_CHECK(rows_per_seq >= 1 && n_heads / n_kv_heads * rows_per_seq <= 16, "at most 16 rows x heads of a group per sequence");
+    p.block_table = table_arg(q, block_table, p.n_seqs, p.max_pages);
+    TORCH_CHECK(p.n_seqs <= 65535 && (int64_t)p.max_pages * 64 <= INT32_MAX, "more than 65535 sequences, or too many pages");
+    TORCH_CHECK(q.numel() == p.n_seqs * rows_per_seq * n_heads * head_dim, "q must be [sequences * rows, heads, head size]");
+    same_device(q, out, "out");
+    want(out, torch::kBFloat16, "out");
+    TORCH_CHECK(out.numel() == q.numel(), "out must be like q");
+    TORCH_CHECK(((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) & 15) == 0, "q and out must be 16-byte aligned");
+    uint8_t* at = nullptr;
+    size_t page_bytes = 0, scale_off = 0;
+    int q8 = 0;
+    cache_args(q, kv, n_kv_heads, head_dim, at, p.n_pages, page_bytes, scale_off, q8);
+    TORCH_CHECK(!q8, "attention behind a shared prefix reads bf16 pages");
+    p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()); p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()); p.kv = reinterpret_cast<const __nv_bfloat16*>(at);
+    p.seq_lens = ints_on(q, seq_lens, p.n_seqs, "seq_lens");
+    p.shared_len = ints_on(q, shared_len, 1, "shared_len");
+    p.rows_per_seq = rows_per_seq; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.head_dim = head_dim; p.scale = scale;
+    if (gate) {
+        same_device(q, *gate, "gate");
+        TORCH_CHECK(gate->scalar_type() == torch::kBFloat16 && gate->dim() == 3 && gate->size(0) == p.n_seqs * rows_per_seq && gate->size(1) == n_heads && gate->size(2) == head_dim && gate->stride(2) == 1 &&
+                    gate->stride(0) >= 0 && gate->stride(1) >= 0, "gate must be bf16 [rows, heads, head size]");
+        p.gate = reinterpret_cast<const __nv_bfloat16*>(gate->data_ptr()); p.gate_token = gate->stride(0); p.gate_head = gate->stride(1);
+    }
+    TORCH_CHECK(max_shared >= 0 && max_tail >= 0 && prefix_row >= 0 && (p.n_seqs == 0 || prefix_row < p.n_seqs), "max_shared, max_tail or prefix_row");
+    if (p.n_seqs == 0) return 0;
+    const int64_t table = (int64_t)p.max_pages * 64;
+    p.prefix_row = prefix_row;
+    same_device(q, tickets, "tickets"); same_device(q, status, "status");
+    want(status, torch::kInt32, "status");
+    const int* t = ints(tickets, "tickets");
+    const llm::AttnSharedPlan plan = llm::attn_shared_plan(p.n_seqs, p.rows_per_seq, p.n_heads, p.n_kv_heads, p.head_dim, std::min(max_shared, table),
+                                                           std::min(max_tail ? max_tail : table, table), tickets.numel());
+    const c10::cuda::CUDAGuard guard(q.device());
+    p.splits = plan.splits; p.tail_splits = plan.tail_splits; p.tickets = reinterpret_cast<unsigned*>(const_cast<int*>(t));
+    const int64_t rows = plan.prefix_rows + plan.tail_rows;
+    Tensor parts;
+    if (rows) {
+        parts = torch::empty({rows * (head_dim + 2)}, q.options().dtype(torch::kFloat32));
+        p.part_o = parts.data_ptr<float>(); p.tail_o = p.part_o + plan.prefix_rows * head_dim;
+        p.part_ml = p.part_o + rows * head_dim; p.tail_ml = p.part_ml + plan.prefix_rows * 2;
+    }
+    check(llm::launch_attn_shared(p, status.data_ptr<int>(), stream()), "attn_decode_shared");
+    return p.splits ? 2 : 1;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -183,6 +235,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gdn_commit", &gdn_commit);
     m.def("gdn_chunk_bytes", &llm::gdn_chunk_bytes);
     m.def("rope_part_kv", &rope_part_kv);
+    m.def("attn_decode_shared", &attn_decode_shared);
     m.def("set_pdl", [](bool on) { llm::pdl_enabled() = on; });
-    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset) | llm::bounds_status_gdn_chunk(reset) | llm::bounds_status_rope_part(reset); });
+    m.def("bounds_status", [](bool reset) { return llm::bounds_status_gdn_rows(reset) | llm::bounds_status_gdn_chunk(reset) | llm::bounds_status_rope_part(reset) | llm::bounds_status_attn_shared(reset); });
 }

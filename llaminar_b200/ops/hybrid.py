@@ -1,5 +1,5 @@
-"""Python surface of the hybrid extension (csrc/gdn_rows.cu, gdn_chunk.cu, rope_part.cu): the blocks of the Gated-DeltaNet family where
-a step has more than one new row per sequence.
+"""Python surface of the hybrid extension (csrc/gdn_rows.cu, gdn_chunk.cu, rope_part.cu, attn_shared.cu): the blocks of the Gated-DeltaNet
+family where a step has more than one new row per sequence, its softmax blocks, and attention of batches behind a shared prefix.
 
 As in :mod:`llaminar_b200.ops`, every call launches hand-written CUDA on the current stream; there is no fallback.  Arguments are checked
 on the host, indices that lie on the device (slots, page ids, row ranges) are the caller's promise.  The PyTorch form of the
@@ -99,6 +99,18 @@ def rope_part_kv(rows: torch.Tensor, q_out: torch.Tensor, kv: torch.Tensor, q_no
     ext().rope_part_kv(rows, q_out, kv, q_norm, k_norm, freqs, float(magnitude), positions, seq_ids, block_table, n_heads, n_kv_heads, head_dim, eps,
                        bool(gated), bool(interleaved))
     _count()
+
+
+def attn_decode_shared(q: torch.Tensor, kv: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, shared_len: torch.Tensor,
+                       n_heads: int, n_kv_heads: int, head_dim: int, rows_per_seq: int, scale: float, scratch, *, gate: torch.Tensor | None = None,
+                       max_shared: int, max_tail: int = 0, prefix_row: int = 0) -> None:
+    """`attn_decode` over bf16 pages for sequences that share their first keys, which are read and multiplied once for all of them: keys 0 .. shared_len (one
+    int32 on the device), in the pages that block_table[prefix_row] begins with.  Those pages, the last one whole even if the prefix ends in it, stand
+    in front of the table of every sequence whose rows all see the prefix; a shorter sequence, or one of no keys, takes nothing from it.  ``max_shared``
+    (host; 0: nothing is shared) and ``max_tail`` (most keys of a sequence behind the prefix; 0: unknown) only decide how the keys are shared out.
+    ``gate`` [rows, heads, head size]: its sigmoid multiplies the result.  Head sizes 64, 128 and 256, up to 16 rows x query heads per K/V head."""
+    _count(ext().attn_decode_shared(q, kv, out, block_table, seq_lens, shared_len, n_heads, n_kv_heads, head_dim, rows_per_seq, scale, gate, max_shared, max_tail,
+                                    prefix_row, scratch.attn_tickets, scratch.status))
 
 
 def bounds_status(reset: bool = True) -> int:

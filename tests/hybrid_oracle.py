@@ -62,3 +62,22 @@ def rope_part(rows, n_heads, n_kv_heads, D, q_norm, k_norm, freqs, magnitude, po
         return out
 
     return turn(q, q_norm), turn(k, k_norm), v
+
+
+def attention_rows(q, kv, table, seq_len, R, n_kv_heads, scale, gate=None):
+    """The R rows of one sequence over its own table: q [R, H, D]; row r sees keys < seq_len - (R - 1 - r).  Returns the rows and, as large, sum p |v|."""
+    H, D = q.shape[1:]
+    out, size = torch.zeros(R, H, D, dtype=F64), torch.zeros(R, H, D, dtype=F64)
+    for r in range(R):
+        n = seq_len - (R - 1 - r)
+        if n <= 0:
+            continue
+        pages = table[:(n + 63) // 64].long()
+        for h in range(H):
+            kvh = h // (H // n_kv_heads)
+            K = kv[pages, 0, kvh].reshape(-1, D)[:n].to(F64)
+            V = kv[pages, 1, kvh].reshape(-1, D)[:n].to(F64)
+            p = torch.softmax(K @ q[r, h].to(F64) * scale, 0)
+            out[r, h], size[r, h] = p @ V, p @ V.abs()
+    g = 1.0 if gate is None else 1 / (1 + torch.exp(-gate.to(F64)))
+    return out * g, size * g

@@ -307,3 +307,182 @@ def test_rope_part_kv_refuses_what_it_cannot_take():
             ops.rope_part_kv(**{**good, **change})
     ops.rope_part_kv(**{**good, "rows": good["rows"][:0], "q_out": good["q_out"][:0], "positions": it([]), "seq_ids": it([])})
     torch.cuda.synchronize()
+
+
+# -- attention behind a shared prefix -------------------------------------------------------------------------------------
+
+SHARED = [
+    # heads, kv heads, head size, rows per sequence, prefix, keys behind it (or, negative, a sequence of that many keys that does not share)
+    (4, 2, 64, 1, 64, [1]),
+    (6, 1, 64, 2, 128, [2, 70, 64]),
+    (8, 2, 128, 1, 500, [1, 63, 64, 65, 300]),                 # a prefix that ends inside a page
+    (16, 1, 128, 1, 130, [5, -40, 7, 0]),                      # one shorter than the prefix, one of the prefix alone
+    (28, 4, 128, 2, 1000, [30] * 20),                          # more than a tile of rows
+    (2, 2, 128, 16, 200, [16, 40]),
+    (24, 4, 256, 1, 700, [9, 100, 1]),
+    (6, 1, 256, 2, 65, [3, -1, 66, 2]),                        # a sequence of one key and two rows
+    (16, 2, 256, 1, 1, [1, 200]),
+    (8, 8, 64, 1, 0, [10, 130]),                               # nothing is shared
+    (32, 8, 128, 1, 3000, [17] * 40),
+    (16, 4, 64, 1, 300, [2000, 3]),                            # a long tail
+    (12, 2, 256, 2, 640, [200] * 30),
+]
+
+
+def _shared_problem(H, Hk, D, R, prefix, tails, gated):
+    """The prefix's pages, the last one whole, stand in front of the tables of the sequences that share it; what a sequence has behind the prefix in a page
+    where the prefix ends is then everybody's."""
+    g = torch.Generator().manual_seed(H * D + prefix)
+    B, pre = len(tails), -(-prefix // 64)
+    total = [prefix + n if n >= 0 else -n for n in tails]
+    pages = [-(-n // 64) for n in total]
+    table = torch.zeros(B, max(pages + [pre]) + 1, dtype=torch.int32)
+    ids = iter((torch.randperm(pre + sum(pages) + 1, generator=g) + 1).tolist())
+    front = [next(ids) for _ in range(pre)]
+    for b in range(B):
+        mine = (front if tails[b] >= 0 else []) + [next(ids) for _ in range(pages[b])]
+        table[b, :pages[b]] = torch.tensor(mine[:pages[b]], dtype=torch.int32)
+    kv = torch.randn(pre + sum(pages) + 2, 2, Hk, 64, D, generator=g).to(torch.bfloat16)
+    q = torch.randn(B * R, H, D, generator=g).to(torch.bfloat16)
+    rows = torch.randn(B * R, H, 2, D, generator=g).to(torch.bfloat16) if gated else None
+    return table, kv, q, rows, total
+
+
+def _check_attention(got, want, size):
+    """Probabilities enter the second product as bf16: each is off by half a step at most, 2^-8 of it, so the sum by 2^-8 sum p |v|; the result is rounded to bf16
+    once more.  Scores, sums and exponentials are 32-bit: less than 2^-12 of sum p |v|."""
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * size + 1e-30
+    err = (got.double().cpu() - want).abs()
+    assert (err <= bound).all(), float((err - bound).max())
+
+
+def _scratch():
+    from llaminar_b200 import ops
+    return ops.scratch_for(torch.device(DEV, torch.cuda.current_device()))
+
+
+def _clean():
+    assert int(_scratch().status[0]) == 0 and int(_scratch().attn_tickets.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("H,Hk,D,R,prefix,tails", SHARED)
+@pytest.mark.parametrize("gated", [False, True])
+def test_attn_decode_shared_equals_attention_over_each_table(H, Hk, D, R, prefix, tails, gated):
+    from llaminar_b200 import ops
+    table, kv, q, rows, total = _shared_problem(H, Hk, D, R, prefix, tails, gated)
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    # what no row sees: pages of nobody, and the keys behind each sequence
+    seen = torch.zeros(kv.shape[0], 64, dtype=torch.bool)
+    for b in range(len(tails)):
+        for k in range(total[b]):
+            seen[int(table[b, k // 64]), k % 64] = True
+    if not any(t >= 0 and total[b] > 0 for b, t in enumerate(tails)):
+        seen[table[0, :-(-prefix // 64)].long()] = True
+    kv.permute(0, 3, 1, 2, 4)[~seen] = torch.tensor([float("nan"), float("inf")] * (D // 2), dtype=torch.bfloat16)
+    scale, out = D ** -0.5, torch.empty_like(q, device=DEV)
+    gate = rows.to(DEV)[:, :, 1] if gated else None
+    want = [oracle.attention_rows(q[b * R:(b + 1) * R], kv, table[b], total[b], R, Hk, scale, rows[b * R:(b + 1) * R, :, 1] if gated else None) for b in range(len(tails))]
+    for max_shared, max_tail in ((prefix, 0), (prefix, max(64, *tails)), (0, 0)):
+        out.fill_(float("nan"))
+        ops.attn_decode_shared(q.to(DEV), kv.to(DEV), out, table.to(DEV), it(total), it([prefix]), H, Hk, D, R, scale, _scratch(), gate=gate,
+                               max_shared=max_shared, max_tail=max_tail)
+        torch.cuda.synchronize()
+        for b in range(len(tails)):
+            _check_attention(out[b * R:(b + 1) * R], *want[b])
+            if total[b] == 0:
+                assert (out[b * R:(b + 1) * R] == 0).all()
+    _clean()
+
+
+def test_a_drafted_key_that_is_not_finite_reaches_the_rows_that_see_it_alone():
+    from llaminar_b200 import ops
+    H, Hk, D, R, prefix = 4, 1, 128, 3, 128
+    table, kv, q, _, total = _shared_problem(H, Hk, D, R, prefix, [20, 64], False)
+    kv[int(table[0, (total[0] - 1) // 64]), 1, 0, (total[0] - 1) % 64] = float("nan")        # the value of the first sequence's last key
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q, device=DEV)
+    ops.attn_decode_shared(q.to(DEV), kv.to(DEV), out, table.to(DEV), it(total), it([prefix]), H, Hk, D, R, D ** -0.5, _scratch(), max_shared=prefix)
+    assert torch.isnan(out[2]).all() and torch.isfinite(out[[0, 1, 3, 4, 5]].float()).all()
+    want = oracle.attention_rows(q[3:], kv, table[1], total[1], R, Hk, D ** -0.5)
+    _check_attention(out[3:], *want)
+
+
+@pytest.mark.parametrize("D,gated", [(128, False), (256, True)])
+def test_attn_decode_shared_is_captured_and_follows_lengths_on_the_device(D, gated):
+    """One captured call: the prefix shrinks to nothing, sequences grow and end, the row that the prefix is read from stays."""
+    from llaminar_b200 import ops
+    H, Hk, R, prefix, tails = 8, 2, 1, 256, [40, 100, 7]
+    table, kv, q, rows, total = _shared_problem(H, Hk, D, R, prefix, tails, gated)
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    lens, shared, out, qd, kvd, td = it(total), it([prefix]), torch.empty_like(q, device=DEV), q.to(DEV), kv.to(DEV), table.to(DEV)
+    gate = rows.to(DEV)[:, :, 1] if gated else None
+    call = lambda: ops.attn_decode_shared(qd, kvd, out, td, lens, shared, H, Hk, D, R, D ** -0.5, _scratch(), gate=gate, max_shared=prefix, max_tail=128, prefix_row=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for n, now in ((prefix, total), (128, total), (0, total), (prefix, [total[0] - 5, total[1], 0]), (prefix, [3, total[1], total[2]])):
+        shared.copy_(it([n]))
+        lens.copy_(it(now))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for b in range(3):
+            _check_attention(out[b:b + 1], *oracle.attention_rows(q[b:b + 1], kv, table[b], now[b], R, Hk, D ** -0.5, rows[b:b + 1, :, 1] if gated else None))
+    _clean()
+
+
+def test_rows_are_appended_and_read_behind_a_shared_prefix():
+    """A softmax block of a decode step as it is used: [query | gate] rows, norm, rotation of a quarter of each head and append, attention, gate."""
+    from llaminar_b200 import ops
+    H, Hk, D, prefix, tails = 6, 2, 256, 192, [1, 30, 65, 64]
+    table, kv, _, _, total = _shared_problem(H, Hk, D, 1, prefix, tails, False)
+    B = len(tails)
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn(B, (2 * H + 2 * Hk) * D, generator=g).to(torch.bfloat16)
+    gain, freqs = torch.rand(D, generator=g) + 0.5, 1e6 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    pos = [n - 1 for n in total]
+    kvd, q_out, rd, td = kv.to(DEV), torch.empty(B, H, D, dtype=torch.bfloat16, device=DEV), rows.to(DEV), table.to(DEV)
+    ops.rope_part_kv(rd, q_out, kvd, gain.to(DEV), gain.to(DEV), freqs.to(DEV), 1.0, it(pos), it(list(range(B))), td, H, Hk, D, EPS, gated=True)
+    out = torch.empty_like(q_out)
+    gate = rd[:, :2 * H * D].view(B, H, 2, D)[:, :, 1]
+    ops.attn_decode_shared(q_out, kvd, out, td, it(total), it([prefix]), H, Hk, D, 1, D ** -0.5, _scratch(), gate=gate, max_shared=prefix)
+    torch.cuda.synchronize()
+    q, k, v = oracle.rope_part(rows, H, Hk, D, gain, gain, freqs, 1.0, pos, EPS, True, False)
+    for b in range(B):
+        page, off = int(table[b, pos[b] // 64]), pos[b] % 64
+        kv[page, 0, :, off], kv[page, 1, :, off] = k[b].to(torch.bfloat16), v[b].to(torch.bfloat16)
+        want, size = oracle.attention_rows(q_out[b:b + 1].cpu(), kv, table[b], total[b], 1, Hk, D ** -0.5, gate[b:b + 1].cpu())
+        # the new key may round the other way than the oracle's, a step of 2^-7 of it, which moves its score by less than 2^-7 |q||k| / 16 and its share by that much
+        slack = 2.0 ** -7 * size * float((q[b].norm(dim=-1).max() * k[b].norm(dim=-1).max()) / 16) / total[b] ** 0.5
+        err = (out[b].double().cpu() - want[0]).abs()
+        assert (err <= 2.0 ** -8 * want[0].abs() + (2.0 ** -8 + 2.0 ** -12) * size[0] + slack[0]).all()
+
+
+def test_attn_decode_shared_refuses_what_it_cannot_take():
+    from llaminar_b200 import ops
+    it = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    H, Hk, D, B = 4, 2, 128, 2
+    good = dict(q=torch.zeros(B, H, D, dtype=torch.bfloat16, device=DEV), kv=torch.zeros(4, 2, Hk, 64, D, dtype=torch.bfloat16, device=DEV),
+                out=torch.zeros(B, H, D, dtype=torch.bfloat16, device=DEV), block_table=it([[1, 2], [1, 3]]), seq_lens=it([70, 80]), shared_len=it([64]), n_heads=H,
+                n_kv_heads=Hk, head_dim=D, rows_per_seq=1, scale=0.1, scratch=_scratch(), max_shared=64)
+    ops.attn_decode_shared(**good)
+    for change in (dict(q=good["q"].float()), dict(q=good["q"][:1]), dict(q=good["q"].cpu()), dict(kv=good["kv"].half()), dict(kv=good["kv"][:, :1]),
+                   dict(kv=torch.zeros(4, 2 * Hk * 64 * D * 17 // 16, dtype=torch.uint8, device=DEV)), dict(out=good["out"].float()), dict(out=good["out"][:, :2]),
+                   dict(block_table=good["block_table"].long()), dict(block_table=good["block_table"][0]), dict(seq_lens=it([1])), dict(shared_len=it([1, 2])),
+                   dict(shared_len=torch.tensor([64], dtype=torch.int32)), dict(n_heads=3), dict(n_kv_heads=3), dict(head_dim=96), dict(rows_per_seq=0), dict(rows_per_seq=2),
+                   dict(gate=torch.zeros(B, H, D, device=DEV)), dict(gate=torch.zeros(B, H, D - 1, dtype=torch.bfloat16, device=DEV)), dict(max_shared=-1), dict(prefix_row=2),
+                   dict(prefix_row=-1)):
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.attn_decode_shared(**{**good, **change})
+    with pytest.raises(RuntimeError):                            # 17 rows x heads of a group
+        ops.attn_decode_shared(**{**good, "q": torch.zeros(2 * 17, 1, D, dtype=torch.bfloat16, device=DEV), "out": torch.zeros(2 * 17, 1, D, dtype=torch.bfloat16, device=DEV),
+                                  "n_heads": 1, "n_kv_heads": 1, "kv": good["kv"][:, :, :1].contiguous(), "rows_per_seq": 17})
+    ops.attn_decode_shared(**{**good, "q": good["q"][:0], "out": good["out"][:0], "block_table": good["block_table"][:0], "seq_lens": it([])})
+    torch.cuda.synchronize()
+    _clean()
