@@ -33,20 +33,20 @@ LLM_DEVICE bool shares(const AttnSharedParams& p, int b, int prefix) { return p.
 // ------------------------------------------------------------------------------------------------
 // prefix
 // ------------------------------------------------------------------------------------------------
+// Tiles of 64 keys (a page).  Each slot of 128 rows has two tiles of S in tensor memory (P in the first half of each), so that a product is always on its way while
+// its softmax is at work: with one tile of 128 keys per slot a tile took 3550 clocks, of which the softmax waited 1500 (32 / 8 heads, 122 rows).
 template <int D, int SLOTS>
 struct Prefix {
-    static constexpr int BK = D == 256 ? 64 : 128, DA = D / 64;               // keys of a tile, atoms of 64 values in a head
+    static constexpr int BK = 64, DA = D / 64, STAGES = D == 256 ? 2 : 4;     // keys of a tile, atoms of 64 values in a head, tiles of K and of V
     static constexpr int K_ATOM = BK * 128, TILE = DA * K_ATOM;
-    static constexpr int OFF_K = SLOTS * DA * ATOM, OFF_V = OFF_K + 2 * TILE, SMEM = OFF_V + 2 * TILE + 1024;
-    // a row's scores stay in registers: with two slots a third warpgroup hands most of its registers to the softmax
-    static constexpr int THREADS = SLOTS == 2 ? 384 : 192, REGS_LAUNCH = 168, REGS_SOFTMAX = 224, REGS_OTHER = 56;
-    static_assert(2 * REGS_SOFTMAX + REGS_OTHER <= 3 * REGS_LAUNCH, "a warpgroup would wait for registers that nobody gives back");
-    // tensor memory: two tiles of S (P in the first half of each), then O per slot.  With one slot its two tiles alternate.
-    static constexpr uint32_t COL_O = 2 * BK;
+    static constexpr int OFF_K = SLOTS * DA * ATOM, OFF_V = OFF_K + STAGES * TILE, SMEM = OFF_V + STAGES * TILE + 1024;
+    static constexpr int THREADS = SLOTS * 128 + 64;
+    static constexpr uint32_t COL_O = SLOTS * 2 * BK;                         // behind the tiles of S: O per slot
     static constexpr uint32_t IDESC_S = instr_desc(BK), IDESC_O = instr_desc(D) | (1u << 16);       // bit 16: B is MN-major
-    static_assert(SMEM <= 227 * 1024 && COL_O + SLOTS * D <= 512, "a CTA's memories");
+    static_assert(SMEM <= 225 * 1024 && COL_O + SLOTS * D <= 512, "a CTA's memories");
+    static_assert(SLOTS * 128 * D * 4 <= OFF_V + STAGES * TILE, "results on their way out");
 };
-enum Bar { K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, PV_DONE = 12, O_FULL = 14, Q_FULL = 16, N_BARS };
+enum Bar { K_FULL = 0, K_EMPTY = 4, V_FULL = 8, V_EMPTY = 12, S_FULL = 16, P_FULL = 20, PV_DONE = 24, Q_FULL = 26, N_BARS };       // S_FULL, P_FULL: slot * 2 + tile of S
 
 template <int D, int SLOTS>
 __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kernel(const __grid_constant__ CUtensorMap map_kv, const AttnSharedParams p, int* status) {
@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
     __shared__ __align__(8) uint64_t s_bars[N_BARS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort[2];       // [1] stays 0 here (tc_common.cuh: restarts the wait clock when set)
+    __shared__ int s_query[SLOTS * BQ];                    // where a row's query lies, in heads; -1: there is none
     pdl_wait();
     pdl_trigger();                   // the tails may begin: what they read was there before this kernel
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
     auto bar = [&](int i) { return bars + i * 8; };
     if (tid == 0) {
         s_abort[0] = 0; s_abort[1] = 0;
-        for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i == Q_FULL ? (both ? 8 : 4) : i == P_FULL || i == P_FULL + 1 ? 4 : 1);
+        for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i == Q_FULL ? (both ? 8 : 4) : i >= P_FULL && i < P_FULL + 4 ? 4 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
     }
@@ -88,22 +89,22 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     volatile int* abort_flag = s_abort;
-    // S tile of (slot, key tile), and the phase of its barriers
-    auto buffer = [&](int slot, int j) { return SLOTS == 2 ? slot : j & 1; };
-    auto phase = [&](int j) { return (uint32_t)(SLOTS == 2 ? j & 1 : (j >> 1) & 1); };
+    auto buffer = [](int slot, int j) { return slot * 2 + (j & 1); };         // tile of S
+    auto phase = [](int j) { return (uint32_t)((j >> 1) & 1); };              // of its barriers
 
     if (warp < SLOTS * 4) {
         // ------------------------------ softmax: one thread per query row (== TMEM lane) ------------------------------
-        if (SLOTS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(X::REGS_SOFTMAX));
         const int slot = warp >> 2, row = tid & 127;
         if (slot == 0 || both) {
             const int m0 = row_first + slot * BQ;
             const uint32_t sQ = base + slot * DA * ATOM;
+            s_query[slot * BQ + row] = m0 + row < rows_all ? (m0 + row) / G * p.n_heads + kvh * G + (m0 + row) % G : -1;
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + slot) : "memory");
 #pragma unroll 4
             for (int idx = row; idx < BQ * (D / 8); idx += 128) {
-                const int r = idx / (D / 8), u = idx % (D / 8), m = m0 + r;
+                const int r = idx / (D / 8), u = idx % (D / 8), from = s_query[slot * BQ + r];
                 const uint32_t dst = atom_addr(sQ + (u >> 3) * ATOM, r, u & 7);
-                if (m < rows_all) cp_async16(dst, p.q + ((size_t)(m / G) * p.n_heads + kvh * G + m % G) * D + u * 8);
+                if (from >= 0) cp_async16(dst, p.q + (size_t)from * D + u * 8);
                 else st_shared_v4(dst, make_uint4(0, 0, 0, 0));
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -133,9 +134,9 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
                     for (int c = 0; c < BK / 32; ++c)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) s[c][i] = c * 32 + i < hi ? s[c][i] : 0xff800000u;       // -inf
-                    ok = mbar_wait_warp(bar(V_FULL + (j & 1)), (j >> 1) & 1, abort_flag);
+                    ok = mbar_wait_warp(bar(V_FULL + j % X::STAGES), j / X::STAGES & 1, abort_flag);
                     if (!ok) break;
-                    const uint32_t v = base + X::OFF_V + (j & 1) * X::TILE;
+                    const uint32_t v = base + X::OFF_V + j % X::STAGES * X::TILE;
                     for (int idx = row; idx < (BK - hi) * DA * 8; idx += 128) {
                         const int r = hi + idx / (DA * 8), u = idx % (DA * 8);
                         st_shared_v4(v + (u >> 3) * X::K_ATOM + r * 128 + ((u & 7) << 4), make_uint4(0, 0, 0, 0));
@@ -157,11 +158,10 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
                 const float factor = raise ? ex2(m - top) : 1.f;
                 if (raise) m = top;
                 if (j > 0 && __any_sync(0xffffffffu, raise)) {
-                    if (SLOTS == 1) {                      // this tile's S was issued in front of the last tile's P V: O has to be complete
-                        ok = mbar_wait_warp(bar(PV_DONE), (j - 1) & 1, abort_flag);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
+                    // this tile's S was issued in front of the last tile's P V: O has to be complete
+                    ok = mbar_wait_warp(bar(PV_DONE + slot), (j - 1) & 1, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t r[32];
@@ -191,102 +191,97 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
                 __syncwarp();
                 mbar_arrive_if(bar(P_FULL + buf), lane == 0);
             }
-            ok = ok && mbar_wait_warp(bar(O_FULL + slot), 0, abort_flag);
+            // the last product is complete (the one before it first: a wait tells apart two neighbouring phases only)
+            ok = ok && (nt < 2 || mbar_wait_warp(bar(PV_DONE + slot), (nt - 2) & 1, abort_flag)) && mbar_wait_warp(bar(PV_DONE + slot), (nt - 1) & 1, abort_flag);
+            if (both) asm volatile("bar.sync 3, 256;" ::: "memory");            // both slots' products are done with Q, K and V
             if (ok) {
+                // O through shared memory, so that a warp writes whole rows (a row per thread took 15000 clocks); 16-byte units XOR-swizzled
                 tc_fence_after();
                 const size_t at = part + (size_t)(slot * BQ + row) * p.splits;
-                float4* dst = reinterpret_cast<float4*>(p.part_o + at * D);
+                if (m0 + row < rows_all) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+                const uint32_t mine = base + (slot * BQ + (warp & 3) * 32) * (D * 4);
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t r[32];
                     tmem_ld_n<32>(t_o + c * 32, r);
-                    if (m0 + row < rows_all) {
 #pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            dst[c * 8 + u] = make_float4(__uint_as_float(r[4 * u]), __uint_as_float(r[4 * u + 1]), __uint_as_float(r[4 * u + 2]), __uint_as_float(r[4 * u + 3]));
-                    }
+                    for (int u = 0; u < 8; ++u) st_shared_v4(mine + lane * (D * 4) + (((c * 8 + u) ^ (lane & 7)) << 4), make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
                 }
-                if (m0 + row < rows_all) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+                __syncwarp();
+                constexpr int UNITS = D / 4;                // of a row
+#pragma unroll 8
+                for (int i = lane; i < 32 * UNITS; i += 32) {
+                    const int r = i / UNITS, u = i % UNITS, row_of = (warp & 3) * 32 + r;
+                    float4 v;
+                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mine + r * (D * 4) + ((u ^ (r & 7)) << 4)));
+                    if (m0 + row_of < rows_all) *(reinterpret_cast<float4*>(p.part_o + (part + (size_t)(slot * BQ + row_of) * p.splits) * D) + u) = v;
+                }
             }
         }
-    } else {
-        if (SLOTS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(X::REGS_OTHER));
-        if (warp == SLOTS * 4) {
-            // ------------------------------ K and V pages, 64 values at a time ------------------------------
-            if (elect_one()) {
-                bool ok = true;
-                const int n_pages = (keys + PAGE - 1) / PAGE;
-                auto load = [&](int j, int kv, int full, int empty) {
-                    const int b = j & 1;
-                    ok = mbar_wait(bar(empty + b), ((j >> 1) & 1) ^ 1, abort_flag);
-                    if (!ok) return;
-                    mbar_arrive_expect_tx(bar(full + b), X::TILE);
-                    const uint32_t dst = base + (kv ? X::OFF_V : X::OFF_K) + b * X::TILE;
+    } else if (warp == SLOTS * 4) {
+        // ------------------------------ K and V pages, 64 values at a time ------------------------------
+        if (elect_one()) {
+            bool ok = true;
+            const int* table = p.block_table + (size_t)p.prefix_row * p.max_pages + tile0;
+            int page = LLM_CHECK_INDEX(table[0], p.n_pages);
+            auto load = [&](int j, int kv, int full, int empty) {
+                const int b = j % X::STAGES;
+                ok = mbar_wait(bar(empty + b), (j / X::STAGES & 1) ^ 1, abort_flag);
+                if (!ok) return;
+                mbar_arrive_expect_tx(bar(full + b), X::TILE);
+                const uint32_t dst = base + (kv ? X::OFF_V : X::OFF_K) + b * X::TILE;
+                const int y = ((page * 2 + kv) * p.n_kv_heads + kvh) * PAGE;
 #pragma unroll
-                    for (int h = 0; h < BK / PAGE; ++h) {
-                        // a page past the end repeats the last one (its keys are masked)
-                        const int page = LLM_CHECK_INDEX(p.block_table[(size_t)p.prefix_row * p.max_pages + min((tile0 + j) * (BK / PAGE) + h, n_pages - 1)], p.n_pages);
-                        const int y = ((page * 2 + kv) * p.n_kv_heads + kvh) * PAGE;
-#pragma unroll
-                        for (int a = 0; a < DA; ++a) tma_load_2d(dst + a * X::K_ATOM + h * (PAGE * 128), &map_kv, a * 64, y, bar(full + b));
-                    }
-                };
-                for (int j = 0; j < nt && ok; ++j) {
-                    load(j, 0, K_FULL, K_EMPTY);
-                    if (ok) load(j, 1, V_FULL, V_EMPTY);
-                }
+                for (int a = 0; a < DA; ++a) tma_load_2d(dst + a * X::K_ATOM, &map_kv, a * 64, y, bar(full + b));
+            };
+            for (int j = 0; j < nt && ok; ++j) {
+                const int next = j + 1 < nt ? table[j + 1] : 0;
+                load(j, 0, K_FULL, K_EMPTY);
+                if (ok) load(j, 1, V_FULL, V_EMPTY);
+                page = LLM_CHECK_INDEX(next, p.n_pages);
             }
-        } else if (warp == SLOTS * 4 + 1 && elect_one()) {
-            // ------------------------------ products ------------------------------
-            auto issue_s = [&](int slot, int j) {
-                const uint32_t q = base + slot * DA * ATOM, k = base + X::OFF_K + (j & 1) * X::TILE;
+        }
+    } else if (elect_one()) {
+        // ------------------------------ products ------------------------------
+        const int slots = both ? 2 : 1;
+        auto issue_s = [&](int slot, int j) {
+            const uint64_t q = smem_desc_sw128(base + slot * DA * ATOM), k = smem_desc_sw128(base + X::OFF_K + j % X::STAGES * X::TILE);
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    mma_f16(tmem + buffer(slot, j) * BK, smem_desc_sw128(q + (ks >> 2) * ATOM) + 2 * (ks & 3), smem_desc_sw128(k + (ks >> 2) * X::K_ATOM) + 2 * (ks & 3), X::IDESC_S, ks > 0 ? 1u : 0u);
-                mma_commit(bar(S_FULL + buffer(slot, j)));
-            };
-            auto issue_o = [&](int slot, int j) {
-                const uint32_t v = base + X::OFF_V + (j & 1) * X::TILE;
+            for (int ks = 0; ks < D / 16; ++ks)             // (a descriptor counts 16 bytes)
+                mma_f16(tmem + buffer(slot, j) * BK, q + (ks >> 2) * (ATOM / 16) + 2 * (ks & 3), k + (ks >> 2) * (X::K_ATOM / 16) + 2 * (ks & 3), X::IDESC_S, ks > 0 ? 1u : 0u);
+            mma_commit(bar(S_FULL + buffer(slot, j)));
+        };
+        auto issue_o = [&](int slot, int j) {
+            const uint64_t v = smem_desc_mn_sw128(base + X::OFF_V + j % X::STAGES * X::TILE, X::K_ATOM);
 #pragma unroll
-                for (int ks = 0; ks < BK / 16; ++ks)            // 16 keys: 8 TMEM columns of P, 16 rows of the V tile
-                    mma_f16_ts(tmem + X::COL_O + slot * D, tmem + buffer(slot, j) * BK + ks * 8, smem_desc_mn_sw128(v + ks * 16 * 128, X::K_ATOM), X::IDESC_O, j > 0 || ks > 0 ? 1u : 0u);
-            };
-            auto keys_of = [&](int j) { return mbar_wait(bar(K_FULL + (j & 1)), (j >> 1) & 1, abort_flag); };
-            auto probabilities = [&](int slot, int j) { return mbar_wait(bar(P_FULL + buffer(slot, j)), phase(j), abort_flag); };
-            bool ok = mbar_wait(bar(Q_FULL), 0, abort_flag);
-            const int ahead = SLOTS == 2 ? 1 : min(2, nt);      // tiles whose S is issued before the first P V
-            for (int j = 0; j < ahead && ok; ++j) {
-                ok = keys_of(j);
+            for (int ks = 0; ks < BK / 16; ++ks)            // 16 keys: 8 TMEM columns of P, 16 rows of the V tile
+                mma_f16_ts(tmem + X::COL_O + slot * D, tmem + buffer(slot, j) * BK + ks * 8, v + ks * (16 * 128 / 16), X::IDESC_O, j > 0 || ks > 0 ? 1u : 0u);
+            mma_commit(bar(PV_DONE + slot));
+        };
+        auto scores = [&](int j) {                          // of a tile of keys, all slots
+            if (!mbar_wait(bar(K_FULL + j % X::STAGES), j / X::STAGES & 1, abort_flag)) return false;
+            tc_fence_after();
+            return true;
+        };
+        bool ok = mbar_wait(bar(Q_FULL), 0, abort_flag);
+        for (int j = 0; j < min(2, nt) && ok; ++j) {
+            ok = scores(j);
+            if (!ok) break;
+            for (int slot = 0; slot < slots; ++slot) issue_s(slot, j);
+            mma_commit(bar(K_EMPTY + j % X::STAGES));
+        }
+        for (int j = 0; j < nt && ok; ++j) {
+            ok = mbar_wait(bar(V_FULL + j % X::STAGES), j / X::STAGES & 1, abort_flag) && (j + 2 >= nt || scores(j + 2));
+            for (int slot = 0; slot < slots && ok; ++slot) {
+                ok = mbar_wait(bar(P_FULL + buffer(slot, j)), phase(j), abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                issue_s(0, j);
-                if (SLOTS == 2 && both) issue_s(1, j);
-                mma_commit(bar(K_EMPTY + (j & 1)));
+                issue_o(slot, j);
+                if (j + 2 < nt) issue_s(slot, j + 2);       // behind the P V that reads P from the same columns
             }
-            for (int j = 0; j < nt && ok; ++j) {
-                const int next = j + (SLOTS == 2 ? 1 : 2);
-                ok = mbar_wait(bar(V_FULL + (j & 1)), (j >> 1) & 1, abort_flag) && (next >= nt || SLOTS == 1 || keys_of(next));
-                for (int slot = 0; slot < (SLOTS == 2 && both ? 2 : 1) && ok; ++slot) {
-                    ok = probabilities(slot, j);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_o(slot, j);
-                    if (j + 1 == nt) mma_commit(bar(O_FULL + slot));
-                    if (SLOTS == 2 && next < nt) issue_s(slot, next);      // behind the P V that reads P from the same columns
-                }
-                if (!ok) break;
-                mma_commit(bar(V_EMPTY + (j & 1)));
-                if (SLOTS == 1) {
-                    mma_commit(bar(PV_DONE));
-                    if (next < nt) {
-                        ok = keys_of(next);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_s(0, next);
-                    }
-                }
-                if (next < nt) mma_commit(bar(K_EMPTY + (next & 1)));
-            }
+            if (!ok) break;
+            mma_commit(bar(V_EMPTY + j % X::STAGES));
+            if (j + 2 < nt) mma_commit(bar(K_EMPTY + (j + 2) % X::STAGES));
         }
     }
     tc_fence_before();
@@ -298,40 +293,94 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
 // ------------------------------------------------------------------------------------------------
 // tails
 // ------------------------------------------------------------------------------------------------
+constexpr int MAX_PARTS = 64;
 template <int D>
 struct Tail {
-    static constexpr int STAGES = D == 256 ? 2 : 3, SUB = 16 * D * 2, PER_WARP = STAGES * 2 * SUB;      // SUB: a warp's 16 keys of K or V
-    static constexpr int MERGE = 5 * 16 * (D + 2) * 4;      // four warps' results and that of the last drafted keys
+    static constexpr int STAGES = 2, SUB = 16 * D * 2, PER_WARP = STAGES * 2 * SUB;      // SUB: a warp's 16 keys of K or V
+    static constexpr int ROW = D + 8;                       // of a merged row: eight rows of an accumulator start 32 bytes apart, no two in one bank
+    static constexpr int MERGE = 5 * 16 * (ROW + 2) * 4 + 16 * MAX_PARTS * 4;         // four warps' results and that of the last drafted keys; weights of parts
     static constexpr int BYTES = 4 * PER_WARP > MERGE ? 4 * PER_WARP : MERGE;
 };
 
-// one more set of keys joins a row
-template <int N> LLM_DEVICE void join(float& m, float& l, float (&acc)[N], const float2& ml, const float (&v)[N]) {
-    if (ml.x == -INFINITY && ml.y == 0.f) return;            // no keys there
-    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
-    const float a = exp2f(m - base), b = exp2f(ml.x - base);
-    m = top;
-    l = l * a + ml.y * b;
+// A row among the lanes of a warp: D / 32 values each, four (two) neighbours at a time
+template <int D> LLM_DEVICE int column(int e) { return D == 64 ? (threadIdx.x & 31) * 2 + e : (e >> 2) * 128 + (threadIdx.x & 31) * 4 + (e & 3); }
+template <int D> LLM_DEVICE void load_row(const float* x, float (&v)[D / 32]) {
+    if constexpr (D == 64) {
+        const float2 t = __ldcg(reinterpret_cast<const float2*>(x + column<D>(0)));
+        v[0] = t.x; v[1] = t.y;
+    } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = acc[e] * a + b * v[e];
+        for (int e = 0; e < D / 32; e += 4) {
+            const float4 t = __ldcg(reinterpret_cast<const float4*>(x + column<D>(e)));
+            v[e] = t.x; v[e + 1] = t.y; v[e + 2] = t.z; v[e + 3] = t.w;
+        }
+    }
 }
-// `n` sets that lie `step` rows apart, four on their way at a time; a lane has values lane, lane + 32, ... of a row
-template <int N> LLM_DEVICE void join_parts(float& m, float& l, float (&acc)[N], const float* part_o, const float* part_ml, size_t first, int step, int n) {
+template <int D> LLM_DEVICE void load_row_shared(const float* x, float (&v)[D / 32]) {
+    if constexpr (D == 64) {
+        const float2 t = *reinterpret_cast<const float2*>(x + column<D>(0));
+        v[0] = t.x; v[1] = t.y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < D / 32; e += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(x + column<D>(e));
+            v[e] = t.x; v[e + 1] = t.y; v[e + 2] = t.z; v[e + 3] = t.w;
+        }
+    }
+}
+template <int D> LLM_DEVICE void store_row(float* x, const float (&v)[D / 32]) {
+    if constexpr (D == 64) {
+        *reinterpret_cast<float2*>(x + column<D>(0)) = make_float2(v[0], v[1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < D / 32; e += 4) *reinterpret_cast<float4*>(x + column<D>(e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    }
+}
+// `n` <= MAX_PARTS sets of keys, whose results lie `step` rows apart, join a row.  The maxima and sums of all of them first, a lane each, which gives every set its
+// weight (kept in `w`); then the values, many sets on their way at a time.
+template <int D> LLM_DEVICE void join_parts(float& m, float& l, float (&acc)[D / 32], const float* part_o, const float* part_ml, size_t first, int step, int n, float* w) {
+    constexpr int N = D / 32, DEEP = 64 / N > 16 ? 16 : 64 / N;
     const int lane = threadIdx.x & 31;
-    for (int s0 = 0; s0 < n; s0 += 4) {
-        float2 ml[4];
-        float v[4][N];
+    float2 ml[2];
+    float top = m;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const size_t at = first + (size_t)min(s0 + k, n - 1) * step;
-            ml[k] = __ldcg(reinterpret_cast<const float2*>(part_ml + at * 2));
+    for (int k = 0; k < 2; ++k) {
+        const int s = k * 32 + lane;
+        ml[k] = s < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + (first + (size_t)s * step) * 2)) : make_float2(-INFINITY, 0.f);
+    }
+    float v[DEEP][N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[k][e] = __ldcg(part_o + at * (N * 32) + e * 32 + lane);
+    for (int k = 0; k < DEEP; ++k) load_row<D>(part_o + (first + (size_t)min(k, n - 1) * step) * D, v[k]);
+    top = fmaxf(top, warp_max(fmaxf(ml[0].x, ml[1].x)));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const bool none = ml[k].x == -INFINITY && ml[k].y == 0.f;      // no keys there: nothing was written either
+        const float c = none ? 0.f : exp2f(ml[k].x - base);
+        sum += none ? 0.f : c * ml[k].y;
+        w[k * 32 + lane] = none ? -1.f : c;
+    }
+    const float old = l == 0.f && m == -INFINITY ? 0.f : exp2f(m - base);
+    l = l * old + warp_sum(sum);
+    m = top;
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] *= old;
+    __syncwarp();
+    for (int s0 = 0; s0 < n; s0 += DEEP) {
+        if (s0 > 0) {
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) load_row<D>(part_o + (first + (size_t)min(s0 + k, n - 1) * step) * D, v[k]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (s0 + k < n) join<N>(m, l, acc, ml[k], v[k]);
+        for (int k = 0; k < DEEP; ++k) {
+            const float c = s0 + k < n ? w[s0 + k] : -1.f;
+            if (c < 0.f) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += c * v[k][e];
+        }
     }
+    __syncwarp();
 }
 
 template <int D>
@@ -458,62 +507,65 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
     __syncthreads();
 
     // ---- the four warps' results (disjoint keys) and those of the last drafted keys, in shared memory ----
-    float* s_o = reinterpret_cast<float*>(smem);             // [5][16 rows][D]
-    float* s_ml = s_o + 5 * 16 * D;                          // [5][16][2]
+    constexpr int VPL = D / 32, ROW = SM::ROW;
+    const int sets = R > 1 ? 5 : 4;
+    float* s_o = reinterpret_cast<float*>(smem);             // [5][16][ROW]
+    float* s_ml = s_o + 5 * 16 * ROW;                        // [5][16][2]
+    float* s_w = s_ml + 5 * 16 * 2;                          // [16][MAX_PARTS]
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
         const int col = n * 8 + (lane & 3) * 2;
-        *reinterpret_cast<float2*>(&s_o[(warp * 16 + i0) * D + col]) = make_float2(o[n][0], o[n][1]);
-        *reinterpret_cast<float2*>(&s_o[(warp * 16 + i1) * D + col]) = make_float2(o[n][2], o[n][3]);
+        *reinterpret_cast<float2*>(&s_o[(warp * 16 + i0) * ROW + col]) = make_float2(o[n][0], o[n][1]);
+        *reinterpret_cast<float2*>(&s_o[(warp * 16 + i1) * ROW + col]) = make_float2(o[n][2], o[n][3]);
     }
     if ((lane & 3) == 0) {
         s_ml[(warp * 16 + i0) * 2] = m0; s_ml[(warp * 16 + i0) * 2 + 1] = l0;
         s_ml[(warp * 16 + i1) * 2] = m1; s_ml[(warp * 16 + i1) * 2 + 1] = l1;
     }
-    constexpr int VPL = D / 32;                              // values of a row a lane has from here on
-    for (int i = warp; i < rows; i += 4) {                   // a warp per row: keys stop .. seq_len - (R - 1 - r), one by one
+    for (int i = warp; R > 1 && i < rows; i += 4) {          // a warp per row: keys stop .. seq_len - (R - 1 - r), one by one
         float m = -INFINITY, l = 0.f, acc[VPL], x[VPL];
 #pragma unroll
         for (int e = 0; e < VPL; ++e) { acc[e] = 0.f; x[e] = 0.f; }
         const int end = seq_len - (R - 1 - i / G);
         if (split == 0 && stop < end) {
 #pragma unroll
-            for (int e = 0; e < VPL; ++e) x[e] = __bfloat162float(query(i)[e * 32 + lane]);
+            for (int e = 0; e < VPL; ++e) x[e] = __bfloat162float(query(i)[column<D>(e)]);
             for (int key = stop; key < end; ++key) {
                 const size_t at = (size_t)(key % PAGE) * D;
                 const __nv_bfloat16 *k = page_of(key / PAGE, 0) + at, *v = page_of(key / PAGE, 1) + at;
-                float d = 0.f;
+                float kx[VPL], vx[VPL], d = 0.f;
 #pragma unroll
-                for (int e = 0; e < VPL; ++e) d += x[e] * __bfloat162float(k[e * 32 + lane]);
+                for (int e = 0; e < VPL; ++e) { kx[e] = __bfloat162float(k[column<D>(e)]); vx[e] = __bfloat162float(v[column<D>(e)]); }
+#pragma unroll
+                for (int e = 0; e < VPL; ++e) d += x[e] * kx[e];
                 const float score = warp_sum(d) * sl2, top = fmaxf(m, score);
                 if (top == -INFINITY) continue;
                 const float c = exp2f(m - top), w = exp2f(score - top);
                 m = top;
                 l = l * c + w;
 #pragma unroll
-                for (int e = 0; e < VPL; ++e) acc[e] = acc[e] * c + w * __bfloat162float(v[e * 32 + lane]);
+                for (int e = 0; e < VPL; ++e) acc[e] = acc[e] * c + w * vx[e];
             }
         }
-#pragma unroll
-        for (int e = 0; e < VPL; ++e) s_o[(4 * 16 + i) * D + e * 32 + lane] = acc[e];
+        store_row<D>(&s_o[(4 * 16 + i) * ROW], acc);
         if (lane == 0) { s_ml[(4 * 16 + i) * 2] = m; s_ml[(4 * 16 + i) * 2 + 1] = l; }
     }
     __syncthreads();
 
     // the prefix, the quotient, the gate
     auto finish = [&](int i, float m, float l, float (&acc)[VPL]) {
-        if (joins) join_parts<VPL>(m, l, acc, p.part_o, p.part_ml, ((size_t)kvh * p.n_seqs * rows + (size_t)seq * rows + i) * p.splits, 1, p.splits);
+        if (joins) join_parts<D>(m, l, acc, p.part_o, p.part_ml, ((size_t)kvh * p.n_seqs * rows + (size_t)seq * rows + i) * p.splits, 1, p.splits, s_w + i * MAX_PARTS);
         const size_t token = (size_t)seq * R + i / G;
         const int head = kvh * G + i % G;
-        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;       // (a sum that is not a number stays one)
+        const float inv = l == 0.f ? 0.f : 1.f / l;          // (a sum that is not a number makes the row one)
 #pragma unroll
         for (int e = 0; e < VPL; ++e) {
-            float v = l > 0.f || l == 0.f ? acc[e] * inv : l;
-            if (l == 0.f) v = 0.f;
-            const int col = e * 32 + lane;
-            if (p.gate) v *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[token * p.gate_token + (size_t)head * p.gate_head + col])));
-            p.out[(token * p.n_heads + head) * D + col] = __float2bfloat16(v);
+            acc[e] = l == 0.f ? 0.f : acc[e] * inv;
+            if (p.gate) acc[e] *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[token * p.gate_token + (size_t)head * p.gate_head + column<D>(e)])));
         }
+        __nv_bfloat16* dst = p.out + (token * p.n_heads + head) * D;
+#pragma unroll
+        for (int e = 0; e < VPL; e += 2) *reinterpret_cast<uint32_t*>(dst + column<D>(e)) = pack_bf16(acc[e], acc[e + 1]);
     };
     const int S = (int)gridDim.y;
     const size_t mine = (((size_t)seq * p.n_kv_heads + kvh) * S + split) * 16;
@@ -522,18 +574,20 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
         float m = -INFINITY, l = 0.f, acc[VPL];
 #pragma unroll
         for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < 5; ++w) {
+        for (int w = 0; w < sets; ++w) m = fmaxf(m, s_ml[(w * 16 + i) * 2]);
+        for (int w = 0; w < sets; ++w) {
+            const float wm = s_ml[(w * 16 + i) * 2], c = wm == -INFINITY ? 0.f : exp2f(wm - m);
+            if (c == 0.f && s_ml[(w * 16 + i) * 2 + 1] == 0.f) continue;     // no keys there
             float v[VPL];
+            load_row_shared<D>(&s_o[(w * 16 + i) * ROW], v);
+            l += c * s_ml[(w * 16 + i) * 2 + 1];
 #pragma unroll
-            for (int e = 0; e < VPL; ++e) v[e] = s_o[(w * 16 + i) * D + e * 32 + lane];
-            join<VPL>(m, l, acc, make_float2(s_ml[(w * 16 + i) * 2], s_ml[(w * 16 + i) * 2 + 1]), v);
+            for (int e = 0; e < VPL; ++e) acc[e] += c * v[e];
         }
         if (S == 1) {
             finish(i, m, l, acc);
         } else {
-#pragma unroll
-            for (int e = 0; e < VPL; ++e) p.tail_o[(mine + i) * D + e * 32 + lane] = acc[e];
+            store_row<D>(p.tail_o + (mine + i) * D, acc);
             if (lane == 0) *reinterpret_cast<float2*>(p.tail_ml + (mine + i) * 2) = make_float2(m, l);
         }
     }
@@ -551,12 +605,11 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
     __syncthreads();
     if (!s_last) return;
     if (p.splits > 0) pdl_wait();
-    const size_t parts = ((size_t)seq * p.n_kv_heads + kvh) * S * 16;
     for (int i = warp; i < rows; i += 4) {
         float m = -INFINITY, l = 0.f, acc[VPL];
 #pragma unroll
         for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
-        join_parts<VPL>(m, l, acc, p.tail_o, p.tail_ml, parts + i, 16, S);
+        join_parts<D>(m, l, acc, p.tail_o, p.tail_ml, ((size_t)seq * p.n_kv_heads + kvh) * S * 16 + i, 16, S, s_w + i * MAX_PARTS);
         finish(i, m, l, acc);
     }
 }
@@ -578,23 +631,23 @@ template <int D> static cudaError_t tail(const AttnSharedParams& p, cudaStream_t
 
 }  // namespace ash
 
-// Parts of the keys: as many CTAs of the prefix as fill the GPU once, two tiles of keys in each at least; tails like the decode kernel's.
+// Parts of the keys: as many CTAs as fill the GPU once, two tiles (pages) of keys in each at least.
 AttnSharedPlan attn_shared_plan(int n_seqs, int rows_per_seq, int n_heads, int n_kv_heads, int head_dim, int max_shared, int max_tail, int max_tickets) {
     AttnSharedPlan plan = {0, 1, 0, 0};
     const int G = n_heads / n_kv_heads;
     const long long rows = (long long)n_seqs * rows_per_seq * G;
     if (max_shared > 0 && rows > 0) {
-        const int per_cta = head_dim == 256 || rows <= ash::BQ ? ash::BQ : 2 * ash::BQ, bk = head_dim == 256 ? 64 : 128;
+        const int per_cta = head_dim == 256 || rows <= ash::BQ ? ash::BQ : 2 * ash::BQ, bk = ash::PAGE;
         const long long ctas = (rows + per_cta - 1) / per_cta * n_kv_heads, tiles = (max_shared + bk - 1) / bk;
         long long s = 148 / ctas;
         if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
-        if (s > 64) s = 64;
+        if (s > ash::MAX_PARTS) s = ash::MAX_PARTS;
         plan.splits = s < 1 ? 1 : (int)s;
     }
     const long long pairs = (long long)n_seqs * n_kv_heads, pages = (max_tail + ash::PAGE - 1) / ash::PAGE;
-    long long t = pairs > 0 ? (296 + pairs - 1) / pairs : 1;
+    long long t = pairs > 0 ? 148 * (head_dim == 256 ? 1 : head_dim == 128 ? 2 : 4) / pairs : 1;
     if (t > (pages + 1) / 2) t = (pages + 1) / 2;
-    if (t > 64) t = 64;
+    if (t > ash::MAX_PARTS) t = ash::MAX_PARTS;
     plan.tail_splits = t < 1 || pairs > max_tickets ? 1 : (int)t;
     plan.prefix_rows = rows * n_kv_heads * plan.splits;
     plan.tail_rows = plan.tail_splits > 1 ? pairs * plan.tail_splits * 16 : 0;

@@ -212,8 +212,8 @@ int attn_decode_shared(const Tensor& q, const Tensor& kv, const Tensor& out, con
     same_device(q, tickets, "tickets"); same_device(q, status, "status");
     want(status, torch::kInt32, "status");
     const int* t = ints(tickets, "tickets");
-    const llm::AttnSharedPlan plan = llm::attn_shared_plan(p.n_seqs, p.rows_per_seq, p.n_heads, p.n_kv_heads, p.head_dim, std::min(max_shared, table),
-                                                           std::min(max_tail ? max_tail : table, table), tickets.numel());
+    const int64_t most = std::min(max_shared, table), rest = std::max<int64_t>(table - most, 64);
+    const llm::AttnSharedPlan plan = llm::attn_shared_plan(p.n_seqs, p.rows_per_seq, p.n_heads, p.n_kv_heads, p.head_dim, most, max_tail ? std::min(max_tail, table) : rest, tickets.numel());
     const c10::cuda::CUDAGuard guard(q.device());
     p.splits = plan.splits; p.tail_splits = plan.tail_splits; p.tickets = reinterpret_cast<unsigned*>(const_cast<int*>(t));
     const int64_t rows = plan.prefix_rows + plan.tail_rows;
