@@ -28,6 +28,12 @@ constexpr float RESCALE_STEP = 8.f;
 
 // keys of the prefix, and whether sequence `b` takes part
 LLM_DEVICE int prefix_of(const AttnSharedParams& p) { return p.splits > 0 ? max(0, min(*p.shared_len, p.max_pages * PAGE)) : 0; }
+// tiles of the prefix in a part, and the parts that have any
+LLM_DEVICE int tiles_per_part(int prefix, int splits) { return ((prefix + PAGE - 1) / PAGE + splits - 1) / splits; }
+LLM_DEVICE int parts_of(int prefix, int splits) {
+    const int per = tiles_per_part(prefix, splits);
+    return per > 0 ? ((prefix + PAGE - 1) / PAGE + per - 1) / per : 0;
+}
 LLM_DEVICE bool shares(const AttnSharedParams& p, int b, int prefix) { return p.seq_lens[b] - (p.rows_per_seq - 1) >= prefix; }
 
 // ------------------------------------------------------------------------------------------------
@@ -63,14 +69,10 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
     const int kvh = blockIdx.y, split = blockIdx.z, G = p.n_heads / p.n_kv_heads;
     const int rows_all = p.n_seqs * p.rows_per_seq * G, row_first = blockIdx.x * (SLOTS * BQ);
     const bool both = SLOTS == 2 && row_first + BQ < rows_all;
-    const int keys = prefix_of(p), tiles = (keys + BK - 1) / BK, per = (tiles + p.splits - 1) / p.splits;
+    const int keys = prefix_of(p), tiles = (keys + BK - 1) / BK, per = tiles_per_part(keys, p.splits);
     const int tile0 = split * per, nt = min(tiles, tile0 + per) - tile0;
     const size_t part = ((size_t)kvh * rows_all + row_first) * p.splits + split;        // of the first row; the next one is `splits` further
-    if (nt <= 0) {                                         // uniform for the CTA, before any barrier or allocation
-        for (int i = tid; i < SLOTS * BQ; i += X::THREADS)
-            if (row_first + i < rows_all) *reinterpret_cast<float2*>(p.part_ml + (part + (size_t)i * p.splits) * 2) = make_float2(-INFINITY, 0.f);
-        return;
-    }
+    if (nt <= 0) return;                                   // uniform for the CTA, before any barrier or allocation; nobody reads this part
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = smem_u32(s_bars);
     auto bar = [&](int i) { return bars + i * 8; };
@@ -336,55 +338,62 @@ template <int D> LLM_DEVICE void store_row(float* x, const float (&v)[D / 32]) {
         for (int e = 0; e < D / 32; e += 4) *reinterpret_cast<float4*>(x + column<D>(e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
 }
-// `n` <= MAX_PARTS sets of keys, whose results lie `step` rows apart, join a row.  The maxima and sums of all of them first, a lane each, which gives every set its
-// weight (kept in `w`); then the values, many sets on their way at a time.
-template <int D> LLM_DEVICE void join_parts(float& m, float& l, float (&acc)[D / 32], const float* part_o, const float* part_ml, size_t first, int step, int n, float* w) {
-    constexpr int N = D / 32, DEEP = 64 / N > 16 ? 16 : 64 / N;
+// `n` <= MAX_PARTS sets of keys, whose results lie `step` rows apart, join two rows.  Maxima and sums of all sets first, a lane each, which gives every set its
+// weight (kept in `w`); the values of many sets of both rows are on their way meanwhile (a row after the other, eight sets at a time, it was 17000 clocks for six rows of 18
+// parts of 256).
+template <int D> LLM_DEVICE void join_parts(float (&m)[2], float (&l)[2], float (&acc)[2][D / 32], const float* part_o, const float* part_ml, const size_t (&first)[2], int step, int n,
+                                            float* const (&w)[2]) {
+    constexpr int N = D / 32, DEEP = N == 2 ? 16 : 8;
     const int lane = threadIdx.x & 31;
-    float2 ml[2];
-    float top = m;
+    float2 ml[2][2];
+    float v[2][DEEP][N];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int s = k * 32 + lane;
-        ml[k] = s < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + (first + (size_t)s * step) * 2)) : make_float2(-INFINITY, 0.f);
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int s = k * 32 + lane;
+            ml[r][k] = s < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + (first[r] + (size_t)s * step) * 2)) : make_float2(-INFINITY, 0.f);
+        }
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) load_row<D>(part_o + (first[r] + (size_t)min(s0 + k, n - 1) * step) * D, v[r][k]);
+    };
+    load(0);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const float top = fmaxf(m[r], warp_max(fmaxf(ml[r][0].x, ml[r][1].x))), base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float c = ex2(ml[r][k].x - base);
+            sum += c * ml[r][k].y;
+            w[r][k * 32 + lane] = c;
+        }
+        const float old = ex2(m[r] - base);
+        l[r] = l[r] * old + warp_sum(sum);
+        m[r] = top;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[r][e] *= old;
     }
-    float v[DEEP][N];
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k) load_row<D>(part_o + (first + (size_t)min(k, n - 1) * step) * D, v[k]);
-    top = fmaxf(top, warp_max(fmaxf(ml[0].x, ml[1].x)));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const bool none = ml[k].x == -INFINITY && ml[k].y == 0.f;      // no keys there: nothing was written either
-        const float c = none ? 0.f : exp2f(ml[k].x - base);
-        sum += none ? 0.f : c * ml[k].y;
-        w[k * 32 + lane] = none ? -1.f : c;
-    }
-    const float old = l == 0.f && m == -INFINITY ? 0.f : exp2f(m - base);
-    l = l * old + warp_sum(sum);
-    m = top;
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] *= old;
     __syncwarp();
     for (int s0 = 0; s0 < n; s0 += DEEP) {
-        if (s0 > 0) {
+        if (s0 > 0) load(s0);
 #pragma unroll
-            for (int k = 0; k < DEEP; ++k) load_row<D>(part_o + (first + (size_t)min(s0 + k, n - 1) * step) * D, v[k]);
-        }
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int k = 0; k < DEEP; ++k) {
-            const float c = s0 + k < n ? w[s0 + k] : -1.f;
-            if (c < 0.f) continue;
+            for (int k = 0; k < DEEP; ++k) {
+                const float c = w[r][s0 + k];               // (0 from n on)
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] += c * v[k][e];
-        }
+                for (int e = 0; e < N; ++e) acc[r][e] += c * v[r][k][e];
+            }
     }
     __syncwarp();
 }
 
 template <int D>
-__global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p) {
+__global__ void __launch_bounds__(128, D == 64 ? 4 : D == 128 ? 3 : 1) attn_tail_kernel(const AttnSharedParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     using SM = Tail<D>;
     pdl_trigger();
@@ -552,16 +561,23 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
     }
     __syncthreads();
 
-    // the prefix, the quotient, the gate
-    auto finish = [&](int i, float m, float l, float (&acc)[VPL]) {
-        if (joins) join_parts<D>(m, l, acc, p.part_o, p.part_ml, ((size_t)kvh * p.n_seqs * rows + (size_t)seq * rows + i) * p.splits, 1, p.splits, s_w + i * MAX_PARTS);
+    // the quotient and the gate
+    struct Gate { __nv_bfloat16 x[VPL]; };
+    auto gate_of = [&](int i) {                              // on its way while the parts are
+        Gate g;
+        const __nv_bfloat16* x = p.gate + (size_t)(seq * R + i / G) * p.gate_token + (size_t)(kvh * G + i % G) * p.gate_head;
+#pragma unroll
+        for (int e = 0; e < VPL; ++e) g.x[e] = p.gate ? x[column<D>(e)] : __nv_bfloat16();
+        return g;
+    };
+    auto finish = [&](int i, float l, float (&acc)[VPL], const Gate& g) {
         const size_t token = (size_t)seq * R + i / G;
         const int head = kvh * G + i % G;
         const float inv = l == 0.f ? 0.f : 1.f / l;          // (a sum that is not a number makes the row one)
 #pragma unroll
         for (int e = 0; e < VPL; ++e) {
             acc[e] = l == 0.f ? 0.f : acc[e] * inv;
-            if (p.gate) acc[e] *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[token * p.gate_token + (size_t)head * p.gate_head + column<D>(e)])));
+            if (p.gate) acc[e] *= __fdividef(1.f, 1.f + __expf(-__bfloat162float(g.x[e])));
         }
         __nv_bfloat16* dst = p.out + (token * p.n_heads + head) * D;
 #pragma unroll
@@ -569,26 +585,44 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
     };
     const int S = (int)gridDim.y;
     const size_t mine = (((size_t)seq * p.n_kv_heads + kvh) * S + split) * 16;
+    // rows i and i + 4 (the same one twice at the end): the prefix's parts join them
+    auto prefix_parts = [&](int i, int i2, float (&m)[2], float (&l)[2], float (&acc)[2][VPL]) {
+        const size_t first = ((size_t)kvh * p.n_seqs + seq) * rows;
+        const size_t at[2] = {(first + i) * p.splits, (first + i2) * p.splits};
+        float* const w[2] = {s_w + i * MAX_PARTS, s_w + i2 * MAX_PARTS};
+        join_parts<D>(m, l, acc, p.part_o, p.part_ml, at, 1, parts_of(prefix, p.splits), w);
+    };
     if (S == 1 && p.splits > 0) pdl_wait();                  // the prefix kernel's parts
-    for (int i = warp; i < rows; i += 4) {
-        float m = -INFINITY, l = 0.f, acc[VPL];
+    for (int i = warp; i < rows; i += 8) {
+        const int i2 = i + 4 < rows ? i + 4 : i;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[2][VPL] = {};
+        Gate g[2] = {gate_of(i), gate_of(i2)};
+        if (S == 1 && joins) prefix_parts(i, i2, m, l, acc);
 #pragma unroll
-        for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
-        for (int w = 0; w < sets; ++w) m = fmaxf(m, s_ml[(w * 16 + i) * 2]);
-        for (int w = 0; w < sets; ++w) {
-            const float wm = s_ml[(w * 16 + i) * 2], c = wm == -INFINITY ? 0.f : exp2f(wm - m);
-            if (c == 0.f && s_ml[(w * 16 + i) * 2 + 1] == 0.f) continue;     // no keys there
-            float v[VPL];
-            load_row_shared<D>(&s_o[(w * 16 + i) * ROW], v);
-            l += c * s_ml[(w * 16 + i) * 2 + 1];
+        for (int r = 0; r < 2; ++r) {
+            const int row = r ? i2 : i;
+            if (r && i2 == i) break;
+            float top = m[r];
+            for (int w = 0; w < sets; ++w) top = fmaxf(top, s_ml[(w * 16 + row) * 2]);
+            const float base = top == -INFINITY ? 0.f : top, old = ex2(m[r] - base);
+            l[r] *= old;
 #pragma unroll
-            for (int e = 0; e < VPL; ++e) acc[e] += c * v[e];
-        }
-        if (S == 1) {
-            finish(i, m, l, acc);
-        } else {
-            store_row<D>(p.tail_o + (mine + i) * D, acc);
-            if (lane == 0) *reinterpret_cast<float2*>(p.tail_ml + (mine + i) * 2) = make_float2(m, l);
+            for (int e = 0; e < VPL; ++e) acc[r][e] *= old;
+#pragma unroll 2
+            for (int w = 0; w < sets; ++w) {
+                const float wm = s_ml[(w * 16 + row) * 2], wl = s_ml[(w * 16 + row) * 2 + 1], c = ex2(wm - base);
+                float v[VPL];
+                load_row_shared<D>(&s_o[(w * 16 + row) * ROW], v);
+                l[r] += c * wl;
+#pragma unroll
+                for (int e = 0; e < VPL; ++e) acc[r][e] += c * v[e];
+            }
+            if (S == 1) {
+                finish(row, l[r], acc[r], g[r]);
+            } else {
+                store_row<D>(p.tail_o + (mine + row) * D, acc[r]);
+                if (lane == 0) *reinterpret_cast<float2*>(p.tail_ml + (mine + row) * 2) = make_float2(top, l[r]);
+            }
         }
     }
     if (S == 1) return;
@@ -605,12 +639,16 @@ __global__ void __launch_bounds__(128) attn_tail_kernel(const AttnSharedParams p
     __syncthreads();
     if (!s_last) return;
     if (p.splits > 0) pdl_wait();
-    for (int i = warp; i < rows; i += 4) {
-        float m = -INFINITY, l = 0.f, acc[VPL];
-#pragma unroll
-        for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
-        join_parts<D>(m, l, acc, p.tail_o, p.tail_ml, ((size_t)seq * p.n_kv_heads + kvh) * S * 16 + i, 16, S, s_w + i * MAX_PARTS);
-        finish(i, m, l, acc);
+    for (int i = warp; i < rows; i += 8) {
+        const int i2 = i + 4 < rows ? i + 4 : i;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[2][VPL] = {};
+        const size_t first = ((size_t)seq * p.n_kv_heads + kvh) * S * 16;
+        const size_t at[2] = {first + i, first + i2};
+        float* const w[2] = {s_w + i * MAX_PARTS, s_w + i2 * MAX_PARTS};
+        join_parts<D>(m, l, acc, p.tail_o, p.tail_ml, at, 16, S, w);
+        if (joins) prefix_parts(i, i2, m, l, acc);
+        finish(i, l[0], acc[0], gate_of(i));
+        if (i2 != i) finish(i2, l[1], acc[1], gate_of(i2));
     }
 }
 

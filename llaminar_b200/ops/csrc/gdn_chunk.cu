@@ -28,6 +28,7 @@
 
 #include "hybrid.h"
 #include "launch.h"
+#include "pairs.cuh"
 #include "tc_tile.cuh"
 
 namespace llm {
@@ -165,28 +166,6 @@ LLM_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     lo = pack_half(a - h.x, b - h.y);
 }
 
-// two numbers at a time
-typedef unsigned long long f32x2;
-LLM_DEVICE f32x2 pair(float a, float b) {
-    f32x2 v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-LLM_DEVICE float2 both(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
 LLM_DEVICE void split2(f32x2 v, uint32_t& hi, uint32_t& lo) {
     const float2 x = both(v);
     hi = pack_half(x.x, x.y);

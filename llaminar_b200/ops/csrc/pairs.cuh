@@ -1,0 +1,29 @@
+// Two 32-bit numbers in one 64-bit register: the packed FP32 instructions, which do twice the work of an issue slot.
+#pragma once
+#include "common.cuh"
+
+namespace llm {
+
+typedef unsigned long long f32x2;
+LLM_DEVICE f32x2 pair(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+LLM_DEVICE float2 both(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+}  // namespace llm

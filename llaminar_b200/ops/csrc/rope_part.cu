@@ -10,36 +10,13 @@
 // (reference: src/v2/kernels/cuda/ops/CUDARoPEKernels.cu, ring append of src/v2/kernels/cuda/kvcache/CUDARingKVCache.cu.)
 #include <cuda_fp16.h>
 
-#include "common.cuh"
 #include "hybrid.h"
 #include "launch.h"
+#include "pairs.cuh"
 
 namespace llm {
 
 constexpr int PAGE = 64, WARPS = 4;
-
-// two numbers at a time
-typedef unsigned long long f32x2;
-LLM_DEVICE f32x2 pair(float a, float b) {
-    f32x2 v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-LLM_DEVICE float2 both(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
 
 // N bf16 values as they lie in memory (N = 2, 4, 8)
 template <int N> struct Raw {
