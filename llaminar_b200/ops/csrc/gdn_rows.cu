@@ -5,9 +5,9 @@
 //     a = exp(ssm_a softplus(alpha + dt_bias))       b = sigmoid(beta)
 //     u = b (v - a S^T k)       S = a S + k u^T      o = S^T q       out = o / rms(o) * norm_w * silu(z)
 //
-// A CTA has one value head of one sequence; two neighbouring threads keep a column of the d x d state in registers, so that both products with the state are
-// sums inside a thread (and one exchange) and a row costs no barrier.  q, k and v of a block of four rows are convolved, normed and left in shared memory
-// first; the loads of the state, of the rows and of the gates are all on their way together.
+// A CTA takes one value head of one sequence after the other; four neighbouring threads keep a column of the d x d state in registers, so that both products
+// with the state are sums inside a thread (and two exchanges) and a row costs no barrier.  q, k and v of a block of four rows are convolved, normed and left in shared memory
+// first; the next state, rows and gates are on their way meanwhile.
 // What bounds it: few rows, the state's bytes (64 KB read per head at d = 128; written too unless the state is left alone); more rows, the chain of a row.
 //
 // gdn_commit brings the state behind the accepted rows: a streaming pass, S = A S + sum_r k_r (u_r prod_{s > r} a_s)^T, bound by the
@@ -41,154 +41,171 @@ LLM_DEVICE GdnSeq gdn_seq(const GdnParams& p, int b) {
     return s;
 }
 
-// K4: four taps, a row loaded once per channel; another number of taps loads rows again.
+// Four neighbouring threads have a column of the state, a quarter of its rows each.  What the next block of rows (or the next item's first one) needs is loaded
+// while a block is at work, and the state of the next item too.  K4: four taps; another number of taps loads its rows when it needs them.
 template <int D, bool KEEP, bool K4>
-__global__ void __launch_bounds__(2 * D, D == 128 ? 2 : 4) gdn_rows_kernel(const GdnParams p) {
-    constexpr int WARPS = 2 * D / 32, EPL = D / 32, HALF = D / 2, ROW = D + 4;             // the second half of a vector starts four banks further
-    constexpr int MINE = (TB + WARPS - 1) / WARPS;           // rows of a block that a warp finishes
+__global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
+    constexpr int THREADS = 4 * D, WARPS = THREADS / 32, EPL = D / 32, QUARTER = D / 4, ROW = D + 16;        // a quarter of a vector starts four banks behind the one before
     __shared__ __align__(16) float s_q[TB][ROW], s_k[TB][ROW];
     __shared__ float s_v[TB][D], s_o[TB][D], s_a[TB], s_b[TB];
-    extern __shared__ __align__(16) float s_state[];         // [D][D]; the second half of the rows with its columns XORed by 16, so that a column's two threads meet other banks
+    extern __shared__ __align__(16) float s_state[];         // two states [D][D], a quarter's 16-byte units XORed so that a column's four threads meet other banks
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int j = tid >> 1, part = tid & 1;                  // column of the state, half of its rows
-    const int items = p.n_seqs * p.n_v;
-    // the state of an item, on its way while the item before it is at work
-    auto fetch = [&](int item) {
-        if (item < items) {
-            const GdnSeq q = gdn_seq(p, item / p.n_v);
-            if (q.rows > 0 && !q.fresh) {
-                const float* from = p.rec + (q.slot * p.n_v + item % p.n_v) * (size_t)(D * D);
+    const int j = tid >> 2, part = tid & 3;                  // column of the state, quarter of its rows
+    const int items = p.n_seqs * p.n_v, K = K4 ? 4 : p.K;
+    auto seq_of = [&](int item) { return gdn_seq(p, min(item, items - 1) / p.n_v); };
+    auto unit_of = [](int row, int u) { return u ^ (2 * (row / QUARTER)) % (D / 4); };       // 16-byte unit u of a row of the state
+
+    auto fetch = [&](int item, const GdnSeq& q, int buffer) {
+        if (item < items && q.rows > 0 && !q.fresh) {
+            const float* from = p.rec + (q.slot * p.n_v + item % p.n_v) * (size_t)(D * D);
+            float* to = s_state + buffer * D * D;
 #pragma unroll 8
-                for (int u = tid; u < D * D / 4; u += 2 * D) {
-                    const int row = u / (D / 4), at = u % (D / 4) ^ (row >= HALF ? 4 : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s_state + row * D + at * 4)), "l"(from + (size_t)u * 4) : "memory");
-                }
+            for (int u = tid; u < D * D / 4; u += THREADS) {
+                const int row = u / (D / 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to + row * D + unit_of(row, u % (D / 4)) * 4)), "l"(from + (size_t)u * 4) : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    fetch(blockIdx.x);
+
+    // this thread's channel: of q, k and v in the first three quarters of the threads
+    const int kind = tid / D, i_ch = tid % D;
+    auto channel = [&](int h) {
+        const int kh = (h + p.v_head_offset) % p.n_k;
+        return (kind == 0 ? kh : kind == 1 ? p.n_k + kh : 2 * p.n_k + h) * D + i_ch;
+    };
+    struct Block {                                           // of rows, as they were loaded
+        float before[3], w[4];
+        __nv_bfloat16 x[TB + 3], z[(TB + WARPS - 1) / WARPS][EPL], alpha, beta;
+    };
+    constexpr int MINE = (TB + WARPS - 1) / WARPS;           // rows of a block that a warp finishes
+    auto load = [&](int item, const GdnSeq& q, int t0, Block& k) {
+        const int h = item % p.n_v, last = q.rows - 1;
+        if (q.rows == 0) return;
+        if (K4 && kind < 3) {
+            const int c = channel(h);
+#pragma unroll
+            for (int i = 0; i < TB + 3; ++i) k.x[i] = p.in[(size_t)(q.first + min(max(t0 + i - 3, 0), last)) * p.in_row + c];        // (behind the last row: that one)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k.w[i] = p.conv_w[(size_t)c * 4 + i];
+            if (t0 == 0 && !q.fresh) {
+                const float* x = p.conv + (q.slot * p.C + c) * (size_t)3;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) k.before[i] = x[i];
+            }
+        }
+        if (kind == 3 && i_ch < TB) {
+            const __nv_bfloat16* ab = p.in + (size_t)(q.first + min(t0 + i_ch, last)) * p.in_row + p.ab_off;
+            k.alpha = ab[h];
+            k.beta = ab[p.n_v + h];
+        }
+#pragma unroll
+        for (int r = 0; r < MINE; ++r) {
+            const __nv_bfloat16* x = p.in + (size_t)(q.first + min(t0 + r * WARPS + warp, last)) * p.in_row + p.z_off + h * D;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                if (r * WARPS + warp < TB) k.z[r][e] = x[e * 32 + lane];
+        }
+    };
+
+    int item = blockIdx.x, buffer = 0;
+    GdnSeq q = seq_of(item), q1 = seq_of(item + gridDim.x);
+    fetch(item, q, 0);
+    Block now;
+    load(item, q, 0, now);
     float gain[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) gain[e] = p.norm_w[e * 32 + lane];
 
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int h = item % p.n_v, b = item / p.n_v;
-        const GdnSeq q = gdn_seq(p, b);
+    for (; item < items; item += gridDim.x, buffer ^= 1) {
+        const int h = item % p.n_v, b = item / p.n_v, next = item + gridDim.x;
+        const GdnSeq q2 = seq_of(next + gridDim.x);          // used by the item after this one
+        fetch(next, q1, buffer ^ 1);
         if (q.rows == 0) {
-            fetch(item + gridDim.x);
+            if (next < items) load(next, q1, 0, now);
+            q = q1; q1 = q2;
             continue;
         }
-        const int K = K4 ? 4 : p.K, kh = (h + p.v_head_offset) % p.n_k;
-        const float* window = p.conv + q.slot * (size_t)p.C * (K - 1);
-        float* state = p.rec + ((q.slot * p.n_v + h) * D + part * HALF) * (size_t)D + j;
-        const float ssm_a = p.ssm_a[h], dt = p.dt_bias[h];
-        // this thread's channel of q (first half of the threads) or k, and of v (first half)
-        const int c_qk = tid < D ? kh * D + tid : (p.n_k + kh) * D + tid - D, c_v = 2 * p.n_k * D + h * D + tid;
-
-        // channel c of n rows from t0: convolution and SiLU
-        auto convolved = [&](int c, int t0, int n, float (&y)[TB]) {
-            auto row = [&](int t) { return p.in[(size_t)(q.first + min(t, q.rows - 1)) * p.in_row + c]; };      // (behind the last row: that one)
-            auto before = [&](int t) { return q.fresh ? 0.f : window[(size_t)c * (K - 1) + (K - 1 + t)]; };    // t < 0
-            if (K4) {
-                float x[TB + 3], w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = p.conv_w[(size_t)c * 4 + i];
-                __nv_bfloat16 in[TB + 3];
-#pragma unroll
-                for (int i = 0; i < TB + 3; ++i) in[i] = row(max(t0 + i - 3, 0));
-                if (t0 == 0) {
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) x[i] = before(i - 3);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) x[i] = __bfloat162float(in[i]);
-                }
-#pragma unroll
-                for (int i = 3; i < TB + 3; ++i) x[i] = __bfloat162float(in[i]);
-#pragma unroll
-                for (int i = 0; i < TB; ++i) y[i] = w[0] * x[i] + w[1] * x[i + 1] + w[2] * x[i + 2] + w[3] * x[i + 3];
-            } else {
-#pragma unroll
-                for (int i = 0; i < TB; ++i) y[i] = 0.f;
-                for (int i = 0; i < K; ++i) {
-                    const float w = p.conv_w[(size_t)c * K + i];
-#pragma unroll
-                    for (int r = 0; r < TB; ++r) {
-                        const int t = t0 + r + i - (K - 1);
-                        y[r] += w * (t >= 0 ? __bfloat162float(row(t)) : before(t));
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < TB; ++i) y[i] = silu(y[i]);
-        };
-
-        f32x2 S[HALF / 2];
+        float* state = p.rec + ((q.slot * p.n_v + h) * D + part * QUARTER) * (size_t)D + j;
+        f32x2 S[QUARTER / 2];
+#pragma unroll 1
         for (int t0 = 0; t0 < q.rows; t0 += TB) {
             const int n = min(TB, q.rows - t0);
-            __nv_bfloat16 z[MINE][EPL];                          // of the rows that this warp finishes
+            // ---- convolution, SiLU, gates ----
+            if (kind < 3) {
+                float y[TB];
+                if (K4) {
+                    float x[TB + 3];
 #pragma unroll
-            for (int r = 0; r < MINE; ++r) {
-                const __nv_bfloat16* x = p.in + (size_t)(q.first + min(t0 + r * WARPS + warp, q.rows - 1)) * p.in_row + p.z_off + h * D;
+                    for (int i = 0; i < TB + 3; ++i) x[i] = i < 3 && t0 == 0 ? q.fresh ? 0.f : now.before[i % 3] : __bfloat162float(now.x[i]);
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) z[r][e] = x[e * 32 + lane];
-            }
-            float alpha = 0.f, beta = 0.f;
-            if (tid < n) {
-                const __nv_bfloat16* ab = p.in + (size_t)(q.first + t0 + tid) * p.in_row + p.ab_off;
-                alpha = __bfloat162float(ab[h]);
-                beta = __bfloat162float(ab[p.n_v + h]);
-            }
-            float y[TB], v[TB];
-            convolved(c_qk, t0, n, y);
-            if (tid < D) convolved(c_v, t0, n, v);
-            float(*to)[ROW] = tid < D ? s_q : s_k;
-            const int i_qk = tid & (D - 1), at = i_qk + (i_qk >= HALF ? 4 : 0);
+                    for (int i = 0; i < TB; ++i) y[i] = now.w[0] * x[i] + now.w[1] * x[i + 1] + now.w[2] * x[i + 2] + now.w[3] * x[i + 3];
+                } else {
+                    const int c = channel(h);
 #pragma unroll
-            for (int i = 0; i < TB; ++i) {
-                to[i][at] = y[i];
-                if (tid < D) s_v[i][tid] = v[i];
+                    for (int r = 0; r < TB; ++r) y[r] = 0.f;
+                    for (int i = 0; i < K; ++i) {
+                        const float w = p.conv_w[(size_t)c * K + i];
+#pragma unroll
+                        for (int r = 0; r < TB; ++r) {
+                            const int t = t0 + r + i - (K - 1);
+                            y[r] += w * (t >= 0 ? __bfloat162float(p.in[(size_t)(q.first + min(t, q.rows - 1)) * p.in_row + c]) : q.fresh ? 0.f : p.conv[(q.slot * p.C + c) * (size_t)(K - 1) + (K - 1 + t)]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    const float v = silu(y[i]);
+                    if (kind == 2) s_v[i][i_ch] = v;
+                    else (kind ? s_k : s_q)[i][i_ch + i_ch / QUARTER * 4] = v;
+                }
+            } else if (i_ch < n) {
+                const float x = __bfloat162float(now.alpha) + p.dt_bias[h];
+                s_a[i_ch] = expf(p.ssm_a[h] * (x > 20.f ? x : log1pf(expf(x))));
+                s_b[i_ch] = 1.f / (1.f + expf(-__bfloat162float(now.beta)));
             }
-            if (tid < n) {
-                const float x = alpha + dt;
-                s_a[tid] = expf(ssm_a * (x > 20.f ? x : log1pf(expf(x))));
-                s_b[tid] = 1.f / (1.f + expf(-beta));
-            }
+            float z[MINE][EPL];
+#pragma unroll
+            for (int r = 0; r < MINE; ++r)
+#pragma unroll
+                for (int e = 0; e < EPL; ++e) z[r][e] = __bfloat162float(now.z[r][e]);
+            // the next block is on its way from here on
+            if (t0 + TB < q.rows) load(item, q, t0 + TB, now);
+            else if (next < items) load(next, q1, 0, now);
             __syncthreads();
-            for (int i = warp; i < 2 * n; i += WARPS) {          // a warp norms one vector
+            // ---- norms, a warp per vector ----
+            for (int i = warp; i < 2 * n; i += WARPS) {
                 float* x = i < n ? s_q[i] : s_k[i - n];
-                float ss = 0.f, e_v[EPL];
+                float ss = 0.f, v[EPL];
 #pragma unroll
                 for (int e = 0; e < EPL; ++e) {
                     const int k = e * 32 + lane;
-                    e_v[e] = x[k + (k >= HALF ? 4 : 0)];
-                    ss += e_v[e] * e_v[e];
+                    v[e] = x[k + k / QUARTER * 4];
+                    ss += v[e] * v[e];
                 }
                 const float r = rsqrtf(warp_sum(ss) + 1e-6f) * (i < n ? rsqrtf((float)D) : 1.f);
 #pragma unroll
                 for (int e = 0; e < EPL; ++e) {
                     const int k = e * 32 + lane;
-                    x[k + (k >= HALF ? 4 : 0)] = e_v[e] * r;
-                    if (KEEP && i >= n) p.keep_k[((size_t)(q.first + t0 + i - n) * p.n_v + h) * D + k] = e_v[e] * r;
+                    x[k + k / QUARTER * 4] = v[e] * r;
+                    if (KEEP && i >= n) p.keep_k[((size_t)(q.first + t0 + i - n) * p.n_v + h) * D + k] = v[e] * r;
                 }
             }
-            if (t0 == 0) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                __syncthreads();
-                const float* x = s_state + part * HALF * D + (j ^ (part << 4));
-#pragma unroll
-                for (int i = 0; i < HALF / 2; ++i) S[i] = q.fresh ? pair(0.f, 0.f) : pair(x[2 * i * D], x[(2 * i + 1) * D]);
-            }
+            if (t0 == 0) asm volatile("cp.async.wait_group 1;" ::: "memory");     // this item's state; the next one's may still be on its way
             __syncthreads();
-            if (t0 == 0) fetch(item + gridDim.x);
+            if (t0 == 0) {
+                const float* x = s_state + buffer * D * D + part * QUARTER * D + unit_of(part * QUARTER, j >> 2) * 4 + (j & 3);
+#pragma unroll
+                for (int i = 0; i < QUARTER / 2; ++i) S[i] = q.fresh ? pair(0.f, 0.f) : pair(x[2 * i * D], x[(2 * i + 1) * D]);
+            }
+            // ---- the rows ----
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
                 const float a = s_a[i];
-                const float4 *k = reinterpret_cast<const float4*>(&s_k[i][part * (HALF + 4)]), *x = reinterpret_cast<const float4*>(&s_q[i][part * (HALF + 4)]);
+                const float4 *k = reinterpret_cast<const float4*>(&s_k[i][part * (QUARTER + 4)]), *x = reinterpret_cast<const float4*>(&s_q[i][part * (QUARTER + 4)]);
                 f32x2 d0 = pair(0.f, 0.f), d1 = d0, o0 = d0, o1 = d0;
 #pragma unroll
-                for (int e = 0; e < HALF / 4; ++e) {
+                for (int e = 0; e < QUARTER / 4; ++e) {
                     const float4 f = k[e];
                     d0 = fma2(S[2 * e], pair(f.x, f.y), d0);
                     d1 = fma2(S[2 * e + 1], pair(f.z, f.w), d1);
@@ -196,9 +213,10 @@ __global__ void __launch_bounds__(2 * D, D == 128 ? 2 : 4) gdn_rows_kernel(const
                 const float2 e0 = both(d0), e1 = both(d1);
                 float dot = (e0.x + e0.y) + (e1.x + e1.y);
                 dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+                dot += __shfl_xor_sync(0xffffffffu, dot, 2);
                 const float u = s_b[i] * (s_v[i][j] - a * dot);
 #pragma unroll
-                for (int e = 0; e < HALF / 4; ++e) {
+                for (int e = 0; e < QUARTER / 4; ++e) {
                     const float4 f = k[e], g = x[e];
                     S[2 * e] = fma2(pair(f.x, f.y), pair(u, u), mul2(S[2 * e], pair(a, a)));
                     S[2 * e + 1] = fma2(pair(f.z, f.w), pair(u, u), mul2(S[2 * e + 1], pair(a, a)));
@@ -208,18 +226,20 @@ __global__ void __launch_bounds__(2 * D, D == 128 ? 2 : 4) gdn_rows_kernel(const
                 const float2 f0 = both(o0), f1 = both(o1);
                 float o = (f0.x + f0.y) + (f1.x + f1.y);
                 o += __shfl_xor_sync(0xffffffffu, o, 1);
+                o += __shfl_xor_sync(0xffffffffu, o, 2);
                 if (part == 0) {
                     s_o[i][j] = o;
                     if (KEEP) {
-                        const size_t at_row = (size_t)(q.first + t0 + i) * p.n_v + h;
-                        p.keep_u[at_row * D + j] = u;
-                        if (j == 0) p.keep_a[at_row] = a;
+                        const size_t at = (size_t)(q.first + t0 + i) * p.n_v + h;
+                        p.keep_u[at * D + j] = u;
+                        if (j == 0) p.keep_a[at] = a;
                     }
                 }
             }
             __syncthreads();
+            // ---- gated norm, a warp per row ----
 #pragma unroll
-            for (int r = 0; r < MINE; ++r) {                     // gated norm, a warp per row
+            for (int r = 0; r < MINE; ++r) {
                 const int i = r * WARPS + warp;
                 if (i >= n) break;
                 float ss = 0.f;
@@ -228,23 +248,24 @@ __global__ void __launch_bounds__(2 * D, D == 128 ? 2 : 4) gdn_rows_kernel(const
                 const float f = rsqrtf(warp_sum(ss) / D + p.eps);
                 __nv_bfloat16* dst = p.out + (size_t)(q.first + t0 + i) * p.out_row + h * D;
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) dst[e * 32 + lane] = __float2bfloat16(s_o[i][e * 32 + lane] * f * gain[e] * silu(__bfloat162float(z[r][e])));
+                for (int e = 0; e < EPL; ++e) dst[e * 32 + lane] = __float2bfloat16(s_o[i][e * 32 + lane] * f * gain[e] * silu(z[r][e]));
             }
         }
-        if (KEEP) {                                              // a share of the convolution's inputs, for the commit
+        if (KEEP) {                                          // a share of the convolution's inputs, for the commit
             const int c0 = (int)((long long)p.C * h / p.n_v), c1 = (int)((long long)p.C * (h + 1) / p.n_v);
-            for (int i = tid; i < (c1 - c0) * q.rows; i += 2 * D) {
+            for (int i = tid; i < (c1 - c0) * q.rows; i += THREADS) {
                 const int t = i / (c1 - c0), c = c0 + i % (c1 - c0);
                 p.keep_x[((size_t)b * p.rows_per_seq + t) * p.C + c] = p.in[(size_t)(q.first + t) * p.in_row + c];
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < HALF / 2; ++i) {
+            for (int i = 0; i < QUARTER / 2; ++i) {
                 const float2 x = both(S[i]);
                 state[(size_t)(2 * i) * D] = x.x;
                 state[(size_t)(2 * i + 1) * D] = x.y;
             }
         }
+        q = q1; q1 = q2;
     }
 }
 
@@ -320,13 +341,14 @@ __global__ void __launch_bounds__(256) gdn_commit_kernel(const GdnParams p, cons
 LLM_DEFINE_BOUNDS_STATUS_READER(bounds_status_gdn_rows)
 
 template <int D> static cudaError_t rows_of(const GdnParams& p, cudaStream_t st) {
-    constexpr int SMEM = D * D * 4, CTAS = D == 128 ? 2 : 4;                  // CTAs of an SM
+    constexpr int SMEM = 2 * D * D * 4;
     const long long items = (long long)p.n_v * p.n_seqs;
     if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
+    const int ctas = 148 * (D == 128 ? 1 : D == 64 ? 2 : 4);                  // as many as fit at once
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)(items < 148 * CTAS ? items : 148 * CTAS), 2 * D, SMEM, st>>>(p);
+        kernel<<<(unsigned)(items < ctas ? items : ctas), 4 * D, SMEM, st>>>(p);
         return cudaGetLastError();
     };
     if (p.keep_u) return p.K == 4 ? go(gdn_rows_kernel<D, true, true>) : go(gdn_rows_kernel<D, true, false>);
