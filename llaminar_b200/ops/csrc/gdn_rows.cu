@@ -17,10 +17,12 @@
 //  src/v2/models/qwen35/Qwen35Graph.cpp:886-887.)
 #include "hybrid.h"
 #include "pairs.cuh"
+#include "tc_tile.cuh"
 
 namespace llm {
 
 constexpr int TB = 4;                                        // rows prepared together
+constexpr int DRAFT_ROWS = 8;                                // most rows of a sequence that are drafts
 
 struct GdnSeq {
     int first, rows;
@@ -269,6 +271,214 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
     }
 }
 
+// Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, a quarter each, 32 bytes further than the one before: a
+// column's four threads meet other banks.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
+// them.)  o comes from the state in front of the row, S^T q = a S0^T q + u (k.q), so that a row has one round of sums.
+template <int D, int TB, bool K4>
+__global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) {
+    using namespace tc5;
+    constexpr int THREADS = 4 * D, WARPS = THREADS / 32, EPL = D / 32, QUARTER = D / 4, ROW = D + 16, STRIDE = QUARTER * D + 8;
+    __shared__ __align__(16) float s_q[TB][ROW], s_k[TB][ROW];
+    __shared__ float s_v[TB][D], s_o[TB][D], s_a[TB], s_b[TB], s_kq[TB];
+    __shared__ __align__(8) uint64_t s_bar[2];
+    __shared__ int s_abort[2];                               // [1] stays 0 here (tc_common.cuh: restarts the wait clock when set)
+    extern __shared__ __align__(16) float s_state[];         // two states of four quarters, STRIDE apart
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int j = tid >> 2, part = tid & 3;
+    const int items = p.n_seqs * p.n_v, K = K4 ? 4 : p.K, n = p.rows_per_seq;
+    const uint32_t bars = smem_u32(s_bar);
+    volatile int* abort_flag = s_abort;
+    if (tid == 0) {
+        s_abort[0] = 0; s_abort[1] = 0;
+        mbar_init(bars, 1);
+        mbar_init(bars + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    __syncthreads();
+    auto slot_of = [&](int item) { return (size_t)LLM_CHECK_INDEX(p.slots[item / p.n_v], p.n_slots); };
+    auto fetch = [&](int item, size_t slot, int buffer) {    // by one thread
+        const float* from = p.rec + (slot * p.n_v + item % p.n_v) * (size_t)(D * D);
+        fence_proxy_async();                                 // what stood there has been read
+        mbar_arrive_expect_tx(bars + buffer * 8, D * D * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bulk_load(smem_u32(s_state + (buffer * 4 + i) * STRIDE), from + i * QUARTER * D, QUARTER * D * 4, bars + buffer * 8);
+    };
+    const int kind = tid / D, i_ch = tid % D;                // this thread's channel: of q, k and v in the first three quarters of the threads
+    struct Rows {                                            // an item's, as they were loaded
+        float before[3], w[4], ssm_a, dt;
+        __nv_bfloat16 x[TB], z[EPL], alpha, beta;
+    };
+    auto channel = [&](int h) {
+        const int kh = (h + p.v_head_offset) % p.n_k;
+        return (kind == 0 ? kh : kind == 1 ? p.n_k + kh : 2 * p.n_k + h) * D + i_ch;
+    };
+    auto load = [&](int item, size_t slot, Rows& r) {
+        const int h = item % p.n_v, first = item / p.n_v * n;
+        if (kind < 3) {
+            const int c = channel(h);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) r.x[i] = p.in[(size_t)(first + min(i, n - 1)) * p.in_row + c];
+            if (K4) {
+                const float* window = p.conv + (slot * p.C + c) * (size_t)3;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r.w[i] = p.conv_w[(size_t)c * 4 + i];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) r.before[i] = window[i];
+            }
+        } else if (i_ch < n) {
+            const __nv_bfloat16* ab = p.in + (size_t)(first + i_ch) * p.in_row + p.ab_off;
+            r.alpha = ab[h]; r.beta = ab[p.n_v + h];
+            r.ssm_a = p.ssm_a[h]; r.dt = p.dt_bias[h];
+        }
+        if (warp < n) {
+            const __nv_bfloat16* x = p.in + (size_t)(first + warp) * p.in_row + p.z_off + h * D;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) r.z[e] = x[e * 32 + lane];
+        }
+    };
+    int item = blockIdx.x, buffer = 0;
+    uint32_t phase = 0;                                      // of both barriers: it turns with every second item
+    size_t slot = slot_of(item), slot1 = slot_of(min(item + (int)gridDim.x, items - 1));
+    if (tid == 0) fetch(item, slot, 0);
+    Rows now;
+    load(item, slot, now);
+    float gain[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) gain[e] = p.norm_w[e * 32 + lane];
+    for (; item < items; item += gridDim.x) {
+        const int h = item % p.n_v, b = item / p.n_v, first = b * n, next = item + gridDim.x;
+        if (tid == 0 && next < items) fetch(next, slot1, buffer ^ 1);          // (its place was read two barriers ago)
+        const size_t slot2 = slot_of(min(next + (int)gridDim.x, items - 1));
+        // ---- convolution, SiLU, gates ----
+        if (kind < 3) {
+            const int c = channel(h);
+            float y[TB];
+            if (K4) {
+                float x[TB + 3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x[i] = now.before[i];
+#pragma unroll
+                for (int i = 0; i < TB; ++i) x[i + 3] = __bfloat162float(now.x[i]);
+#pragma unroll
+                for (int i = 0; i < TB; ++i) y[i] = now.w[0] * x[i] + now.w[1] * x[i + 1] + now.w[2] * x[i + 2] + now.w[3] * x[i + 3];
+            } else {
+                const float* window = p.conv + (slot * p.C + c) * (size_t)(K - 1);
+#pragma unroll
+                for (int r = 0; r < TB; ++r) y[r] = 0.f;
+                for (int i = 0; i < K; ++i) {
+                    const float w = p.conv_w[(size_t)c * K + i];
+#pragma unroll
+                    for (int r = 0; r < TB; ++r) {
+                        const int t = r + i - (K - 1);
+                        y[r] += w * (t >= 0 ? __bfloat162float(p.in[(size_t)(first + min(t, n - 1)) * p.in_row + c]) : window[K - 1 + t]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                if (i >= n) break;
+                const float v = silu(y[i]);
+                if (kind == 2) s_v[i][i_ch] = v;
+                else (kind ? s_k : s_q)[i][i_ch + i_ch / QUARTER * 4] = v;
+                // the convolution's inputs, for the commit: a channel of q and k by the first value head that reads it
+                if (kind == 2 || (h < p.n_k && p.n_v >= p.n_k)) p.keep_x[((size_t)b * n + i) * p.C + c] = now.x[i];
+            }
+        } else {
+            if (i_ch < n) {
+                const float x = __bfloat162float(now.alpha) + now.dt;
+                s_a[i_ch] = expf(now.ssm_a * (x > 20.f ? x : log1pf(expf(x))));
+                s_b[i_ch] = 1.f / (1.f + expf(-__bfloat162float(now.beta)));
+            }
+            if (p.n_v < p.n_k) {                             // key heads that no value head reads: all of q and k, shared out
+                const int all = 2 * p.n_k * D, c0 = (int)((long long)all * h / p.n_v), c1 = (int)((long long)all * (h + 1) / p.n_v);
+                for (int c = c0 + i_ch; c < c1; c += D)
+                    for (int i = 0; i < n; ++i) p.keep_x[((size_t)b * n + i) * p.C + c] = p.in[(size_t)(first + i) * p.in_row + c];
+            }
+        }
+        float z[EPL];                                        // of the row that this warp finishes
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) z[e] = __bfloat162float(now.z[e]);
+        if (next < items) load(next, slot1, now);            // on their way from here on
+        __syncthreads();
+        // ---- norms and k.q, a warp per row ----
+        if (warp < n) {
+            float qs = 0.f, ks = 0.f, kq = 0.f, q[EPL], k[EPL];
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                q[e] = s_q[warp][to]; k[e] = s_k[warp][to];
+                qs += q[e] * q[e]; ks += k[e] * k[e]; kq += k[e] * q[e];
+            }
+            const float rq = rsqrtf(warp_sum(qs) + 1e-6f) * rsqrtf((float)D), rk = rsqrtf(warp_sum(ks) + 1e-6f);
+            kq = warp_sum(kq) * rq * rk;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                s_q[warp][to] = q[e] * rq; s_k[warp][to] = k[e] * rk;
+                p.keep_k[((size_t)(first + warp) * p.n_v + h) * D + at] = k[e] * rk;
+            }
+            if (lane == 0) s_kq[warp] = kq;
+        }
+        mbar_wait_warp(bars + buffer * 8, phase, abort_flag);
+        f32x2 S[QUARTER / 2];
+        {
+            const float* x = s_state + (buffer * 4 + part) * STRIDE + j;
+#pragma unroll
+            for (int i = 0; i < QUARTER / 2; ++i) S[i] = pair(x[2 * i * D], x[(2 * i + 1) * D]);
+        }
+        __syncthreads();
+        if (abort_flag[0]) break;
+        // ---- the rows ----
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const float a = s_a[i];
+            const float4 *k4 = reinterpret_cast<const float4*>(&s_k[i][part * (QUARTER + 4)]), *q4 = reinterpret_cast<const float4*>(&s_q[i][part * (QUARTER + 4)]);
+            f32x2 d0 = pair(0.f, 0.f), d1 = d0, o0 = d0, o1 = d0, k[QUARTER / 2];
+#pragma unroll
+            for (int e = 0; e < QUARTER / 4; ++e) {
+                const float4 f = k4[e], g = q4[e];
+                k[2 * e] = pair(f.x, f.y); k[2 * e + 1] = pair(f.z, f.w);
+                d0 = fma2(S[2 * e], k[2 * e], d0);
+                d1 = fma2(S[2 * e + 1], k[2 * e + 1], d1);
+                o0 = fma2(S[2 * e], pair(g.x, g.y), o0);
+                o1 = fma2(S[2 * e + 1], pair(g.z, g.w), o1);
+            }
+            const float2 e0 = both(d0), e1 = both(d1), f0 = both(o0), f1 = both(o1);
+            float dot = (e0.x + e0.y) + (e1.x + e1.y), o = (f0.x + f0.y) + (f1.x + f1.y);
+            dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+            o += __shfl_xor_sync(0xffffffffu, o, 1);
+            dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+            o += __shfl_xor_sync(0xffffffffu, o, 2);
+            const float u = s_b[i] * (s_v[i][j] - a * dot);
+#pragma unroll
+            for (int e = 0; e < QUARTER / 2; ++e) S[e] = fma2(k[e], pair(u, u), mul2(S[e], pair(a, a)));
+            if (part == 0) {
+                s_o[i][j] = fmaf(a, o, u * s_kq[i]);
+                const size_t at = (size_t)(first + i) * p.n_v + h;
+                p.keep_u[at * D + j] = u;
+                if (j == 0) p.keep_a[at] = a;
+            }
+        }
+        __syncthreads();
+        // ---- gated norm, a warp per row ----
+        if (warp < n) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) ss += s_o[warp][e * 32 + lane] * s_o[warp][e * 32 + lane];
+            const float f = rsqrtf(warp_sum(ss) / D + p.eps);
+            __nv_bfloat16* dst = p.out + (size_t)(first + warp) * p.out_row + h * D;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) dst[e * 32 + lane] = __float2bfloat16(s_o[warp][e * 32 + lane] * f * gain[e] * silu(z[e]));
+        }
+        slot = slot1; slot1 = slot2;
+        phase ^= (uint32_t)buffer;
+        buffer ^= 1;
+    }
+    __syncthreads();
+    teardown(abort_flag, tid, p.status);
+}
+
 // One thread per channel of a sequence.  K - 1 values of [old window | rows], from the `n`th on; kept rows come from keep_x.
 template <bool KEPT>
 LLM_DEVICE void gdn_shift(const GdnParams& p, const GdnSeq& q, int b, int c, int n) {
@@ -354,8 +564,30 @@ template <int D> static cudaError_t rows_of(const GdnParams& p, cudaStream_t st)
     if (p.keep_u) return p.K == 4 ? go(gdn_rows_kernel<D, true, true>) : go(gdn_rows_kernel<D, true, false>);
     return p.K == 4 ? go(gdn_rows_kernel<D, false, true>) : go(gdn_rows_kernel<D, false, false>);
 }
+template <int D> static cudaError_t drafts_of(const GdnParams& p, cudaStream_t st) {
+    constexpr int SMEM = 2 * (D * D + 4 * 8) * 4, CTAS = D == 128 ? 1 : D == 64 ? 2 : 4;       // CTAs of an SM
+    const long long items = (long long)p.n_v * p.n_seqs;
+    if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
+    auto go = [&](auto kernel) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return e;
+        kernel<<<(unsigned)(items < 148 * CTAS ? items : 148 * CTAS), 4 * D, SMEM, st>>>(p);
+        return cudaGetLastError();
+    };
+    constexpr int MOST = D == 32 ? 4 : DRAFT_ROWS;           // a warp finishes a row
+    if (p.rows_per_seq > 4 && MOST > 4) return p.K == 4 ? go(gdn_draft_kernel<D, MOST, true>) : go(gdn_draft_kernel<D, MOST, false>);
+    return p.K == 4 ? go(gdn_draft_kernel<D, 4, true>) : go(gdn_draft_kernel<D, 4, false>);
+}
 cudaError_t launch_gdn_rows(const GdnParams& p, cudaStream_t st) {
     if (p.n_seqs == 0 || p.n_rows == 0) return cudaSuccess;
+    if (p.keep_u && p.rows_per_seq <= (p.d == 32 ? 4 : DRAFT_ROWS)) {
+        switch (p.d) {
+            case 32: return drafts_of<32>(p, st);
+            case 64: return drafts_of<64>(p, st);
+            case 128: return drafts_of<128>(p, st);
+            default: return cudaErrorNotSupported;
+        }
+    }
     switch (p.d) {
         case 32: return rows_of<32>(p, st);
         case 64: return rows_of<64>(p, st);

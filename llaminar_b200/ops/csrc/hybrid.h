@@ -25,6 +25,7 @@ struct GdnParams {
     // and the convolution's inputs [C]
     float *keep_a, *keep_k, *keep_u;
     __nv_bfloat16* keep_x;
+    int* status;                                             // drafted rows: receives STATUS_TIMEOUT if a wait gave up
 };
 // rows one after the other, any number of them; d of 32, 64 or 128.  With keep_*: the state stays as it is.
 cudaError_t launch_gdn_rows(const GdnParams& p, cudaStream_t st);

@@ -102,10 +102,14 @@ void keep_args(llm::GdnParams& p, const Tensor& like, const std::vector<Tensor>&
 }
 
 int gdn_verify(const Tensor& in, int64_t C, int64_t z_off, int64_t ab_off, const Tensor& conv_w, const Tensor& ssm_a, const Tensor& dt_bias, const Tensor& norm_w,
-               const Tensor& conv, const Tensor& rec, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps, const std::vector<Tensor>& keep) {
+               const Tensor& conv, const Tensor& rec, const Tensor& slots, const Tensor& out, int64_t n_k, int64_t v_head_offset, double eps, const std::vector<Tensor>& keep,
+               const Tensor& status) {
     llm::GdnParams p = gdn_params(in, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv, rec, slots, out, n_k, v_head_offset, eps);
     keep_args(p, in, keep);
     TORCH_CHECK(in.size(0) == (int64_t)p.n_seqs * p.rows_per_seq, "in must have the same number of rows for every sequence");
+    same_device(in, status, "status");
+    want(status, torch::kInt32, "status");
+    p.status = status.data_ptr<int>();
     const c10::cuda::CUDAGuard guard(in.device());
     check(llm::launch_gdn_rows(p, stream()), "gdn_verify");
     return 1;

@@ -78,7 +78,7 @@ def gdn_verify(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torch
     f = lambda *s: torch.empty(*s, dtype=torch.float32, device=inp.device)
     st = GdnStash(f(B, R, n_v), f(B, R, n_v, d), f(B, R, n_v, d), torch.empty(B, R, C, dtype=torch.bfloat16, device=inp.device), slots, n_k)
     _count(ext().gdn_verify(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, slots, out, n_k, v_head_offset, eps,
-                            [st.decay, st.key, st.correction, st.inputs]))
+                            [st.decay, st.key, st.correction, st.inputs], scratch_for(inp.device).status))
     return st
 
 
