@@ -68,6 +68,8 @@ class ForwardBatch:
     seq_lens: torch.Tensor | None = None     # [B] cache length including this step's rows
     rows_per_seq: int = 1
     n_splits: int = 1
+    shared_len: torch.Tensor | None = None   # [1] leading tokens whose pages stand in front of every sequence's table (row 0 has them)
+    max_shared: int = 0                      # the same on the host, or a bound (0: nothing is shared): how the keys are shared out
     # prefill-style attention
     cu_q: torch.Tensor | None = None         # [B + 1]
     ctx_lens: torch.Tensor | None = None     # [B]
@@ -326,8 +328,8 @@ class CudaModel:
         self.gdn_v_local = pl.gdn_v_stop - pl.gdn_v_start
         self.gdn_conv_local = 2 * c.gdn_key_dim + self.gdn_v_local * c.ssm_state
         # hybrid models whose softmax blocks have a head size without an attention kernel here (qwen3.5 checkpoints use 256)
-        # run attention on PyTorch ops: decode steps as one batched, shape-static expression that CUDA graphs capture,
-        # prefill chunks sequence by sequence
+        # run prefill attention on PyTorch ops, sequence by sequence (and decode steps of head sizes that no kernel takes as one batched,
+        # shape-static expression that CUDA graphs capture)
         self.torch_attention = c.is_hybrid and c.head_dim not in (64, 128)
         self.graph_safe = True
         self.layers = [self._build_layer(weights, i) for i in self.layer_ids]
@@ -540,7 +542,10 @@ class CudaModel:
                     self.n_heads_local, self.n_kv_local, c.head_dim, c.rope_theta, c.rms_eps)
         scale = 1.0 / math.sqrt(c.head_dim)
         o3 = o.view(T, self.n_heads_local, c.head_dim)
-        if fb.is_decode:
+        if fb.is_decode and fb.max_shared:
+            ops.attn_decode_shared(q, kv_layer, o3, fb.block_table, fb.seq_lens, fb.shared_len, self.n_heads_local, self.n_kv_local,
+                                   c.head_dim, fb.rows_per_seq, scale, self.scratch, max_shared=fb.max_shared)
+        elif fb.is_decode:
             ops.attn_decode(q, kv_layer, o3, fb.block_table, fb.seq_lens, self.n_heads_local, self.n_kv_local,
                             c.head_dim, fb.rows_per_seq, scale, fb.n_splits, self.scratch)
         else:
@@ -549,19 +554,29 @@ class CudaModel:
                              self.n_kv_local, c.head_dim, scale, fb.max_q_len, scratch=self.scratch, max_kv_len=fb.max_kv_len)
         return o
 
+    def shares_prefixes(self, rows_per_seq: int = 1) -> bool:
+        """Whether decode steps can take the keys that all their sequences share once for all (`ops.attn_decode_shared`)."""
+        return (self.stack is None and self.cfg.head_dim in ops.SHARED_HEAD_SIZES and self.n_heads_local % self.n_kv_local == 0
+                and self.n_heads_local // self.n_kv_local * rows_per_seq <= 16)
+
     def _linear_attention(self, L: CudaLayer, fb: ForwardBatch, inp: torch.Tensor, T: int) -> torch.Tensor:
         """Between the input and output projections of a Gated-DeltaNet block.  Decode steps (one row per sequence) run
-        the two step kernels on the sequences' state slots; prefill chunks run the chunk-parallel form on PyTorch ops,
-        sequence by sequence (one host synchronisation per forward pass for the row ranges)."""
+        the two step kernels on the sequences' state slots, prefill chunks the chunk-parallel kernels, and a deferred pass (drafts) leaves the
+        states alone and a stash behind.  State sizes without a kernel run on PyTorch ops, sequence by sequence."""
         c, hs = self.cfg, self._kv.hybrid
         d, nv = c.ssm_state, self.gdn_v_local
         o = self.ws_gdn_o[:T]
         conv, rec = hs.conv[L.gdn_index], hs.rec[L.gdn_index]
+        C, kernels = self.gdn_conv_local, d in ops.GDN_HEAD_SIZES
+        args = (inp, C, L.z_off, L.ab_off, L.conv_w, L.ssm_a, L.dt_bias, L.ssm_norm, conv, rec)
+        if fb.defer_state and kernels:
+            hs.stash[L.gdn_index] = ops.gdn_verify(*args, fb.state_slots, o, c.ssm_k_heads, self.plan.gdn_v_start, c.rms_eps)
+            hs.stash_slots = fb.state_slots.long()
+            return o
         from ..models import gdn
         if fb.defer_state:
             B = fb.state_slots.shape[0]
             x = inp.float().view(B, T // B, -1)
-            C = self.gdn_conv_local
             rows, hs.stash[L.gdn_index] = gdn.gdn_rows_deferred(
                 x[..., :C], x[..., L.z_off:L.z_off + nv * d], x[..., L.ab_off:L.ab_off + nv], x[..., L.ab_off + nv:L.ab_off + 2 * nv],
                 L.conv_w, L.ssm_a, L.dt_bias, L.ssm_norm, conv, rec, fb.state_slots.long(), c.ssm_k_heads, nv, d, c.rms_eps,
@@ -570,13 +585,14 @@ class CudaModel:
             o.copy_(rows)
             return o
         if fb.is_decode and fb.rows_per_seq == 1:
-            ops.gdn_step(inp, self.gdn_conv_local, L.z_off, L.ab_off, L.conv_w, L.ssm_a, L.dt_bias, L.ssm_norm, conv, rec,
-                         fb.state_slots, self.ws_gdn_y[:T], o, c.ssm_k_heads, self.plan.gdn_v_start, c.rms_eps)
+            ops.gdn_step(*args, fb.state_slots, self.ws_gdn_y[:T], o, c.ssm_k_heads, self.plan.gdn_v_start, c.rms_eps)
+            return o
+        if fb.cu_q is not None and kernels:
+            ops.gdn_prefill(*args, fb.positions, fb.cu_q, fb.state_slots, o, c.ssm_k_heads, self.plan.gdn_v_start, c.rms_eps)
             return o
         seqs = getattr(fb, "_gdn_seqs", None)
         if seqs is None:
             seqs = fb._gdn_seqs = gdn.batch_sequences(fb.seq_ids, fb.positions, fb.state_slots)
-        C = self.gdn_conv_local
         x = inp.float()
         rows = gdn.gdn_block_rows(x[:, :C], x[:, L.z_off:L.z_off + nv * d], x[:, L.ab_off:L.ab_off + nv],
                                   x[:, L.ab_off + nv:L.ab_off + 2 * nv], seqs, conv, rec, L.conv_w, L.ssm_a, L.dt_bias, L.ssm_norm,
@@ -584,48 +600,73 @@ class CudaModel:
         o.copy_(rows)
         return o
 
+    def _rope_freqs(self) -> torch.Tensor:
+        """Angle per position of every rotated pair of a head, in 64 bits on the device."""
+        f = getattr(self, "_freqs", None)
+        if f is None:
+            from ..models.config import Rotary
+            f = self._freqs = torch.tensor(Rotary(self.cfg.rotary_dim, self.cfg.rope_theta).frequencies(), dtype=torch.float64, device=self.device)
+        return f
+
     def _attention_gated(self, L: CudaLayer, fb: ForwardBatch, kv_layer: torch.Tensor, qkv: torch.Tensor, T: int) -> torch.Tensor:
         """Softmax block of the hybrid family: every head's projection rows are [query | gate], only the first `rotary_dim`
         values of a head are rotated, and the attention output is scaled by sigmoid(gate) before the output projection.
-        The split, QK-norm, rotation and cache append are PyTorch ops (a dozen small launches per block, one block in
-        four); attention itself runs the paged kernels for head sizes 64 and 128 and PyTorch otherwise."""
-        from ..models.reference import rmsnorm, rope_split_half
+        The split, QK-norm, rotation and cache append are one kernel; decode attention, gate included, another (two behind a shared prefix).
+        Prompts run the paged kernels for head sizes 64 and 128 and PyTorch otherwise, and the gate on PyTorch ops."""
         c = self.cfg
         H, Hk, D = self.n_heads_local, self.n_kv_local, c.head_dim
         if kv_layer.dtype == torch.uint8:
             raise NotImplementedError("the 8-bit KV cache is not available for the gated-attention blocks of hybrid models")
-        qw = 2 if c.attn_gate else 1
-        qg = qkv[:, :H * D * qw].view(T, H, qw, D)
-        q = qg[:, :, 0].float()
-        gate = qg[:, :, 1].reshape(T, H * D).float() if c.attn_gate else None
-        k = qkv[:, H * D * qw:H * D * qw + Hk * D].view(T, Hk, D).float()
-        v = qkv[:, H * D * qw + Hk * D:H * D * qw + 2 * Hk * D].view(T, Hk, D)
-        if L.q_norm is not None:
-            q, k = rmsnorm(q, L.q_norm, c.rms_eps), rmsnorm(k, L.k_norm, c.rms_eps)
-        pos = fb.positions.long()
-        q = rope_split_half(q, pos, c.rope_theta, c.rotary_dim)
-        k = rope_split_half(k, pos, c.rope_theta, c.rotary_dim)
-        page = fb.block_table.long()[fb.seq_ids.long(), pos // 64]
-        off = pos % 64
-        kv_layer[page, 0, :, off] = k.to(kv_layer.dtype)
-        kv_layer[page, 1, :, off] = v.to(kv_layer.dtype)
+        q = self.ws_q[:T]
+        gate = qkv[:, :2 * H * D].unflatten(1, (H, 2, D))[:, :, 1] if c.attn_gate else None
+        if D in ops.SHARED_HEAD_SIZES:
+            ops.rope_part_kv(qkv, q, kv_layer, L.q_norm, L.k_norm, self._rope_freqs(), 1.0, fb.positions, fb.seq_ids, fb.block_table, H, Hk, D,
+                             c.rms_eps, gated=c.attn_gate)
+        else:
+            self._append_torch(L, fb, kv_layer, qkv, T, q)
         o = self.ws_o[:T]
         o3 = o.view(T, H, D)
         scale = 1.0 / math.sqrt(D)
+        if fb.is_decode and self.shares_prefixes(fb.rows_per_seq):
+            shared = fb.shared_len if fb.max_shared else self._no_prefix()
+            ops.attn_decode_shared(q, kv_layer, o3, fb.block_table, fb.seq_lens, shared, H, Hk, D, fb.rows_per_seq, scale, self.scratch, gate=gate,
+                                   max_shared=fb.max_shared)
+            return o
         if self.torch_attention and fb.is_decode and fb.rows_per_seq == 1:
             o3.copy_(paged_decode_attention_torch(q, kv_layer, fb.block_table, fb.seq_lens, scale))
         elif self.torch_attention:
-            o3.copy_(self._attention_torch(q, fb, kv_layer, scale))
+            o3.copy_(self._attention_torch(q.float(), fb, kv_layer, scale))
+        elif fb.is_decode:
+            ops.attn_decode(q, kv_layer, o3, fb.block_table, fb.seq_lens, H, Hk, D, fb.rows_per_seq, scale, fb.n_splits, self.scratch)
         else:
-            qb = self.ws_q[:T]
-            qb.copy_(q)
-            if fb.is_decode:
-                ops.attn_decode(qb, kv_layer, o3, fb.block_table, fb.seq_lens, H, Hk, D, fb.rows_per_seq, scale, fb.n_splits, self.scratch)
-            else:
-                ops.attn_prefill(qb, kv_layer, o3, fb.block_table, fb.cu_q, fb.ctx_lens, H, Hk, D, scale, fb.max_q_len, scratch=self.scratch, max_kv_len=fb.max_kv_len)
+            ops.attn_prefill(q, kv_layer, o3, fb.block_table, fb.cu_q, fb.ctx_lens, H, Hk, D, scale, fb.max_q_len, scratch=self.scratch, max_kv_len=fb.max_kv_len)
         if gate is not None:
-            o.copy_(o.float() * torch.sigmoid(gate))
+            o3.copy_(o3.float() * torch.sigmoid(gate.float()))
         return o
+
+    def _no_prefix(self) -> torch.Tensor:
+        z = getattr(self, "_zero_len", None)
+        if z is None:
+            z = self._zero_len = torch.zeros(1, dtype=torch.int32, device=self.device)
+        return z
+
+    def _append_torch(self, L: CudaLayer, fb: ForwardBatch, kv_layer: torch.Tensor, qkv: torch.Tensor, T: int, q_out: torch.Tensor) -> None:
+        """Norm, rotation and cache append of head sizes without a kernel, on PyTorch ops."""
+        from ..models.reference import rmsnorm, rope_split_half
+        c = self.cfg
+        H, Hk, D = self.n_heads_local, self.n_kv_local, c.head_dim
+        qw = 2 if c.attn_gate else 1
+        q = qkv[:, :H * D * qw].unflatten(1, (H, qw, D))[:, :, 0].float()
+        k = qkv[:, H * D * qw:H * D * qw + Hk * D].unflatten(1, (Hk, D)).float()
+        v = qkv[:, H * D * qw + Hk * D:H * D * qw + 2 * Hk * D].unflatten(1, (Hk, D))
+        if L.q_norm is not None:
+            q, k = rmsnorm(q, L.q_norm, c.rms_eps), rmsnorm(k, L.k_norm, c.rms_eps)
+        pos = fb.positions.long()
+        q_out.copy_(rope_split_half(q, pos, c.rope_theta, c.rotary_dim))
+        k = rope_split_half(k, pos, c.rope_theta, c.rotary_dim)
+        page = fb.block_table.long()[fb.seq_ids.long(), pos // 64]
+        kv_layer[page, 0, :, pos % 64] = k.to(kv_layer.dtype)
+        kv_layer[page, 1, :, pos % 64] = v.to(kv_layer.dtype)
 
     def _attention_torch(self, q: torch.Tensor, fb: ForwardBatch, kv_layer: torch.Tensor, scale: float) -> torch.Tensor:
         return paged_attention_torch(q, kv_layer, fb.block_table, fb.seq_ids, fb.positions, scale)

@@ -119,9 +119,15 @@ class HybridState(StateSlots):
         """After a deferred pass over R rows per sequence: advance every layer's state of sequence i by its first
         ``n_rows[i]`` rows (the accepted ones) and drop the stash."""
         from ..models.gdn import commit_rows
-        n = torch.tensor(n_rows, dtype=torch.int64)
+        n, n_dev = torch.tensor(n_rows, dtype=torch.int64), None
         for layer, st in self.stash.items():
-            commit_rows(st, self.conv[layer], self.rec[layer], self.stash_slots, n)
+            if isinstance(st, tuple):
+                commit_rows(st, self.conv[layer], self.rec[layer], self.stash_slots, n)
+                continue
+            from .. import ops                 # kept by ops.gdn_verify
+            if n_dev is None:
+                n_dev = n.to(torch.int32).to(self.rec.device)
+            ops.gdn_commit(st, n_dev, self.conv[layer], self.rec[layer])
         self.stash.clear()
         self.stash_slots = None
 

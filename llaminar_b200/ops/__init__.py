@@ -421,4 +421,4 @@ def moe_topk(logits, k, renorm, ids, weights, counts=None) -> None:
     _count()
 
 
-from .hybrid import GdnStash, attn_decode_shared, gdn_commit, gdn_prefill, gdn_verify, rope_part_kv  # noqa: E402,F401
+from .hybrid import GDN_HEAD_SIZES, SHARED_HEAD_SIZES, GdnStash, attn_decode_shared, gdn_commit, gdn_prefill, gdn_verify, rope_part_kv  # noqa: E402,F401

@@ -15,6 +15,8 @@
 //
 // (reference: the recurrence of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu and the verifier's state capture rows,
 //  src/v2/models/qwen35/Qwen35Graph.cpp:886-887.)
+#include <algorithm>
+
 #include "hybrid.h"
 #include "pairs.cuh"
 #include "tc_tile.cuh"
@@ -554,24 +556,25 @@ template <int D> static cudaError_t rows_of(const GdnParams& p, cudaStream_t st)
     constexpr int SMEM = 2 * D * D * 4;
     const long long items = (long long)p.n_v * p.n_seqs;
     if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
-    const int ctas = 148 * (D == 128 ? 1 : D == 64 ? 2 : 4);                  // as many as fit at once
+    const unsigned ctas = (unsigned)std::min<long long>(items, 148 * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)(items < ctas ? items : ctas), 4 * D, SMEM, st>>>(p);
+        kernel<<<ctas, 4 * D, SMEM, st>>>(p);
         return cudaGetLastError();
     };
     if (p.keep_u) return p.K == 4 ? go(gdn_rows_kernel<D, true, true>) : go(gdn_rows_kernel<D, true, false>);
     return p.K == 4 ? go(gdn_rows_kernel<D, false, true>) : go(gdn_rows_kernel<D, false, false>);
 }
 template <int D> static cudaError_t drafts_of(const GdnParams& p, cudaStream_t st) {
-    constexpr int SMEM = 2 * (D * D + 4 * 8) * 4, CTAS = D == 128 ? 1 : D == 64 ? 2 : 4;       // CTAs of an SM
+    constexpr int SMEM = 2 * (D * D + 4 * 8) * 4;
     const long long items = (long long)p.n_v * p.n_seqs;
     if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
+    const unsigned ctas = (unsigned)std::min<long long>(items, 148 * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)(items < 148 * CTAS ? items : 148 * CTAS), 4 * D, SMEM, st>>>(p);
+        kernel<<<ctas, 4 * D, SMEM, st>>>(p);
         return cudaGetLastError();
     };
     constexpr int MOST = D == 32 ? 4 : DRAFT_ROWS;           // a warp finishes a row

@@ -28,6 +28,8 @@ def ext():
     return mod
 
 
+GDN_HEAD_SIZES = (32, 64, 128)
+SHARED_HEAD_SIZES = (64, 128, 256)     # of rope_part_kv and attn_decode_shared
 GDN_CHUNK = 64                 # rows of a chunk
 GDN_CHUNK_MIN_ROWS = 8         # rows per sequence, on average, from which the chunk form is taken
 GDN_WORKSPACE = 256 << 20      # bytes that a pass of the chunk form may hold; longer prompts take several passes
