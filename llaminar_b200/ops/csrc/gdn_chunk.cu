@@ -227,7 +227,13 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
         }
     }
     __syncthreads();
-    if (s_chunk[0] < 0) return;
+    // This kernel starts beside the scan of the pass before, which reads other memory.  The next launch waits for this one alone, so its last block waits for
+    // that scan.
+    const bool waits = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    if (s_chunk[0] < 0) {
+        if (waits) pdl_wait();
+        return;
+    }
     Chunk ch = {s_chunk[1], s_chunk[2], s_chunk[3], s_chunk[4], false};
     ch.fresh = p.positions[ch.first] == 0;
     const bool aligned = cp.in_aligned;
@@ -500,6 +506,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             *reinterpret_cast<uint4*>(head_chunk(cp, u, h0 + hi * p.n_k) + OFF_THI + half * TRI + to) = v;
         }
     }
+    if (waits) pdl_wait();
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -553,6 +560,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
     __shared__ int s_first[3];
     __shared__ float s_top[3][2][D];                        // largest magnitudes of a column, per math group
     __shared__ float s_inv[2][2][D];                        // inverse scales of S and U, by parity of the chunk
+    pdl_trigger();                                          // what comes next writes nothing that is read here
     const GdnParams& p = cp.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int h = blockIdx.x, b = blockIdx.y;
@@ -893,7 +901,7 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
     launches = 0;
     if (g.n_seqs == 0 || g.n_rows == 0) return cudaSuccess;
     if (g.d != gdc::D || (reinterpret_cast<uintptr_t>(workspace) & 1023)) return cudaErrorInvalidValue;
-    const int total = g.n_rows / gdc::C + g.n_seqs;         // no fewer than the sequences' chunks
+    const int total = g.n_seqs == 1 ? (g.n_rows + gdc::C - 1) / gdc::C : g.n_rows / gdc::C + g.n_seqs;       // no fewer than the sequences' chunks
     const size_t most = bytes / gdn_chunk_bytes(1, g.n_k, g.n_v);
     if (most < 1) return cudaErrorInvalidValue;
     gdc::ChunkParams p = {};
@@ -906,12 +914,25 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
     cudaError_t e = tc5::raise_smem(prep, gdc::PREP_SMEM);
     if (e == cudaSuccess) e = tc5::raise_smem(gdc::gdn_chunk_scan_kernel, gdc::SCAN_SMEM);
     if (e != cudaSuccess) return e;
-    for (int u0 = 0; u0 < total; u0 += p.units) {           // as many chunks at a time as the workspace holds
+    // One sequence's scan takes n_v SMs and leaves the others idle, so the next chunks are prepared beside it, in the other half of the workspace; the first
+    // pass is what one wave of blocks prepares.  (8192 rows of 48 heads: 945 us one after the other, 719 us so.)  The scans of several sequences run side by side instead, as long as the
+    // workspace holds all chunks.
+    const int wave = 2 * sm_count() / p.n_ks > 0 ? 2 * sm_count() / p.n_ks : 1;
+    const bool beside = total > wave && most > 1 && (g.n_seqs == 1 || (size_t)total > most);
+    size_t room = beside ? most / 2 : most;
+    if (room > 65535) room = 65535;
+    const int head = beside && (size_t)wave < room ? wave : (int)room;
+    const int more = total > head ? (total - head + (int)room - 1) / (int)room : 0;          // passes behind the first
+    const int each = more ? (total - head + more - 1) / more : 0;
+    for (int u0 = 0, pass = 0; u0 < total; u0 += p.units, ++pass) {
         p.u0 = u0;
-        p.units = (int)((size_t)(total - u0) < most ? (size_t)(total - u0) : most);
-        if (p.units > 65535) p.units = 65535;
-        prep<<<dim3(p.n_ks, p.units), gdc::PREP_THREADS, gdc::PREP_SMEM, st>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        p.ws = static_cast<uint8_t*>(workspace) + (beside && (pass & 1) ? room * gdn_chunk_bytes(1, g.n_k, g.n_v) : 0);
+        p.units = pass ? each : head;
+        if (p.units > total - u0) p.units = total - u0;
+        const dim3 grid(p.n_ks, p.units);
+        if (beside && pass) e = launch_pdl(prep, grid, dim3(gdc::PREP_THREADS), gdc::PREP_SMEM, st, p);
+        else { prep<<<grid, gdc::PREP_THREADS, gdc::PREP_SMEM, st>>>(p); e = cudaGetLastError(); }
+        if (e != cudaSuccess) return e;
         gdc::gdn_chunk_scan_kernel<<<dim3(g.n_v, g.n_seqs), gdc::THREADS, gdc::SCAN_SMEM, st>>>(p);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
         launches += 2;

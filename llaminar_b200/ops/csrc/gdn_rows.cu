@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "hybrid.h"
+#include "launch.h"
 #include "pairs.cuh"
 #include "tc_tile.cuh"
 
@@ -498,8 +499,8 @@ LLM_DEVICE void gdn_shift(const GdnParams& p, const GdnSeq& q, int b, int c, int
 __global__ void __launch_bounds__(256) gdn_windows_kernel(const GdnParams p) {
     const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
     const GdnSeq q = gdn_seq(p, b);
-    if (c >= p.C || q.rows == 0) return;
-    gdn_shift<false>(p, q, b, c, q.rows);
+    if (c < p.C && q.rows > 0) gdn_shift<false>(p, q, b, c, q.rows);
+    pdl_wait();                                             // (the scan of the chunk form reads no windows and runs beside this)
 }
 
 template <int D>
@@ -600,8 +601,7 @@ cudaError_t launch_gdn_rows(const GdnParams& p, cudaStream_t st) {
 }
 cudaError_t launch_gdn_windows(const GdnParams& p, cudaStream_t st) {
     if (p.n_seqs == 0 || p.n_rows == 0) return cudaSuccess;
-    gdn_windows_kernel<<<dim3((p.C + 255) / 256, p.n_seqs), 256, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_pdl(gdn_windows_kernel, dim3((p.C + 255) / 256, p.n_seqs), dim3(256), 0, st, p);
 }
 cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStream_t st) {
     if (p.n_seqs == 0 || p.rows_per_seq == 0) return cudaSuccess;
