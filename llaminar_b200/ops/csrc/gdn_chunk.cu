@@ -90,68 +90,105 @@ LLM_DEVICE uint2 four(const __nv_bfloat16* x, bool aligned) {
     if (aligned) return *reinterpret_cast<const uint2*>(x);
     return make_uint2(__bfloat16_as_ushort(x[0]) | (uint32_t)__bfloat16_as_ushort(x[1]) << 16, __bfloat16_as_ushort(x[2]) | (uint32_t)__bfloat16_as_ushort(x[3]) << 16);
 }
-LLM_DEVICE void add_tap(float4& y, const float4& w, const float4& x) { y.x += w.x * x.x; y.y += w.y * x.y; y.z += w.z * x.z; y.w += w.w * x.w; }
+LLM_DEVICE f32x2 two_of(uint32_t w) { return pair(bf16_lo(w), bf16_hi(w)); }
+LLM_DEVICE f32x2 silu2(f32x2 x) {                           // x / (1 + e^-x)
+    const float2 e = both(mul2(x, pair(-1.44269504f, -1.44269504f)));
+    float2 r = both(add2(pair(ex2(e.x), ex2(e.y)), pair(1.f, 1.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(r.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(r.y));
+    return mul2(x, pair(r.x, r.y));
+}
 
-// ROWS rows from t0 of the chunk, channels c .. c + 3: convolution and SiLU; zeros behind the chunk's rows.  K4: four taps, each row loaded once.
-// Rows are loaded without a branch, from places inside of the sequence, so that all of them are on their way together; then zeros take the place of what is
-// not there and the window that of what lies before the sequence's first row.
-template <int ROWS, bool K4>
-LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, float4 (&y)[ROWS]) {
+// Eight rows from t0 of the chunk and the three in front of them, channels c .. c + 3, as they lie.  They are loaded without a branch, from places inside of the
+// sequence, so that all of them are on their way together, and before the work that they do not depend on; `conv_rows` puts zeros in the place of what
+// lies behind the chunk's rows, and the window in that of what lies before the sequence's first one.
+constexpr int ROWS = 8;
+LLM_DEVICE const __nv_bfloat16* row_of(const GdnParams& p, const Chunk& ch, int t, int c) {
+    return p.in + (size_t)min(max(ch.row0 + t, ch.first), ch.row0 + ch.n - 1) * p.in_row + c;
+}
+LLM_DEVICE void load_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, uint2 (&raw)[ROWS + 3]) {
+    if (aligned) {
+#pragma unroll
+        for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row_of(p, ch, t0 + i - 3, c), true);
+    } else {
+#pragma unroll
+        for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row_of(p, ch, t0 + i - 3, c), false);
+    }
+}
+// Convolution and SiLU of those rows; zeros behind the chunk's.  K4: four taps; otherwise the rows are loaded again, tap by tap.
+template <bool K4>
+LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, bool w_aligned, const uint2 (&raw)[ROWS + 3], f32x2 (&y)[ROWS][2]) {
     const int K = K4 ? 4 : p.K;
-    auto tap = [&](int w) {
-        const float* x = p.conv_w + (size_t)c * K + w;
-        return make_float4(x[0], x[K], x[2 * K], x[3 * K]);
-    };
-    auto row = [&](int t) { return p.in + (size_t)min(max(ch.row0 + t, ch.first), ch.row0 + ch.n - 1) * p.in_row + c; };
-    auto value = [&](const uint2& x, int t) {
-        if (t >= ch.n) return make_float4(0.f, 0.f, 0.f, 0.f);
-        return make_float4(bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y));
-    };
-    auto before = [&](float4& x, int t) {                   // r < 0: of the window
+    auto before = [&](f32x2 (&x)[2], int t) {               // r < 0: of the window
         const int r = ch.row0 + t - ch.first;
         if (r >= 0) return;
+        x[0] = x[1] = pair(0.f, 0.f);
+        if (ch.fresh) return;
         const float* w = p.conv + ((size_t)ch.slot * p.C + c) * (K - 1) + (K - 1 + r);
-        x = ch.fresh ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(w[0], w[K - 1], w[2 * (K - 1)], w[3 * (K - 1)]);
+        x[0] = pair(w[0], w[K - 1]);
+        x[1] = pair(w[2 * (K - 1)], w[3 * (K - 1)]);
     };
     const bool edge = ch.row0 + t0 - (K - 1) < ch.first;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (K4) {
-        uint2 raw[ROWS + 3];
-        if (aligned) {
+        float4 taps[4];                                     // of a channel
+        const float* at = p.conv_w + (size_t)c * 4;
 #pragma unroll
-            for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row(t0 + i - 3), true);
-        } else {
+        for (int e = 0; e < 4; ++e) taps[e] = w_aligned ? *reinterpret_cast<const float4*>(at + 4 * e) : make_float4(at[4 * e], at[4 * e + 1], at[4 * e + 2], at[4 * e + 3]);
+        f32x2 x[ROWS + 3][2];
 #pragma unroll
-            for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row(t0 + i - 3), false);
+        for (int i = 0; i < ROWS + 3; ++i) {
+            const bool there = t0 + i - 3 < ch.n;
+            x[i][0] = two_of(there ? raw[i].x : 0u);
+            x[i][1] = two_of(there ? raw[i].y : 0u);
         }
-        const float4 w0 = tap(0), w1 = tap(1), w2 = tap(2), w3 = tap(3);
-        float4 x[ROWS + 3];
-#pragma unroll
-        for (int i = 0; i < ROWS + 3; ++i) x[i] = value(raw[i], t0 + i - 3);
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 3; ++i) before(x[i], t0 + i - 3);
         }
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) { add_tap(y[i], w0, x[i]); add_tap(y[i], w1, x[i + 1]); add_tap(y[i], w2, x[i + 2]); add_tap(y[i], w3, x[i + 3]); }
+        for (int e = 0; e < 2; ++e) {
+            const float4 a = taps[2 * e], b = taps[2 * e + 1];
+            const f32x2 w0 = pair(a.x, b.x), w1 = pair(a.y, b.y), w2 = pair(a.z, b.z), w3 = pair(a.w, b.w);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) y[i][e] = fma2(w3, x[i + 3][e], fma2(w2, x[i + 2][e], fma2(w1, x[i + 1][e], mul2(w0, x[i][e]))));
+        }
     } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) y[i][0] = y[i][1] = pair(0.f, 0.f);
         for (int w = 0; w < K; ++w) {
-            const float4 f = tap(w);
+            const float* f = p.conv_w + (size_t)c * K + w;
+            const f32x2 f0 = pair(f[0], f[K]), f1 = pair(f[2 * K], f[3 * K]);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
                 const int t = t0 + i + w - (K - 1);
-                float4 x = value(four(row(t), aligned), t);
+                const uint2 v = four(row_of(p, ch, t, c), aligned);
+                f32x2 x[2] = {two_of(t < ch.n ? v.x : 0u), two_of(t < ch.n ? v.y : 0u)};
                 if (edge) before(x, t);
-                add_tap(y[i], f, x);
+                y[i][0] = fma2(f0, x[0], y[i][0]);
+                y[i][1] = fma2(f1, x[1], y[i][1]);
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        if (t0 + i < ch.n) y[i] = make_float4(silu(y[i].x), silu(y[i].y), silu(y[i].z), silu(y[i].w));
-        else y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool there = t0 + i < ch.n;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) y[i][e] = there ? silu2(y[i][e]) : pair(0.f, 0.f);
     }
+}
+// Sums of eight numbers over the warp's lanes: a lane ends up with that of number lane / 4
+LLM_DEVICE float sums8(float (&v)[8], int lane) {
+#pragma unroll
+    for (int n = 4; n; n >>= 1) {
+        const bool up = lane & (4 * n);
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
+        }
+    }
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
 LLM_DEVICE uint32_t pack_half(float a, float b) {
@@ -184,6 +221,8 @@ LLM_DEVICE void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// byte of column c's values of rows 4 q .. 4 q + 3: neighbours both for a lane of every fourth column (who writes) and for a lane of each (who reads)
+LLM_DEVICE int val_at(int c, int q) { return q * (D * 16) + (c & 3) * (D * 4) + (((c >> 2) ^ (2 * (c & 3))) << 4); }
 // byte of 16-byte unit u (0 .. 15) of row t in an image of K or Q
 LLM_DEVICE int img_at(int t, int u) { return (u >> 3) * (IMG / 2) + t * 128 + (((u ^ t) & 7) << 4); }
 
@@ -199,7 +238,7 @@ struct ChunkParams {
     uint8_t* ws;                                            // [units][n_ks] chunks of key heads, then [units][n_v] of value heads
     int n_ks, u0, units;                                    // key heads in use, first chunk of this pass, chunks of it
     int* status;
-    int in_aligned, out_aligned;
+    int in_aligned, out_aligned, w_aligned;
 };
 LLM_DEVICE uint8_t* key_chunk(const ChunkParams& p, int u, int ks) { return p.ws + ((size_t)u * p.n_ks + ks) * KEY_BYTES; }
 LLM_DEVICE uint8_t* head_chunk(const ChunkParams& p, int u, int h) { return p.ws + (size_t)p.units * p.n_ks * KEY_BYTES + ((size_t)u * p.g.n_v + h) * HEAD_BYTES; }
@@ -207,9 +246,9 @@ LLM_DEVICE uint8_t* head_chunk(const ChunkParams& p, int u, int h) { return p.ws
 template <bool K4>
 __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const ChunkParams cp) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ double s_G[PREP_HEADS][C];
+    __shared__ __align__(16) float2 s_G[PREP_HEADS][C];          // a sum as a float and what that leaves of it
     __shared__ float s_b[PREP_HEADS][C];
-    __shared__ int s_chunk[5];
+    __shared__ int s_chunk[6];
     const GdnParams& p = cp.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ks = blockIdx.x, u = blockIdx.y;              // value heads ks, ks + n_k, ... read this key head
@@ -222,7 +261,10 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                 int first;
                 const int n = rows_of(p, b, first), row0 = first + (cp.u0 + u - at) * C;
                 s_chunk[1] = first; s_chunk[2] = row0; s_chunk[3] = min(C, first + n - row0);
-                s_chunk[4] = LLM_CHECK_INDEX(p.slots[b], p.n_slots);
+                if (row0 - (p.K - 1) < first) {             // the window is read here alone
+                    s_chunk[4] = LLM_CHECK_INDEX(p.slots[b], p.n_slots);
+                    s_chunk[5] = p.positions[first];
+                }
             }
         }
     }
@@ -234,27 +276,35 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
         if (waits) pdl_wait();
         return;
     }
-    Chunk ch = {s_chunk[1], s_chunk[2], s_chunk[3], s_chunk[4], false};
-    ch.fresh = p.positions[ch.first] == 0;
-    const bool aligned = cp.in_aligned;
+    const Chunk ch = {s_chunk[1], s_chunk[2], s_chunk[3], s_chunk[4], s_chunk[5] == 0};
+    const bool aligned = cp.in_aligned, w_aligned = cp.w_aligned;
     const int kh = (ks + p.v_head_offset) % p.n_k;
     const uint32_t sm = smem_u32(smem);
 
     // ---- q and k: a warp has eight rows, a lane four channels ----
+    uint2 raw[ROWS + 3];
+    load_rows(p, ch, warp * ROWS, kh * D + lane * 4, aligned, raw);
     {
         uint8_t* img = key_chunk(cp, u, ks);
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {              // 0: q, 1: k
-            float4 y[8];
-            conv_rows<8, K4>(p, ch, warp * 8, part * p.n_k * D + kh * D + lane * 4, aligned, y);
+            f32x2 y[ROWS][2];
+            conv_rows<K4>(p, ch, warp * ROWS, part * p.n_k * D + kh * D + lane * 4, aligned, w_aligned, raw, y);
+            if (K4) load_rows(p, ch, warp * ROWS, (part ? 2 * p.n_k * D + ks * D : p.n_k * D + kh * D) + lane * 4, aligned, raw);     // k, then the first value head
+            float ss[ROWS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = warp * 8 + i;
-                const float ss = warp_sum(y[i].x * y[i].x + y[i].y * y[i].y + y[i].z * y[i].z + y[i].w * y[i].w);
-                const float r = rsqrtf(ss + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
+            for (int i = 0; i < ROWS; ++i) {
+                const float2 q = both(fma2(y[i][0], y[i][0], mul2(y[i][1], y[i][1])));
+                ss[i] = q.x + q.y;
+            }
+            const float mine = rsqrtf(sums8(ss, lane) + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const int t = warp * ROWS + i;
+                const float r = __shfl_sync(0xffffffffu, mine, 4 * i);
                 uint2 hi, lo;
-                split2(y[i].x * r, y[i].y * r, hi.x, lo.x);
-                split2(y[i].z * r, y[i].w * r, hi.y, lo.y);
+                split2(mul2(y[i][0], pair(r, r)), hi.x, lo.x);
+                split2(mul2(y[i][1], pair(r, r)), hi.y, lo.y);
                 const int at = img_at(t, lane >> 1) + (lane & 1) * 8;
                 const int at_hi = (part ? OFF_KHI : OFF_QHI) + at, at_lo = (part ? OFF_KLO : OFF_QLO) + at;
                 *reinterpret_cast<uint2*>(smem + at_hi) = hi; *reinterpret_cast<uint2*>(img + at_hi) = hi;
@@ -336,7 +386,8 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                 if (lane >= o) sum += x;
             }
             const double G1 = sum, G0 = sum - l1, all = __shfl_sync(0xffffffffu, sum, 31);
-            s_G[warp][2 * lane] = G0; s_G[warp][2 * lane + 1] = G1;
+            const float f0 = (float)G0, f1 = (float)G1;
+            s_G[warp][2 * lane] = make_float2(f0, (float)(G0 - f0)); s_G[warp][2 * lane + 1] = make_float2(f1, (float)(G1 - f1));
             s_b[warp][2 * lane] = b[0]; s_b[warp][2 * lane + 1] = b[1];
             float2* vec = reinterpret_cast<float2*>(head_chunk(cp, u, h) + OFF_VEC);
             const float e0 = ex2((float)G0), e1 = ex2((float)G1), ea = ex2((float)all);
@@ -346,59 +397,67 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             vec[V_ALL / 2 + lane] = make_float2(ea, ea);
         }
         __syncthreads();
-        // ---- A and P; b v, transposed ----
+        // ---- A and P, up to the diagonal's blocks: what lies above is not read.  16 rows and 2, 4, 6, 8 units of eight columns for each block of rows ----
+#pragma unroll 1
+        for (int item = tid; item < nh * 320; item += PREP_THREADS) {
+            const int hi = item / 320, k = item % 320, tb = (k >= 32) + (k >= 96) + (k >= 192), off = k - 16 * tb * (tb + 1), half = off >> 1;
+            const int row = tb == 0 ? half : tb == 1 ? half >> 1 : tb == 2 ? (half * 43) >> 7 : half >> 2;       // off / (2 tb + 2), off < 128
+            const int t = 16 * tb + row, unit = off - 2 * (tb + 1) * row;
+            uint8_t* dst = head_chunk(cp, u, h0 + hi * p.n_k);
+            uint8_t* A = smem + PREP_A + hi * 2 * TRI;
+            const float2 Gt = s_G[hi][t];
+            const float b = s_b[hi][t];
+            float a8[8], p8[8], G4[4][4], kk[8], qk[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(G4[e]) = *reinterpret_cast<const float4*>(&s_G[hi][unit * 8 + 2 * e]);
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                *reinterpret_cast<float4*>(kk + e) = *reinterpret_cast<const float4*>(s_kk + t * C + unit * 8 + e);
+                *reinterpret_cast<float4*>(qk + e) = *reinterpret_cast<const float4*>(s_qk + t * C + unit * 8 + e);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = unit * 8 + e;
+                const float m = ex2((Gt.x - G4[e >> 1][2 * (e & 1)]) + (Gt.y - G4[e >> 1][2 * (e & 1) + 1]));
+                p8[e] = i <= t ? m * qk[e] : 0.f;
+                a8[e] = i < t ? b * m * kk[e] : 0.f;
+            }
+            if (unit >> 1 == tb) {
+                float* diag = reinterpret_cast<float*>(smem + PREP_DIAG) + hi * C * 16 + t * 16 + (unit & 1) * 8;
+                *reinterpret_cast<float4*>(diag) = make_float4(a8[0], a8[1], a8[2], a8[3]);
+                *reinterpret_cast<float4*>(diag + 4) = make_float4(a8[4], a8[5], a8[6], a8[7]);
+            }
+            uint4 ph, pl, ah, al;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a8[e] *= SK;
+            split2(a8[0], a8[1], ah.x, al.x); split2(a8[2], a8[3], ah.y, al.y); split2(a8[4], a8[5], ah.z, al.z); split2(a8[6], a8[7], ah.w, al.w);
+            split2(p8[0], p8[1], ph.x, pl.x); split2(p8[2], p8[3], ph.y, pl.y); split2(p8[4], p8[5], ph.z, pl.z); split2(p8[6], p8[7], ph.w, pl.w);
+            const int at = t * 128 + (((unit ^ t) & 7) << 4);
+            *reinterpret_cast<uint4*>(A + at) = ah;
+            *reinterpret_cast<uint4*>(A + TRI + at) = al;
+            *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
+            *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
+        }
+        // ---- b v, transposed ----
 #pragma unroll 1
         for (int hi = 0; hi < nh; ++hi) {
             const int h = h0 + hi * p.n_k;
-            uint8_t* dst = head_chunk(cp, u, h);
-            uint8_t* A = smem + PREP_A + hi * 2 * TRI;
-            float* diag = reinterpret_cast<float*>(smem + PREP_DIAG) + hi * C * 16;
+            uint8_t* dst = head_chunk(cp, u, h) + OFF_V;
+            f32x2 y[ROWS][2];
+            conv_rows<K4>(p, ch, warp * ROWS, 2 * p.n_k * D + h * D + lane * 4, aligned, w_aligned, raw, y);
+            if (K4 && h + p.n_k < p.n_v) load_rows(p, ch, warp * ROWS, 2 * p.n_k * D + (h + p.n_k) * D + lane * 4, aligned, raw);
+            float v[4][ROWS];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int item = tid + r * PREP_THREADS, t = item >> 3, unit = item & 7;
-                const double Gt = s_G[hi][t];
-                const float b = s_b[hi][t];
-                float a8[8], p8[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int i = unit * 8 + e;
-                    a8[e] = p8[e] = 0.f;
-                    if (i <= t) {
-                        const float m = ex2((float)(Gt - s_G[hi][i]));
-                        p8[e] = m * s_qk[t * C + i];
-                        if (i < t) a8[e] = b * m * s_kk[t * C + i];
-                    }
-                }
-                if (unit >> 1 == t >> 4) {
-                    *reinterpret_cast<float4*>(diag + t * 16 + (unit & 1) * 8) = make_float4(a8[0], a8[1], a8[2], a8[3]);
-                    *reinterpret_cast<float4*>(diag + t * 16 + (unit & 1) * 8 + 4) = make_float4(a8[4], a8[5], a8[6], a8[7]);
-                }
-                uint4 ph, pl, ah, al;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) a8[e] *= SK;
-                split2(a8[0], a8[1], ah.x, al.x); split2(a8[2], a8[3], ah.y, al.y); split2(a8[4], a8[5], ah.z, al.z); split2(a8[6], a8[7], ah.w, al.w);
-                split2(p8[0], p8[1], ph.x, pl.x); split2(p8[2], p8[3], ph.y, pl.y); split2(p8[4], p8[5], ph.z, pl.z); split2(p8[6], p8[7], ph.w, pl.w);
-                const int at = t * 128 + (((unit ^ t) & 7) << 4);
-                *reinterpret_cast<uint4*>(A + at) = ah;
-                *reinterpret_cast<uint4*>(A + TRI + at) = al;
-                *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
-                *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
-            }
-            float4 y[8];
-            conv_rows<8, K4>(p, ch, warp * 8, 2 * p.n_k * D + h * D + lane * 4, aligned, y);
-            float v[4][8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float b = s_b[hi][warp * 8 + i];
-                v[0][i] = b * y[i].x; v[1][i] = b * y[i].y; v[2][i] = b * y[i].z; v[3][i] = b * y[i].w;
+            for (int i = 0; i < ROWS; ++i) {
+                const float b = s_b[hi][warp * ROWS + i];
+                const float2 x0 = both(mul2(y[i][0], pair(b, b))), x1 = both(mul2(y[i][1], pair(b, b)));
+                v[0][i] = x0.x; v[1][i] = x0.y; v[2][i] = x1.x; v[3][i] = x1.y;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = lane * 4 + e;
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
-                    *reinterpret_cast<float4*>(dst + OFF_V + col * 256 + (((2 * warp + q) ^ (col & 7)) << 4)) = make_float4(v[e][4 * q], v[e][4 * q + 1], v[e][4 * q + 2], v[e][4 * q + 3]);
-            }
+                    *reinterpret_cast<float4*>(dst + val_at(lane * 4 + e, 2 * warp + q)) = make_float4(v[e][4 * q], v[e][4 * q + 1], v[e][4 * q + 2], v[e][4 * q + 3]);
         }
         __syncthreads();
         // ---- the diagonal's blocks of T, in the place of A's: a thread per column ----
@@ -487,23 +546,26 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             }
         }
         __syncthreads();
-        // ---- T as the scan reads it ----
+        // ---- T as the scan reads it: the blocks below the diagonal back from their transposes, in the place of A's ----
 #pragma unroll 1
-        for (int item = tid; item < nh * 2 * C * 8; item += PREP_THREADS) {
-            const int hi = item / (2 * C * 8), half = item / (C * 8) & 1, t = item / 8 % C, unit = item & 7;
-            const uint8_t* T = smem + PREP_A + hi * 2 * TRI + half * TRI;
-            const int to = t * 128 + (((unit ^ t) & 7) << 4);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (unit >> 1 == t >> 4) {
-                v = *reinterpret_cast<const uint4*>(T + to);
-            } else if (unit >> 1 < t >> 4) {
-                uint32_t x[8];
+        for (int item = warp; item < nh * 12; item += PREP_THREADS / 32) {
+            const int part = item % (nh * 2), pr = item / (nh * 2);        // head and half of the number; block (i, j)
+            const int i = pr == 0 ? 1 : pr < 3 ? 2 : 3, j = pr - i * (i - 1) / 2, mat = lane >> 3, r8 = lane & 7;
+            uint8_t* T = smem + PREP_A + part * TRI;
+            uint32_t x[4];
+            const uint32_t from = smem_u32(T) + (16 * j + 8 * (mat & 1) + r8) * 128 + (((2 * i + (mat >> 1)) ^ r8) << 4);
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(from));
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = *reinterpret_cast<const unsigned short*>(T + (unit * 8 + e) * 128 + (((t >> 3) ^ e) << 4) + (t & 7) * 2);
-                v = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+            for (int m = 0; m < 4; ++m) {
+                const int t = 16 * i + 8 * (m >> 1) + (lane >> 2);
+                *reinterpret_cast<uint32_t*>(T + t * 128 + (((2 * j + (m & 1)) ^ (t & 7)) << 4) + (lane & 3) * 4) = x[m];
             }
-            *reinterpret_cast<uint4*>(head_chunk(cp, u, h0 + hi * p.n_k) + OFF_THI + half * TRI + to) = v;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int item = tid; item < nh * 2 * (TRI / 16); item += PREP_THREADS) {
+            const int hi = item / (2 * TRI / 16), at = item % (2 * TRI / 16) * 16;
+            *reinterpret_cast<uint4*>(head_chunk(cp, u, h0 + hi * p.n_k) + OFF_THI + at) = *reinterpret_cast<const uint4*>(smem + PREP_A + hi * 2 * TRI + at);
         }
     }
     if (waits) pdl_wait();
@@ -621,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
         };
         bool ok = true;
         for (int c = 0; c < nc; ++c) {
-            const uint32_t vec = stage(c) + ST_VEC, vals = base + SM_V + col * 256;
+            const uint32_t vec = stage(c) + ST_VEC, vals = base + SM_V + val_at(col, 0);
             float s, inv;
             // ---- the state as an operand ----
             {
@@ -653,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 float top = 0.f;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float4 v = lds4(vals + (((8 * w + q) ^ (col & 7)) << 4)), be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
+                    const float4 v = lds4(vals + (8 * w + q) * (D * 16)), be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
                     r[2 * q] = fma2(mul2(pair(be.x, be.y), f2), pair_of(x[4 * q], x[4 * q + 1]), pair(v.x, v.y));
                     r[2 * q + 1] = fma2(mul2(pair(be.z, be.w), f2), pair_of(x[4 * q + 2], x[4 * q + 3]), pair(v.z, v.w));
                 }
@@ -910,6 +972,7 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
     auto fits = [](const void* x, size_t row, int off) { return (reinterpret_cast<uintptr_t>(x) & 7) == 0 && row % 4 == 0 && off % 4 == 0; };
     p.in_aligned = fits(g.in, g.in_row, g.z_off);
     p.out_aligned = fits(g.out, g.out_row, 0);
+    p.w_aligned = (reinterpret_cast<uintptr_t>(g.conv_w) & 15) == 0;
     const auto prep = g.K == 4 ? gdc::gdn_chunk_prep_kernel<true> : gdc::gdn_chunk_prep_kernel<false>;
     cudaError_t e = tc5::raise_smem(prep, gdc::PREP_SMEM);
     if (e == cudaSuccess) e = tc5::raise_smem(gdc::gdn_chunk_scan_kernel, gdc::SCAN_SMEM);

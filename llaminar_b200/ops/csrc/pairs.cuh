@@ -20,6 +20,11 @@ LLM_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
+LLM_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
 LLM_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     f32x2 v;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
