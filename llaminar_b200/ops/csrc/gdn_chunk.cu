@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             tc_fence_after();
             return fmaxf(mine, s_top[which][w ^ 1][col]);
         };
-        bool ok = true;
+        bool ok = true;                                     // after a wait that gave up all go on, without further waits, since they meet at barriers
         for (int c = 0; c < nc; ++c) {
             const uint32_t vec = stage(c) + ST_VEC, vals = base + SM_V + val_at(col, 0);
             float s, inv;
@@ -703,8 +703,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 mbar_arrive_if(bar(S_RDY), lane == 0);
             }
             // ---- R = b v - b e^G S^T k ----
-            ok = mbar_wait_warp(bar(IN_FULL + (c & 1)), phase(c), abort_flag) && mbar_wait_warp(bar(V_FULL), c & 1, abort_flag) && mbar_wait_warp(bar(KS_DONE), c & 1, abort_flag);
-            if (!ok) break;
+            ok = ok && mbar_wait_warp(bar(IN_FULL + (c & 1)), phase(c), abort_flag) && mbar_wait_warp(bar(V_FULL), c & 1, abort_flag) && mbar_wait_warp(bar(KS_DONE), c & 1, abort_flag);
             tc_fence_after();
             {
                 uint32_t x[32];
@@ -734,8 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 mbar_arrive_if(bar(V_EMPTY), lane == 0);
             }
             // ---- U = T R; U e^(G_C - G) for the state ----
-            ok = mbar_wait_warp(bar(U_DONE), c & 1, abort_flag);
-            if (!ok) break;
+            ok = ok && mbar_wait_warp(bar(U_DONE), c & 1, abort_flag);
             tc_fence_after();
             const float decay = lds4(vec + V_ALL * 4).x;
             {
@@ -769,8 +767,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
             }
             // ---- S = e^G_C S + sum ----
-            ok = mbar_wait_warp(bar(DS_DONE), c & 1, abort_flag);
-            if (!ok) break;
+            ok = ok && mbar_wait_warp(bar(DS_DONE), c & 1, abort_flag);
             tc_fence_after();
             const float f = inv * (1.f / SK);
 #pragma unroll
@@ -794,8 +791,9 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OUT));
         const int ow = warp - 8, col = tid & 127;
         const uint32_t t_lane = tmem + ((uint32_t)(ow * 32) << 16);
-        const float4 gain = make_float4(p.norm_w[lane * 4], p.norm_w[lane * 4 + 1], p.norm_w[lane * 4 + 2], p.norm_w[lane * 4 + 3]);
+        const f32x2 gain0 = pair(p.norm_w[lane * 4], p.norm_w[lane * 4 + 1]), gain1 = pair(p.norm_w[lane * 4 + 2], p.norm_w[lane * 4 + 3]);
         const bool in_aligned = cp.in_aligned, out_aligned = cp.out_aligned;
+        bool ok = true;
         for (int c = 0; c < nc; ++c) {
             const int row0 = first + (c0 + c) * C, n = min(C, first + n_rows - row0);
             uint2 z[C / 4];                                 // the rows' gates, on their way while the chunk is at work
@@ -804,7 +802,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 const __nv_bfloat16* x = p.in + (size_t)(row0 + min(i * 4 + ow, n - 1)) * p.in_row + p.z_off + h * D + lane * 4;
                 z[i] = four(x, in_aligned);
             }
-            if (!mbar_wait_warp(bar(O_DONE), c & 1, abort_flag)) break;
+            ok = ok && mbar_wait_warp(bar(O_DONE), c & 1, abort_flag);
             tc_fence_after();
             bar_sync(2, 128);                               // the last chunk's rows have been read
             const uint32_t vec = stage(c) + ST_VEC, rows = base + SM_O;
@@ -831,34 +829,30 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             mbar_arrive_if(bar(O_FREE), lane == 0);
             mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
 #pragma unroll
-            for (int i0 = 0; i0 < C / 4; i0 += 4) {         // four rows at a time: their sums go through the lanes together
-                float4 o[4];
-                float ss[4];
+            for (int i0 = 0; i0 < C / 4; i0 += ROWS) {      // eight rows at a time: their sums go through the lanes together
+                f32x2 o[ROWS][2];
+                float ss[ROWS];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    o[k] = lds4(rows + ((i0 + k) * 4 + ow) * (D * 4) + lane * 16);
-                    ss[k] = o[k].x * o[k].x + o[k].y * o[k].y + o[k].z * o[k].z + o[k].w * o[k].w;
+                for (int k = 0; k < ROWS; ++k) {
+                    const float4 v = lds4(rows + ((i0 + k) * 4 + ow) * (D * 4) + lane * 16);
+                    o[k][0] = pair(v.x, v.y);
+                    o[k][1] = pair(v.z, v.w);
+                    const float2 q = both(fma2(o[k][0], o[k][0], mul2(o[k][1], o[k][1])));
+                    ss[k] = q.x + q.y;
                 }
+                const float mine = rsqrtf(sums8(ss, lane) * (1.f / D) + p.eps);
 #pragma unroll
-                for (int off = 16; off; off >>= 1)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) ss[k] += __shfl_xor_sync(0xffffffffu, ss[k], off);
-                uint2 v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < ROWS; ++k) {
                     const uint2 g = z[i0 + k];
-                    const float r = rsqrtf(ss[k] * (1.f / D) + p.eps);
-                    v[k].x = pack_bf16(o[k].x * r * gain.x * silu(bf16_lo(g.x)), o[k].y * r * gain.y * silu(bf16_hi(g.x)));
-                    v[k].y = pack_bf16(o[k].z * r * gain.z * silu(bf16_lo(g.y)), o[k].w * r * gain.w * silu(bf16_hi(g.y)));
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                    const float r = __shfl_sync(0xffffffffu, mine, 4 * k);
+                    const float2 a = both(mul2(mul2(mul2(o[k][0], pair(r, r)), gain0), silu2(two_of(g.x)))), e = both(mul2(mul2(mul2(o[k][1], pair(r, r)), gain1), silu2(two_of(g.y))));
+                    const uint2 v = make_uint2(pack_bf16(a.x, a.y), pack_bf16(e.x, e.y));
                     const int t = (i0 + k) * 4 + ow;
                     __nv_bfloat16* dst = p.out + (size_t)(row0 + t) * p.out_row + h * D + lane * 4;
-                    if (t < n && out_aligned) *reinterpret_cast<uint2*>(dst) = v[k];
-                    if (t < n && !out_aligned) {
-                        dst[0] = __ushort_as_bfloat16(v[k].x & 0xffff); dst[1] = __ushort_as_bfloat16(v[k].x >> 16);
-                        dst[2] = __ushort_as_bfloat16(v[k].y & 0xffff); dst[3] = __ushort_as_bfloat16(v[k].y >> 16);
+                    if (t < n && ok && out_aligned) *reinterpret_cast<uint2*>(dst) = v;
+                    if (t < n && ok && !out_aligned) {
+                        dst[0] = __ushort_as_bfloat16(v.x & 0xffff); dst[1] = __ushort_as_bfloat16(v.x >> 16);
+                        dst[2] = __ushort_as_bfloat16(v.y & 0xffff); dst[3] = __ushort_as_bfloat16(v.y >> 16);
                     }
                 }
             }
