@@ -10,8 +10,8 @@
 // first; the next state, rows and gates are on their way meanwhile.
 // What bounds it: few rows, the state's bytes (64 KB read per head at d = 128; written too unless the state is left alone); more rows, the chain of a row.
 //
-// gdn_commit brings the state behind the accepted rows: a streaming pass, S = A S + sum_r k_r (u_r prod_{s > r} a_s)^T, bound by the
-// state's bytes in both directions.
+// gdn_commit brings the state behind the accepted rows: a streaming pass, S = a S + k u^T for each of them, bound by the state's bytes in both
+// directions.
 //
 // (reference: the recurrence of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu and the verifier's state capture rows,
 //  src/v2/models/qwen35/Qwen35Graph.cpp:886-887.)
@@ -503,52 +503,65 @@ __global__ void __launch_bounds__(256) gdn_windows_kernel(const GdnParams p) {
     pdl_wait();                                             // (the scan of the chunk form reads no windows and runs beside this)
 }
 
+// A block has half a state at d = 128, a whole one otherwise: 32 KB at most, so that an SM has four or more of them on their way.  The kept rows come in together.
+template <int D> constexpr int COMMIT_PARTS = D == 128 ? 2 : 1;
 template <int D>
-__global__ void __launch_bounds__(256) gdn_commit_kernel(const GdnParams p, const int* accepted) {
+__global__ void __launch_bounds__(256, 4) gdn_commit_kernel(const GdnParams p, const int* accepted) {
     constexpr int BLOCK = 16;                                // kept rows in shared memory at a time
     __shared__ __align__(16) float s_u[BLOCK][D], s_k[BLOCK][D];
+    __shared__ float s_a[BLOCK];
     const int b = blockIdx.y, tid = threadIdx.x, R = p.rows_per_seq;
     const int n = max(0, min(accepted[b], R));
     if (n == 0) return;
     const GdnSeq q = gdn_seq(p, b);
-    if ((int)blockIdx.x >= p.n_v) {                          // the convolution's windows
-        const int c = ((int)blockIdx.x - p.n_v) * 256 + tid;
+    constexpr int PARTS = COMMIT_PARTS<D>;
+    if ((int)blockIdx.x >= p.n_v * PARTS) {                  // the convolution's windows
+        const int c = ((int)blockIdx.x - p.n_v * PARTS) * 256 + tid;
         if (c < p.C) gdn_shift<true>(p, q, b, c, n);
         return;
     }
-    const int h = blockIdx.x;
+    const int h = blockIdx.x / PARTS;
     const size_t kept = (size_t)b * R * p.n_v + h;           // of the sequence's first kept row; the next one is n_v further
-    float4* state = reinterpret_cast<float4*>(p.rec + (q.slot * p.n_v + h) * (size_t)(D * D));
-    constexpr int QUADS = D / 4, STEP = 256 / QUADS, PER = D / STEP;         // a thread has PER rows i of four columns
-    const int j4 = tid % QUADS, i0 = tid / QUADS;
-    float4 S[PER];
+    constexpr int QUADS = D / 4, STEP = 256 / QUADS, PER = D / PARTS / STEP;       // a thread has PER rows i of four columns
+    const int j4 = tid % QUADS, i0 = blockIdx.x % PARTS * (D / PARTS) + tid / QUADS;
+    float4* state = reinterpret_cast<float4*>(p.rec + (q.slot * p.n_v + h) * (size_t)(D * D)) + i0 * QUADS + j4;
+    f32x2 S[PER][2];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) S[e] = state[(size_t)(i0 + e * STEP) * QUADS + j4];
-    float all = 1.f;
-    for (int r = 0; r < n; ++r) all *= p.keep_a[kept + (size_t)r * p.n_v];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) { S[e].x *= all; S[e].y *= all; S[e].z *= all; S[e].w *= all; }
-    float after = 1.f;                                       // decays behind row r
-    for (int r1 = n; r1 > 0; r1 -= BLOCK) {
-        const int r0 = max(0, r1 - BLOCK);
+    for (int e = 0; e < PER; ++e) {
+        const float4 x = __ldcs(state + e * STEP * QUADS);
+        S[e][0] = pair(x.x, x.y);
+        S[e][1] = pair(x.z, x.w);
+    }
+    for (int r0 = 0; r0 < n; r0 += BLOCK) {
+        const int rows = min(BLOCK, n - r0);
         __syncthreads();
-        for (int r = r1 - 1; r >= r0; --r) {
-            const size_t at = kept + (size_t)r * p.n_v;
-            if (tid < D) { s_u[r - r0][tid] = after * p.keep_u[at * D + tid]; s_k[r - r0][tid] = p.keep_k[at * D + tid]; }
-            after *= p.keep_a[at];
+#pragma unroll 4
+        for (int i = tid; i < rows * QUADS; i += 256) {
+            const int r = i / QUADS, c = i % QUADS * 4;
+            const size_t at = (kept + (size_t)(r0 + r) * p.n_v) * D + c;
+            const float4 u = *reinterpret_cast<const float4*>(p.keep_u + at), k = *reinterpret_cast<const float4*>(p.keep_k + at);
+            *reinterpret_cast<float4*>(&s_u[r][c]) = u;
+            *reinterpret_cast<float4*>(&s_k[r][c]) = k;
         }
+        if (tid < rows) s_a[tid] = p.keep_a[kept + (size_t)(r0 + tid) * p.n_v];
         __syncthreads();
-        for (int r = 0; r < r1 - r0; ++r) {
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
             const float4 u = *reinterpret_cast<const float4*>(&s_u[r][j4 * 4]);
+            const f32x2 a = pair(s_a[r], s_a[r]), u0 = pair(u.x, u.y), u1 = pair(u.z, u.w);
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
                 const float k = s_k[r][i0 + e * STEP];
-                S[e].x += k * u.x; S[e].y += k * u.y; S[e].z += k * u.z; S[e].w += k * u.w;
+                S[e][0] = fma2(pair(k, k), u0, mul2(a, S[e][0]));
+                S[e][1] = fma2(pair(k, k), u1, mul2(a, S[e][1]));
             }
         }
     }
 #pragma unroll
-    for (int e = 0; e < PER; ++e) state[(size_t)(i0 + e * STEP) * QUADS + j4] = S[e];
+    for (int e = 0; e < PER; ++e) {
+        const float2 x = both(S[e][0]), y = both(S[e][1]);
+        state[e * STEP * QUADS] = make_float4(x.x, x.y, y.x, y.y);
+    }
 }
 
 LLM_DEFINE_BOUNDS_STATUS_READER(bounds_status_gdn_rows)
@@ -605,7 +618,7 @@ cudaError_t launch_gdn_windows(const GdnParams& p, cudaStream_t st) {
 }
 cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStream_t st) {
     if (p.n_seqs == 0 || p.rows_per_seq == 0) return cudaSuccess;
-    const dim3 grid(p.n_v + (p.C + 255) / 256, p.n_seqs);
+    const dim3 grid(p.n_v * (p.d == 128 ? COMMIT_PARTS<128> : 1) + (p.C + 255) / 256, p.n_seqs);
     switch (p.d) {
         case 32: gdn_commit_kernel<32><<<grid, 256, 0, st>>>(p, accepted); break;
         case 64: gdn_commit_kernel<64><<<grid, 256, 0, st>>>(p, accepted); break;

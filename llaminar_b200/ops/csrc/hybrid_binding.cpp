@@ -96,6 +96,7 @@ void keep_args(llm::GdnParams& p, const Tensor& like, const std::vector<Tensor>&
     p.rows_per_seq = R;
     p.keep_a = const_cast<float*>(floats_on(like, keep[0], n, "decays")); p.keep_k = const_cast<float*>(floats_on(like, keep[1], n * p.d, "keys"));
     p.keep_u = const_cast<float*>(floats_on(like, keep[2], n * p.d, "corrections"));
+    TORCH_CHECK(((reinterpret_cast<uintptr_t>(p.keep_k) | reinterpret_cast<uintptr_t>(p.keep_u)) & 15) == 0, "keys and corrections must start on 16 bytes");
     same_device(like, keep[3], "inputs");
     want(keep[3], torch::kBFloat16, "inputs");
     p.keep_x = reinterpret_cast<__nv_bfloat16*>(keep[3].data_ptr());
