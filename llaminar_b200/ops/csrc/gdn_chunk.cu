@@ -589,7 +589,7 @@ static_assert(SCAN_SMEM <= 227 * 1024, "shared memory of a CTA");
 constexpr uint32_t T_SHI = 0, T_SLO = 64, T_DS = 0, T_KS = 128, T_QS = 192, T_PU = 256, T_RHI = 320, T_RLO = 352, T_UHI = 384, T_ULO = 416;
 __host__ __device__ constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }     // fp16 x fp16 -> fp32, M = 128
 
-enum Bar { IN_FULL = 0, IN_EMPTY = 2, V_FULL = 4, V_EMPTY, Q_FULL, Q_EMPTY, P_FULL, P_EMPTY, S_RDY, KS_DONE, R_RDY, U_DONE, U_RDY, DS_DONE, O_DONE, O_FREE, N_BARS };
+enum Bar { IN_FULL = 0, IN_EMPTY = 2, V_FULL = 4, V_EMPTY, Q_FULL, Q_EMPTY, P_FULL, P_EMPTY, S_RDY, KS_DONE = S_RDY + 2, R_RDY, U_DONE, U_RDY, UO_RDY, DS_DONE, O_DONE, O_FREE, N_BARS };
 
 // the power of two that brings `top` into [2^13, 2^14), and its inverse
 LLM_DEVICE void scale_for(float top, float& s, float& inv) {
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
         for (int i = 0; i < N_BARS; ++i) {
             int n = 1;
             if (i == IN_EMPTY || i == IN_EMPTY + 1) n = 1 + 8 + 4;                   // the products, the math and the output warps
-            if (i == S_RDY || i == R_RDY || i == U_RDY || i == V_EMPTY) n = 8;
+            if (i == S_RDY || i == S_RDY + 1 || i == R_RDY || i == U_RDY || i == UO_RDY || i == V_EMPTY) n = 8;
             if (i == O_FREE) n = 4;
             mbar_init(bar(i), n);
         }
@@ -683,31 +683,38 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
             tc_fence_after();
             return fmaxf(mine, s_top[which][w ^ 1][col]);
         };
+        float top_s = 0.f;                                  // of the state
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top_s = top2(top_s, S[i]);
         bool ok = true;                                     // after a wait that gave up all go on, without further waits, since they meet at barriers
         for (int c = 0; c < nc; ++c) {
             const uint32_t vec = stage(c) + ST_VEC, vals = base + SM_V + val_at(col, 0);
             float s, inv;
             // ---- the state as an operand ----
             {
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) top = top2(top, S[i]);
-                scale_for(column_top(0, top), s, inv);
-                uint32_t hi[32], lo[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) split2(mul2(S[i], pair(s, s)), hi[i], lo[i]);
-                tmem_st32(t_lane + T_SHI + w * 32, hi);
-                tmem_st32(t_lane + T_SLO + w * 32, lo);
+                scale_for(column_top(0, top_s), s, inv);
                 if (w == 0) s_inv[c & 1][0][col] = inv;
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                mbar_arrive_if(bar(S_RDY), lane == 0);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {       // S^T k begins with the first half
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) split2(mul2(S[16 * half + i], pair(s, s)), hi[i], lo[i]);
+                    tmem_st_n<16>(t_lane + T_SHI + w * 32 + half * 16, hi);
+                    tmem_st_n<16>(t_lane + T_SLO + w * 32 + half * 16, lo);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    mbar_arrive_if(bar(S_RDY + half), lane == 0);
+                }
             }
             // ---- R = b v - b e^G S^T k ----
-            ok = ok && mbar_wait_warp(bar(IN_FULL + (c & 1)), phase(c), abort_flag) && mbar_wait_warp(bar(V_FULL), c & 1, abort_flag) && mbar_wait_warp(bar(KS_DONE), c & 1, abort_flag);
-            tc_fence_after();
+            ok = ok && mbar_wait_warp(bar(IN_FULL + (c & 1)), phase(c), abort_flag) && mbar_wait_warp(bar(V_FULL), c & 1, abort_flag);
             {
+                float4 v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = lds4(vals + (8 * w + q) * (D * 16));
+                ok = ok && mbar_wait_warp(bar(KS_DONE), c & 1, abort_flag);
+                tc_fence_after();
                 uint32_t x[32];
                 tmem_ld_n<32>(t_lane + T_KS + w * 32, x);
                 const float f = -inv * (1.f / SK);
@@ -716,9 +723,9 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 float top = 0.f;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float4 v = lds4(vals + (8 * w + q) * (D * 16)), be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
-                    r[2 * q] = fma2(mul2(pair(be.x, be.y), f2), pair_of(x[4 * q], x[4 * q + 1]), pair(v.x, v.y));
-                    r[2 * q + 1] = fma2(mul2(pair(be.z, be.w), f2), pair_of(x[4 * q + 2], x[4 * q + 3]), pair(v.z, v.w));
+                    const float4 be = lds4(vec + (V_BE + 32 * w + 4 * q) * 4);
+                    r[2 * q] = fma2(mul2(pair(be.x, be.y), f2), pair_of(x[4 * q], x[4 * q + 1]), pair(v[q].x, v[q].y));
+                    r[2 * q + 1] = fma2(mul2(pair(be.z, be.w), f2), pair_of(x[4 * q + 2], x[4 * q + 3]), pair(v[q].z, v[q].w));
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = top2(top, r[i]);
@@ -735,49 +742,61 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 mbar_arrive_if(bar(V_EMPTY), lane == 0);
             }
             // ---- U = T R; U e^(G_C - G) for the state ----
+            float4 el[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) el[q] = lds4(vec + (V_EL + 32 * w + 4 * q) * 4);
+            const float decay = lds4(vec + V_ALL * 4).x;
             ok = ok && mbar_wait_warp(bar(U_DONE), c & 1, abort_flag);
             tc_fence_after();
-            const float decay = lds4(vec + V_ALL * 4).x;
             {
-                uint32_t x[32];
+                uint32_t x[32], hi[16], lo[16];
                 tmem_ld_n<32>(t_lane + T_KS + w * 32, x);
                 const float f = inv * (1.f / SK);
                 float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(__uint_as_float(x[i])));
+                for (int i = 0; i < 32; i += 2) top = top2(top, pair_of(x[i], x[i + 1]));
                 scale_for(column_top(2, top), s, inv);       // of the accumulator as it is: its own factor f goes into the inverse
-                uint32_t uh[16], ul[16], hi[16], lo[16];
+                inv *= f;
+                f32x2 a[16];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float4 el = lds4(vec + (V_EL + 32 * w + 4 * q) * 4);
-                    const f32x2 a = mul2(pair_of(x[4 * q], x[4 * q + 1]), pair(s, s)), e = mul2(pair_of(x[4 * q + 2], x[4 * q + 3]), pair(s, s));
-                    split2(a, uh[2 * q], ul[2 * q]);
-                    split2(e, uh[2 * q + 1], ul[2 * q + 1]);
-                    split2(mul2(a, pair(el.x, el.y)), hi[2 * q], lo[2 * q]);
-                    split2(mul2(e, pair(el.z, el.w)), hi[2 * q + 1], lo[2 * q + 1]);
+                    a[2 * q] = mul2(pair_of(x[4 * q], x[4 * q + 1]), pair(s, s));
+                    a[2 * q + 1] = mul2(pair_of(x[4 * q + 2], x[4 * q + 3]), pair(s, s));
+                    split2(mul2(a[2 * q], pair(el[q].x, el[q].y)), hi[2 * q], lo[2 * q]);
+                    split2(mul2(a[2 * q + 1], pair(el[q].z, el[q].w)), hi[2 * q + 1], lo[2 * q + 1]);
                 }
-                inv *= f;
                 tmem_st_n<16>(t_lane + T_RHI + w * 16, hi);
                 tmem_st_n<16>(t_lane + T_RLO + w * 16, lo);
-                tmem_st_n<16>(t_lane + T_UHI + w * 16, uh);
-                tmem_st_n<16>(t_lane + T_ULO + w * 16, ul);
-                if (w == 0) s_inv[c & 1][1][col] = inv;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 mbar_arrive_if(bar(U_RDY), lane == 0);
+                // the state's sum is on its way: U for the output
+#pragma unroll
+                for (int i = 0; i < 16; ++i) split2(a[i], hi[i], lo[i]);
+                tmem_st_n<16>(t_lane + T_UHI + w * 16, hi);
+                tmem_st_n<16>(t_lane + T_ULO + w * 16, lo);
+                if (w == 0) s_inv[c & 1][1][col] = inv;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                mbar_arrive_if(bar(UO_RDY), lane == 0);
                 mbar_arrive_if(bar(IN_EMPTY + (c & 1)), lane == 0);
             }
             // ---- S = e^G_C S + sum ----
             ok = ok && mbar_wait_warp(bar(DS_DONE), c & 1, abort_flag);
             tc_fence_after();
             const float f = inv * (1.f / SK);
+            top_s = 0.f;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t x[32];
                 tmem_ld_n<32>(t_lane + T_DS + w * 64 + half * 32, x);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[half * 16 + i] = fma2(pair(f, f), pair_of(x[2 * i], x[2 * i + 1]), mul2(pair(decay, decay), S[half * 16 + i]));
+                for (int i = 0; i < 16; ++i) {
+                    S[half * 16 + i] = fma2(pair(f, f), pair_of(x[2 * i], x[2 * i + 1]), mul2(pair(decay, decay), S[half * 16 + i]));
+                    top_s = top2(top_s, S[half * 16 + i]);
+                }
             }
         }
         if (ok) {
@@ -893,11 +912,13 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 if (!mbar_wait(bar(IN_FULL + (c & 1)), phase(c), abort_flag) || !mbar_wait(bar(S_RDY), c & 1, abort_flag)) break;
                 tc_fence_after();
                 // (a descriptor counts 16 bytes: what lies in one image is reached by addition)
-                auto with_rows = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {      // [128 columns x d] [64 rows x d]^T
-                    const uint64_t desc = smem_desc_sw128(img);
+                auto with_rows = [&](uint32_t d, uint32_t a, uint32_t img, int half, bool first_one) {        // [128 columns x d] [64 rows x d]^T, d from 32 half and 64 + 32 half on
+                    const uint64_t desc = smem_desc_sw128(img) + 4 * half;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        mma_f16_ts(tm + d, tm + a + k * 8, desc + (k >> 2) * (IMG / 2 / 16) + 2 * (k & 3), idesc(C), !first_one || k > 0 ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) {
+                        const int at = (k >> 1) * 4 + (k & 1);
+                        mma_f16_ts(tm + d, tm + a + (at + 2 * half) * 8, desc + (k >> 1) * (IMG / 2 / 16) + 2 * (k & 1), idesc(C), !first_one || k > 0 ? 1u : 0u);
+                    }
                 };
                 auto with_tri = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {       // [128 columns x 64 rows] times a lower triangle's transpose
                     const uint64_t desc = smem_desc_sw128(img);
@@ -911,15 +932,23 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                     for (int k = 0; k < 4; ++k)
                         mma_f16_ts(tm + T_DS, tm + a + k * 8, desc + k * (16 * 128 / 16), idesc(D) | MN, !first_one || k > 0 ? 1u : 0u);
                 };
-                with_rows(T_KS, T_SHI, key, true);
-                with_rows(T_KS, T_SLO, key, false);
-                with_rows(T_KS, T_SHI, key + IMG, false);
+                with_rows(T_KS, T_SHI, key, 0, true);
+                with_rows(T_KS, T_SLO, key, 0, false);
+                with_rows(T_KS, T_SHI, key + IMG, 0, false);
+                if (!mbar_wait(bar(S_RDY + 1), c & 1, abort_flag)) break;
+                tc_fence_after();
+                with_rows(T_KS, T_SHI, key, 1, false);
+                with_rows(T_KS, T_SLO, key, 1, false);
+                with_rows(T_KS, T_SHI, key + IMG, 1, false);
                 mma_commit(bar(KS_DONE));
                 if (!mbar_wait(bar(Q_FULL), c & 1, abort_flag) || (c > 0 && !mbar_wait(bar(O_FREE), (c - 1) & 1, abort_flag))) break;
                 tc_fence_after();
-                with_rows(T_QS, T_SHI, q, true);
-                with_rows(T_QS, T_SLO, q, false);
-                with_rows(T_QS, T_SHI, q + IMG, false);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    with_rows(T_QS, T_SHI, q, half, half == 0);
+                    with_rows(T_QS, T_SLO, q, half, false);
+                    with_rows(T_QS, T_SHI, q + IMG, half, false);
+                }
                 mma_commit(bar(Q_EMPTY));
                 if (!mbar_wait(bar(R_RDY), c & 1, abort_flag)) break;
                 tc_fence_after();
@@ -927,12 +956,14 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                 with_tri(T_KS, T_RLO, tri, false);
                 with_tri(T_KS, T_RHI, tri + TRI, false);
                 mma_commit(bar(U_DONE));
-                if (!mbar_wait(bar(P_FULL), c & 1, abort_flag) || !mbar_wait(bar(U_RDY), c & 1, abort_flag)) break;
+                if (!mbar_wait(bar(U_RDY), c & 1, abort_flag)) break;
                 tc_fence_after();
                 with_keys(T_RHI, key, true);
                 with_keys(T_RLO, key, false);
                 with_keys(T_RHI, key + IMG, false);
                 mma_commit(bar(DS_DONE));
+                if (!mbar_wait(bar(P_FULL), c & 1, abort_flag) || !mbar_wait(bar(UO_RDY), c & 1, abort_flag)) break;
+                tc_fence_after();
                 with_tri(T_PU, T_UHI, pt, true);
                 with_tri(T_PU, T_ULO, pt, false);
                 with_tri(T_PU, T_UHI, pt + TRI, false);
