@@ -31,7 +31,9 @@ def ext():
 GDN_HEAD_SIZES = (32, 64, 128)
 SHARED_HEAD_SIZES = (64, 128, 256)     # of rope_part_kv and attn_decode_shared
 GDN_CHUNK = 64                 # rows of a chunk
-GDN_CHUNK_MIN_ROWS = 8         # rows per sequence, on average, from which the chunk form is taken
+# Rows per sequence, on average, from which the chunk form is taken.  16 / 32 heads, row by row against chunks: 1 sequence of 16 rows 23 / 32 us, of 37 rows 46 / 31;
+# 8 of 16 rows 46 / 54; 32 of 16 rows 157 / 171, of 24 rows 220 / 172.
+GDN_CHUNK_MIN_ROWS = 20
 GDN_WORKSPACE = 256 << 20      # bytes that a pass of the chunk form may hold; longer prompts take several passes
 
 
