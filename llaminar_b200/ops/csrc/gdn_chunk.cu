@@ -20,8 +20,11 @@
 // R and U are scaled per value column, to 2^13 .. 2^14 at the largest.  (With q, P and the S and U that only the output sees as single fp16 numbers an output whose
 // sum cancels was 2^-7 off behind the gated norm.)  G is summed in 64 bits: differences of sums near -100 would cost a 32-bit one 2^-17.
 //
-// What bounds it: the scan's chain of three products and three passes through registers per chunk.  Every mbarrier wait is bounded; on a timeout the kernel
-// raises the status word and tears down.
+// What bounds it: the scan's chain along the state, 7450 clocks a chunk: the state as an operand 1290, S^T k 1070, R 1280, U 500, U as an operand 960, the
+// state's sum 990, the state 530, and 200 for each of four signals.  Operands are in tensor memory since a product of 64 (128) columns takes 41 (71) clocks so and
+// 71 (100) with both in shared memory.  8192 rows of 16 / 48 heads take 609 us (57 by the bytes), five sequences of 900 rows on average 194 (preparation
+// 92, scan 108), 37 rows 31.
+// Every mbarrier wait is bounded; on a timeout the kernel raises the status word and tears down.
 //
 // (reference: the chunk kernels of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu.)
 #include <cuda_fp16.h>
@@ -1005,7 +1008,7 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
     if (e == cudaSuccess) e = tc5::raise_smem(gdc::gdn_chunk_scan_kernel, gdc::SCAN_SMEM);
     if (e != cudaSuccess) return e;
     // One sequence's scan takes n_v SMs and leaves the others idle, so the next chunks are prepared beside it, in the other half of the workspace; the first
-    // pass is what one wave of blocks prepares.  (8192 rows of 48 heads: 945 us one after the other, 719 us so.)  The scans of several sequences run side by side instead, as long as the
+    // pass is what one wave of blocks prepares.  (8192 rows of 48 heads, when it was taken: 945 us one after the other, 719 so.)  The scans of several sequences run side by side instead, as long as the
     // workspace holds all chunks.
     const int wave = 2 * sm_count() / p.n_ks > 0 ? 2 * sm_count() / p.n_ks : 1;
     const bool beside = total > wave && most > 1 && (g.n_seqs == 1 || (size_t)total > most);

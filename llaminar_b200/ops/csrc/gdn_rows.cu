@@ -8,10 +8,11 @@
 // A CTA takes one value head of one sequence after the other; four neighbouring threads keep a column of the d x d state in registers, so that both products
 // with the state are sums inside a thread (and two exchanges) and a row costs no barrier.  q, k and v of a block of four rows are convolved, normed and left in shared memory
 // first; the next state, rows and gates are on their way meanwhile.
-// What bounds it: few rows, the state's bytes (64 KB read per head at d = 128; written too unless the state is left alone); more rows, the chain of a row.
+// What bounds it: few rows, the state's bytes (64 KB read per head at d = 128; written too unless the state is left alone); more rows, the chain of a row.  Prompts
+// of 32 / 16 heads: one sequence of 16 rows 23 us, 32 of them 157 us.
 //
 // gdn_commit brings the state behind the accepted rows: a streaming pass, S = a S + k u^T for each of them, bound by the state's bytes in both
-// directions.
+// directions (32 sequences x 48 heads: 200 MB in 35 us, 5.7 TB/s).
 //
 // (reference: the recurrence of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu and the verifier's state capture rows,
 //  src/v2/models/qwen35/Qwen35Graph.cpp:886-887.)
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
 
 // Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, a quarter each, 32 bytes further than the one before: a
 // column's four threads meet other banks.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
-// them.)  o comes from the state in front of the row, S^T q = a S0^T q + u (k.q), so that a row has one round of sums.
+// them; now 60 us, 15 of them the states' bytes, 1700 clocks a row.)  o comes from the state in front of the row, S^T q = a S0^T q + u (k.q), so that a row has one round of sums.
 template <int D, int TB, bool K4>
 __global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) {
     using namespace tc5;

@@ -6,7 +6,8 @@
 //
 // Angles are formed in 64 bits as turns, position x frequency / 2 pi, of which the whole turns are dropped before the sine: in 32 bits an angle at position 200000 is
 // 2^-7 off.  A warp has a token (or a part of its heads: few tokens) and forms them once; a lane has D / 32 neighbouring values of a head, partners of the
-// first kind come from the lane rot / 2 values away.  What bounds it: the bytes of the rows, read and written once.
+// first kind come from the lane rot / 2 values away.  What bounds it: the bytes of the rows, read and written once (8190 rows of 24
+// gated heads of 256 values: 207 MB in 44 us, 4.7 TB/s); below a few hundred rows the launch and a warp's chain (32 rows 4.4 us, 700 rows into 8-bit pages 7.0 us).
 // (reference: src/v2/kernels/cuda/ops/CUDARoPEKernels.cu, ring append of src/v2/kernels/cuda/kvcache/CUDARingKVCache.cu.)
 #include <cuda_fp16.h>
 
