@@ -93,6 +93,8 @@ LLM_DEVICE uint2 four(const __nv_bfloat16* x, bool aligned) {
     if (aligned) return *reinterpret_cast<const uint2*>(x);
     return make_uint2(__bfloat16_as_ushort(x[0]) | (uint32_t)__bfloat16_as_ushort(x[1]) << 16, __bfloat16_as_ushort(x[2]) | (uint32_t)__bfloat16_as_ushort(x[3]) << 16);
 }
+// sigmoid of a row's second gate
+LLM_DEVICE float beta(const GdnParams& p, const Chunk& ch, int t, int h) { return 1.f / (1.f + expf(-__bfloat162float(p.in[(size_t)(ch.row0 + t) * p.in_row + p.ab_off + p.n_v + h]))); }
 LLM_DEVICE f32x2 two_of(uint32_t w) { return pair(bf16_lo(w), bf16_hi(w)); }
 LLM_DEVICE f32x2 silu2(f32x2 x) {                           // x / (1 + e^-x)
     const float2 e = both(mul2(x, pair(-1.44269504f, -1.44269504f)));
@@ -109,19 +111,20 @@ constexpr int ROWS = 8;
 LLM_DEVICE const __nv_bfloat16* row_of(const GdnParams& p, const Chunk& ch, int t, int c) {
     return p.in + (size_t)min(max(ch.row0 + t, ch.first), ch.row0 + ch.n - 1) * p.in_row + c;
 }
-LLM_DEVICE void load_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, uint2 (&raw)[ROWS + 3]) {
-    if (aligned) {
+struct Rows {
+    uint2 raw[ROWS + 3];
+    float4 taps[4];                                         // of a channel
+};
+LLM_DEVICE void load_rows(const GdnParams& p, const Chunk& ch, int t0, int c, Rows& x) {
 #pragma unroll
-        for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row_of(p, ch, t0 + i - 3, c), true);
-    } else {
+    for (int e = 0; e < 4; ++e) x.taps[e] = *reinterpret_cast<const float4*>(p.conv_w + (size_t)(c + e) * 4);
 #pragma unroll
-        for (int i = 0; i < ROWS + 3; ++i) raw[i] = four(row_of(p, ch, t0 + i - 3, c), false);
-    }
+    for (int i = 0; i < ROWS + 3; ++i) x.raw[i] = four(row_of(p, ch, t0 + i - 3, c), true);
 }
-// Convolution and SiLU of those rows; zeros behind the chunk's.  K4: four taps; otherwise the rows are loaded again, tap by tap.
-template <bool K4>
-LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bool aligned, bool w_aligned, const uint2 (&raw)[ROWS + 3], f32x2 (&y)[ROWS][2]) {
-    const int K = K4 ? 4 : p.K;
+// Convolution and SiLU of those rows; zeros behind the chunk's.  FAST: four taps, all on their boundaries; otherwise the rows are loaded here, tap by tap.
+template <bool FAST>
+LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, const Rows& in, f32x2 (&y)[ROWS][2]) {
+    const int K = FAST ? 4 : p.K;
     auto before = [&](f32x2 (&x)[2], int t) {               // r < 0: of the window
         const int r = ch.row0 + t - ch.first;
         if (r >= 0) return;
@@ -132,17 +135,13 @@ LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bo
         x[1] = pair(w[2 * (K - 1)], w[3 * (K - 1)]);
     };
     const bool edge = ch.row0 + t0 - (K - 1) < ch.first;
-    if (K4) {
-        float4 taps[4];                                     // of a channel
-        const float* at = p.conv_w + (size_t)c * 4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) taps[e] = w_aligned ? *reinterpret_cast<const float4*>(at + 4 * e) : make_float4(at[4 * e], at[4 * e + 1], at[4 * e + 2], at[4 * e + 3]);
+    if (FAST) {
         f32x2 x[ROWS + 3][2];
 #pragma unroll
         for (int i = 0; i < ROWS + 3; ++i) {
             const bool there = t0 + i - 3 < ch.n;
-            x[i][0] = two_of(there ? raw[i].x : 0u);
-            x[i][1] = two_of(there ? raw[i].y : 0u);
+            x[i][0] = two_of(there ? in.raw[i].x : 0u);
+            x[i][1] = two_of(there ? in.raw[i].y : 0u);
         }
         if (edge) {
 #pragma unroll
@@ -150,7 +149,7 @@ LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bo
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float4 a = taps[2 * e], b = taps[2 * e + 1];
+            const float4 a = in.taps[2 * e], b = in.taps[2 * e + 1];
             const f32x2 w0 = pair(a.x, b.x), w1 = pair(a.y, b.y), w2 = pair(a.z, b.z), w3 = pair(a.w, b.w);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) y[i][e] = fma2(w3, x[i + 3][e], fma2(w2, x[i + 2][e], fma2(w1, x[i + 1][e], mul2(w0, x[i][e]))));
@@ -164,7 +163,7 @@ LLM_DEVICE void conv_rows(const GdnParams& p, const Chunk& ch, int t0, int c, bo
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
                 const int t = t0 + i + w - (K - 1);
-                const uint2 v = four(row_of(p, ch, t, c), aligned);
+                const uint2 v = four(row_of(p, ch, t, c), false);
                 f32x2 x[2] = {two_of(t < ch.n ? v.x : 0u), two_of(t < ch.n ? v.y : 0u)};
                 if (edge) before(x, t);
                 y[i][0] = fma2(f0, x[0], y[i][0]);
@@ -241,12 +240,12 @@ struct ChunkParams {
     uint8_t* ws;                                            // [units][n_ks] chunks of key heads, then [units][n_v] of value heads
     int n_ks, u0, units;                                    // key heads in use, first chunk of this pass, chunks of it
     int* status;
-    int in_aligned, out_aligned, w_aligned;
+    int in_aligned, out_aligned;
 };
 LLM_DEVICE uint8_t* key_chunk(const ChunkParams& p, int u, int ks) { return p.ws + ((size_t)u * p.n_ks + ks) * KEY_BYTES; }
 LLM_DEVICE uint8_t* head_chunk(const ChunkParams& p, int u, int h) { return p.ws + (size_t)p.units * p.n_ks * KEY_BYTES + ((size_t)u * p.g.n_v + h) * HEAD_BYTES; }
 
-template <bool K4>
+template <bool FAST>
 __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const ChunkParams cp) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(16) float2 s_G[PREP_HEADS][C];          // a sum as a float and what that leaves of it
@@ -280,53 +279,78 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
         return;
     }
     const Chunk ch = {s_chunk[1], s_chunk[2], s_chunk[3], s_chunk[4], s_chunk[5] == 0};
-    const bool aligned = cp.in_aligned, w_aligned = cp.w_aligned;
     const int kh = (ks + p.v_head_offset) % p.n_k;
     const uint32_t sm = smem_u32(smem);
 
-    // ---- q and k: a warp has eight rows, a lane four channels ----
-    uint2 raw[ROWS + 3];
-    load_rows(p, ch, warp * ROWS, kh * D + lane * 4, aligned, raw);
+    // ---- q, k, then b v of the value heads, transposed: a warp has eight rows, a lane four channels.  One loop, so that its code is fetched once ----
     {
-        uint8_t* img = key_chunk(cp, u, ks);
+        const int parts = 2 + (p.n_v - ks + p.n_k - 1) / p.n_k;
+        auto channel = [&](int part) { return (part < 2 ? part * p.n_k + kh : 2 * p.n_k + ks + (part - 2) * p.n_k) * D + lane * 4; };
+        Rows in;
+        if (FAST) load_rows(p, ch, warp * ROWS, channel(0), in);
 #pragma unroll 1
-        for (int part = 0; part < 2; ++part) {              // 0: q, 1: k
+        for (int part = 0; part < parts; ++part) {
             f32x2 y[ROWS][2];
-            conv_rows<K4>(p, ch, warp * ROWS, part * p.n_k * D + kh * D + lane * 4, aligned, w_aligned, raw, y);
-            if (K4) load_rows(p, ch, warp * ROWS, (part ? 2 * p.n_k * D + ks * D : p.n_k * D + kh * D) + lane * 4, aligned, raw);     // k, then the first value head
-            float ss[ROWS];
+            conv_rows<FAST>(p, ch, warp * ROWS, channel(part), in, y);
+            if (FAST && part + 1 < parts) load_rows(p, ch, warp * ROWS, channel(part + 1), in);
+            float mine;                                     // a row's factor, in lanes 4 row .. 4 row + 3
+            if (part < 2) {
+                float ss[ROWS];
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                const float2 q = both(fma2(y[i][0], y[i][0], mul2(y[i][1], y[i][1])));
-                ss[i] = q.x + q.y;
+                for (int i = 0; i < ROWS; ++i) {
+                    const float2 q = both(fma2(y[i][0], y[i][0], mul2(y[i][1], y[i][1])));
+                    ss[i] = q.x + q.y;
+                }
+                mine = rsqrtf(sums8(ss, lane) + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);        // 128^-1/2
+            } else {
+                const int t = warp * ROWS + (lane >> 2);
+                mine = t < ch.n ? beta(p, ch, t, ks + (part - 2) * p.n_k) : 0.f;
             }
-            const float mine = rsqrtf(sums8(ss, lane) + 1e-6f) * (part ? SK : SQ * 0.08838834764831845f);       // 128^-1/2
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                const int t = warp * ROWS + i;
                 const float r = __shfl_sync(0xffffffffu, mine, 4 * i);
-                uint2 hi, lo;
-                split2(mul2(y[i][0], pair(r, r)), hi.x, lo.x);
-                split2(mul2(y[i][1], pair(r, r)), hi.y, lo.y);
-                const int at = img_at(t, lane >> 1) + (lane & 1) * 8;
-                const int at_hi = (part ? OFF_KHI : OFF_QHI) + at, at_lo = (part ? OFF_KLO : OFF_QLO) + at;
-                *reinterpret_cast<uint2*>(smem + at_hi) = hi; *reinterpret_cast<uint2*>(img + at_hi) = hi;
-                *reinterpret_cast<uint2*>(smem + at_lo) = lo; *reinterpret_cast<uint2*>(img + at_lo) = lo;
+                y[i][0] = mul2(y[i][0], pair(r, r));
+                y[i][1] = mul2(y[i][1], pair(r, r));
+            }
+            if (part < 2) {
+                uint8_t* img = key_chunk(cp, u, ks);
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    uint2 hi, lo;
+                    split2(y[i][0], hi.x, lo.x);
+                    split2(y[i][1], hi.y, lo.y);
+                    const int at_hi = (part ? OFF_KHI : OFF_QHI) + img_at(warp * ROWS + i, lane >> 1) + (lane & 1) * 8, at_lo = at_hi + IMG;
+                    *reinterpret_cast<uint2*>(smem + at_hi) = hi; *reinterpret_cast<uint2*>(img + at_hi) = hi;
+                    *reinterpret_cast<uint2*>(smem + at_lo) = lo; *reinterpret_cast<uint2*>(img + at_lo) = lo;
+                }
+            } else {
+                uint8_t* dst = head_chunk(cp, u, ks + (part - 2) * p.n_k) + OFF_V;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float2 x[4][2];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { x[i][0] = both(y[4 * q + i][0]); x[i][1] = both(y[4 * q + i][1]); }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        *reinterpret_cast<float4*>(dst + val_at(lane * 4 + 2 * e, 2 * warp + q)) = make_float4(x[0][e].x, x[1][e].x, x[2][e].x, x[3][e].x);
+                        *reinterpret_cast<float4*>(dst + val_at(lane * 4 + 2 * e + 1, 2 * warp + q)) = make_float4(x[0][e].y, x[1][e].y, x[2][e].y, x[3][e].y);
+                    }
+                }
             }
         }
     }
     __syncthreads();
 
-    // ---- k.k (warps 0 - 3) and q.k (warps 4 - 7), 16 rows a warp, up to the diagonal ----
+    // ---- k.k (warps 0 - 3) and q.k (warps 4 - 7, from the other end: as much for each quarter of the SM), 16 rows a warp, up to the diagonal ----
     {
-        const int w = warp & 3, mat = lane >> 3, r8 = lane & 7;
         const bool kk = warp < 4;
+        const int w = kk ? warp : 7 - warp, mat = lane >> 3, r8 = lane & 7;
         float acc[8][4];
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int s = 0; s < 8; ++s) {
             uint32_t ah[4], al[4];
             const int a_at = img_at(16 * w + (lane & 15), 2 * s + (lane >> 4));
@@ -377,7 +401,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                     const __nv_bfloat16* ab = p.in + (size_t)(ch.row0 + t) * p.in_row + p.ab_off;
                     const float x = __bfloat162float(ab[h]) + dt;
                     g[e] = a * (x > 20.f ? x : log1pf(expf(x)));
-                    b[e] = 1.f / (1.f + expf(-__bfloat162float(ab[p.n_v + h])));
+                    b[e] = beta(p, ch, t, h);
                 }
             }
             // sums in units of ln 2, as exp2 takes them
@@ -440,27 +464,6 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             *reinterpret_cast<uint4*>(A + TRI + at) = al;
             *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
             *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
-        }
-        // ---- b v, transposed ----
-#pragma unroll 1
-        for (int hi = 0; hi < nh; ++hi) {
-            const int h = h0 + hi * p.n_k;
-            uint8_t* dst = head_chunk(cp, u, h) + OFF_V;
-            f32x2 y[ROWS][2];
-            conv_rows<K4>(p, ch, warp * ROWS, 2 * p.n_k * D + h * D + lane * 4, aligned, w_aligned, raw, y);
-            if (K4 && h + p.n_k < p.n_v) load_rows(p, ch, warp * ROWS, 2 * p.n_k * D + (h + p.n_k) * D + lane * 4, aligned, raw);
-            float v[4][ROWS];
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                const float b = s_b[hi][warp * ROWS + i];
-                const float2 x0 = both(mul2(y[i][0], pair(b, b))), x1 = both(mul2(y[i][1], pair(b, b)));
-                v[0][i] = x0.x; v[1][i] = x0.y; v[2][i] = x1.x; v[3][i] = x1.y;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    *reinterpret_cast<float4*>(dst + val_at(lane * 4 + e, 2 * warp + q)) = make_float4(v[e][4 * q], v[e][4 * q + 1], v[e][4 * q + 2], v[e][4 * q + 3]);
         }
         __syncthreads();
         // ---- the diagonal's blocks of T, in the place of A's: a thread per column ----
@@ -1002,8 +1005,7 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
     auto fits = [](const void* x, size_t row, int off) { return (reinterpret_cast<uintptr_t>(x) & 7) == 0 && row % 4 == 0 && off % 4 == 0; };
     p.in_aligned = fits(g.in, g.in_row, g.z_off);
     p.out_aligned = fits(g.out, g.out_row, 0);
-    p.w_aligned = (reinterpret_cast<uintptr_t>(g.conv_w) & 15) == 0;
-    const auto prep = g.K == 4 ? gdc::gdn_chunk_prep_kernel<true> : gdc::gdn_chunk_prep_kernel<false>;
+    const auto prep = g.K == 4 && p.in_aligned && (reinterpret_cast<uintptr_t>(g.conv_w) & 15) == 0 ? gdc::gdn_chunk_prep_kernel<true> : gdc::gdn_chunk_prep_kernel<false>;
     cudaError_t e = tc5::raise_smem(prep, gdc::PREP_SMEM);
     if (e == cudaSuccess) e = tc5::raise_smem(gdc::gdn_chunk_scan_kernel, gdc::SCAN_SMEM);
     if (e != cudaSuccess) return e;
