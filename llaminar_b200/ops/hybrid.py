@@ -31,15 +31,16 @@ def ext():
 GDN_HEAD_SIZES = (32, 64, 128)
 SHARED_HEAD_SIZES = (64, 128, 256)     # of rope_part_kv and attn_decode_shared
 GDN_CHUNK = 64                 # rows of a chunk
-# Rows per sequence, on average, from which the chunk form is taken.  16 / 32 heads, row by row against chunks: 1 sequence of 16 rows 23 / 32 us, of 37 rows 46 / 31;
-# 8 of 16 rows 46 / 54; 32 of 16 rows 157 / 171, of 24 rows 220 / 172.
-GDN_CHUNK_MIN_ROWS = 20
+# Rows from which the chunk form is taken, for the call and per sequence.  16 / 32 heads, row by row against chunks: 1 sequence of 16 rows 23 / 32 us, of 37 rows
+# 46 / 31; 8 of 8 rows 33 / 53; 32 of 8 rows 99 / 171, of 24 rows 220 / 172.  Lengths lie on the device: if all but one sequence have a row each, the long one costs
+# 1 us a row, which the bound per sequence keeps below twice the time in chunks.
+GDN_CHUNK_MIN_ROWS = (16, 9)
 GDN_WORKSPACE = 256 << 20      # bytes that a pass of the chunk form may hold; longer prompts take several passes
 
 
 def _gdn_workspace(inp: torch.Tensor, n_seqs: int, n_k: int, n_v: int, d: int):
     """Workspace of the chunk form, or None where the rows go one after the other."""
-    if d != 128 or n_seqs == 0 or inp.shape[0] < GDN_CHUNK_MIN_ROWS * n_seqs:
+    if d != 128 or n_seqs == 0 or inp.shape[0] < GDN_CHUNK_MIN_ROWS[0] + GDN_CHUNK_MIN_ROWS[1] * n_seqs:
         return None
     one = ext().gdn_chunk_bytes(1, n_k, n_v)
     units = max(1, min(inp.shape[0] // GDN_CHUNK + n_seqs, GDN_WORKSPACE // one))
