@@ -14,8 +14,9 @@
 // Nothing that a row does not see reaches it: K and V rows of the tiles' ends are masked and zeroed, and the last drafted keys, which some rows of a
 // sequence see and others do not, are taken one by one (a probability of 0 times an infinity would not be 0).
 // What bounds it: the prefix, once read, by the tensor pipe and the exponentials from about 200 rows per K/V head on, else by its bytes; the tails by theirs.  61
-// sequences x 2 rows behind 20000 keys of 128 values: prefix 50 us (0.8 PFLOP/s), with the tails 66; 32 behind 8192 keys of 256 values 33 (prefix 23, tails 15,
-// side by side); 128 behind 2048 keys of 64 values 20.
+// sequences x 2 rows behind 20000 keys of 128 values: prefix 47 us (0.86 PFLOP/s), with the tails 66; a tile of 64 keys takes 1600 clocks of two slots, all of
+// which the products take (a product of 64 columns with both operands in shared memory 71 clocks, of 128 with one in tensor memory 71).  32 behind 8192
+// keys of 256 values 27, the tails beside the prefix; 128 behind 2048 keys of 64 values 20.
 #include "attn_tile.cuh"
 #include "hybrid.h"
 #include "launch.h"
@@ -104,12 +105,11 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
             const uint32_t sQ = base + slot * DA * ATOM;
             s_query[slot * BQ + row] = m0 + row < rows_all ? (m0 + row) / G * p.n_heads + kvh * G + (m0 + row) % G : -1;
             asm volatile("bar.sync %0, 128;" ::"r"(1 + slot) : "memory");
-#pragma unroll 4
+#pragma unroll 8
             for (int idx = row; idx < BQ * (D / 8); idx += 128) {
                 const int r = idx / (D / 8), u = idx % (D / 8), from = s_query[slot * BQ + r];
-                const uint32_t dst = atom_addr(sQ + (u >> 3) * ATOM, r, u & 7);
-                if (from >= 0) cp_async16(dst, p.q + (size_t)from * D + u * 8);
-                else st_shared_v4(dst, make_uint4(0, 0, 0, 0));
+                // (a row that there is not: zeros, nothing is read)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(atom_addr(sQ + (u >> 3) * ATOM, r, u & 7)), "l"(p.q + (size_t)max(from, 0) * D + u * 8), "r"(from >= 0 ? 16 : 0) : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
@@ -227,8 +227,7 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
         if (elect_one()) {
             bool ok = true;
             const int* table = p.block_table + (size_t)p.prefix_row * p.max_pages + tile0;
-            int page = LLM_CHECK_INDEX(table[0], p.n_pages);
-            auto load = [&](int j, int kv, int full, int empty) {
+            auto load = [&](int j, int page, int kv, int full, int empty) {
                 const int b = j % X::STAGES;
                 ok = mbar_wait(bar(empty + b), (j / X::STAGES & 1) ^ 1, abort_flag);
                 if (!ok) return;
@@ -238,11 +237,15 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
 #pragma unroll
                 for (int a = 0; a < DA; ++a) tma_load_2d(dst + a * X::K_ATOM, &map_kv, a * 64, y, bar(full + b));
             };
+            // K a tile ahead of V: its places become free before V's do
+            int page = LLM_CHECK_INDEX(table[0], p.n_pages), next = LLM_CHECK_INDEX(nt > 1 ? table[1] : 0, p.n_pages);
+            load(0, page, 0, K_FULL, K_EMPTY);
             for (int j = 0; j < nt && ok; ++j) {
-                const int next = j + 1 < nt ? table[j + 1] : 0;
-                load(j, 0, K_FULL, K_EMPTY);
-                if (ok) load(j, 1, V_FULL, V_EMPTY);
-                page = LLM_CHECK_INDEX(next, p.n_pages);
+                const int after = j + 2 < nt ? table[j + 2] : 0;
+                if (j + 1 < nt) load(j + 1, next, 0, K_FULL, K_EMPTY);
+                if (ok) load(j, page, 1, V_FULL, V_EMPTY);
+                page = next;
+                next = LLM_CHECK_INDEX(after, p.n_pages);
             }
         }
     } else if (elect_one()) {
@@ -275,17 +278,18 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
             mma_commit(bar(K_EMPTY + j % X::STAGES));
         }
         for (int j = 0; j < nt && ok; ++j) {
-            ok = mbar_wait(bar(V_FULL + j % X::STAGES), j / X::STAGES & 1, abort_flag) && (j + 2 >= nt || scores(j + 2));
+            ok = mbar_wait(bar(V_FULL + j % X::STAGES), j / X::STAGES & 1, abort_flag);
             for (int slot = 0; slot < slots && ok; ++slot) {
                 ok = mbar_wait(bar(P_FULL + buffer(slot, j)), phase(j), abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 issue_o(slot, j);
-                if (j + 2 < nt) issue_s(slot, j + 2);       // behind the P V that reads P from the same columns
+                if (slot == slots - 1) mma_commit(bar(V_EMPTY + j % X::STAGES));
+                if (j + 2 >= nt) continue;
+                if (slot == 0) ok = scores(j + 2);
+                if (ok) issue_s(slot, j + 2);               // behind the P V that reads P from the same columns
             }
-            if (!ok) break;
-            mma_commit(bar(V_EMPTY + j % X::STAGES));
-            if (j + 2 < nt) mma_commit(bar(K_EMPTY + (j + 2) % X::STAGES));
+            if (ok && j + 2 < nt) mma_commit(bar(K_EMPTY + (j + 2) % X::STAGES));
         }
     }
     tc_fence_before();
