@@ -16,7 +16,7 @@
 // What bounds it: the prefix, once read, by the tensor pipe and the exponentials from about 200 rows per K/V head on, else by its bytes; the tails by theirs.  61
 // sequences x 2 rows behind 20000 keys of 128 values: prefix 47 us (0.86 PFLOP/s), with the tails 66; a tile of 64 keys takes 1600 clocks of two slots, all of
 // which the products take (a product of 64 columns with both operands in shared memory 71 clocks, of 128 with one in tensor memory 71).  32 behind 8192
-// keys of 256 values 27, the tails beside the prefix; 128 behind 2048 keys of 64 values 20.
+// keys of 256 values 26, the tails beside the prefix; 128 behind 2048 keys of 64 values 20.
 #include "attn_tile.cuh"
 #include "hybrid.h"
 #include "launch.h"
