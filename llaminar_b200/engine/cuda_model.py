@@ -623,7 +623,7 @@ class CudaModel:
             ops.rope_part_kv(qkv, q, kv_layer, L.q_norm, L.k_norm, self._rope_freqs(), 1.0, fb.positions, fb.seq_ids, fb.block_table, H, Hk, D,
                              c.rms_eps, gated=c.attn_gate)
         else:
-            self._append_torch(L, fb, kv_layer, qkv, T, q)
+            q = self._append_torch(L, fb, kv_layer, qkv)
         o = self.ws_o[:T]
         o3 = o.view(T, H, D)
         scale = 1.0 / math.sqrt(D)
@@ -650,8 +650,8 @@ class CudaModel:
             z = self._zero_len = torch.zeros(1, dtype=torch.int32, device=self.device)
         return z
 
-    def _append_torch(self, L: CudaLayer, fb: ForwardBatch, kv_layer: torch.Tensor, qkv: torch.Tensor, T: int, q_out: torch.Tensor) -> None:
-        """Norm, rotation and cache append of head sizes without a kernel, on PyTorch ops."""
+    def _append_torch(self, L: CudaLayer, fb: ForwardBatch, kv_layer: torch.Tensor, qkv: torch.Tensor) -> torch.Tensor:
+        """Norm, rotation and cache append of head sizes without a kernel, on PyTorch ops; the queries in fp32."""
         from ..models.reference import rmsnorm, rope_split_half
         c = self.cfg
         H, Hk, D = self.n_heads_local, self.n_kv_local, c.head_dim
@@ -662,11 +662,12 @@ class CudaModel:
         if L.q_norm is not None:
             q, k = rmsnorm(q, L.q_norm, c.rms_eps), rmsnorm(k, L.k_norm, c.rms_eps)
         pos = fb.positions.long()
-        q_out.copy_(rope_split_half(q, pos, c.rope_theta, c.rotary_dim))
+        q = rope_split_half(q, pos, c.rope_theta, c.rotary_dim)
         k = rope_split_half(k, pos, c.rope_theta, c.rotary_dim)
         page = fb.block_table.long()[fb.seq_ids.long(), pos // 64]
         kv_layer[page, 0, :, pos % 64] = k.to(kv_layer.dtype)
         kv_layer[page, 1, :, pos % 64] = v.to(kv_layer.dtype)
+        return q
 
     def _attention_torch(self, q: torch.Tensor, fb: ForwardBatch, kv_layer: torch.Tensor, scale: float) -> torch.Tensor:
         return paged_attention_torch(q, kv_layer, fb.block_table, fb.seq_ids, fb.positions, scale)
