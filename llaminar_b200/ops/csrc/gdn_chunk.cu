@@ -238,7 +238,7 @@ constexpr int PREP_THREADS = 256;
 struct ChunkParams {
     GdnParams g;
     uint8_t* ws;                                            // [units][n_ks] chunks of key heads, then [units][n_v] of value heads
-    int n_ks, u0, units;                                    // key heads in use, first chunk of this pass, chunks of it
+    int n_ks, u0, units, first;                             // key heads in use, first chunk of this pass, chunks of it, whether it is the first pass
     int* status;
     int in_aligned, out_aligned;
 };
@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
     const GdnParams& p = cp.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ks = blockIdx.x, u = blockIdx.y;              // value heads ks, ks + n_k, ... read this key head
+    if (cp.first) pdl_wait();
     if (warp == 0) {
         int at;
         const int b = sequence_of(p, cp.u0 + u, at);
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
         }
     }
     __syncthreads();
-    // This kernel starts beside the scan of the pass before, which reads other memory.  The next launch waits for this one alone, so its last block waits for
+    // From the second pass on this kernel starts beside the scan of the pass before, which reads other memory.  The next launch waits for this one alone, so its last block waits for
     // that scan.
     const bool waits = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
     if (s_chunk[0] < 0) {
@@ -1025,7 +1026,8 @@ cudaError_t launch_gdn_chunk(const GdnParams& g, void* workspace, size_t bytes, 
         p.units = pass ? each : head;
         if (p.units > total - u0) p.units = total - u0;
         const dim3 grid(p.n_ks, p.units);
-        if (beside && pass) e = launch_pdl(prep, grid, dim3(gdc::PREP_THREADS), gdc::PREP_SMEM, st, p);
+        p.first = pass == 0;
+        if (beside || pass == 0) e = launch_pdl(prep, grid, dim3(gdc::PREP_THREADS), gdc::PREP_SMEM, st, p);
         else { prep<<<grid, gdc::PREP_THREADS, gdc::PREP_SMEM, st>>>(p); e = cudaGetLastError(); }
         if (e != cudaSuccess) return e;
         // (blocks of a scan that come up early help a single pass, 37 rows: 34.8 -> 30.8 us, and are in the way of the passes beside each other, 8192 rows: 620 -> 668 us)

@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int j = tid >> 2, part = tid & 3;                  // column of the state, quarter of its rows
     const int items = p.n_seqs * p.n_v, K = K4 ? 4 : p.K;
+    pdl_wait();                                              // (no trigger: the windows behind it are shifted without waiting)
     auto seq_of = [&](int item) { return gdn_seq(p, min(item, items - 1) / p.n_v); };
     auto unit_of = [](int row, int u) { return u ^ (2 * (row / QUARTER)) % (D / 4); };       // 16-byte unit u of a row of the state
 
@@ -300,6 +301,8 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) 
         fence_proxy_async();
     }
     __syncthreads();
+    pdl_wait();
+    pdl_trigger();
     auto slot_of = [&](int item) { return (size_t)LLM_CHECK_INDEX(p.slots[item / p.n_v], p.n_slots); };
     auto fetch = [&](int item, size_t slot, int buffer) {    // by one thread
         const float* from = p.rec + (slot * p.n_v + item % p.n_v) * (size_t)(D * D);
@@ -512,6 +515,7 @@ __global__ void __launch_bounds__(256, 4) gdn_commit_kernel(const GdnParams p, c
     __shared__ __align__(16) float s_u[BLOCK][D], s_k[BLOCK][D];
     __shared__ float s_a[BLOCK];
     const int b = blockIdx.y, tid = threadIdx.x, R = p.rows_per_seq;
+    pdl_wait();
     const int n = max(0, min(accepted[b], R));
     if (n == 0) return;
     const GdnSeq q = gdn_seq(p, b);
@@ -575,8 +579,7 @@ template <int D> static cudaError_t rows_of(const GdnParams& p, cudaStream_t st)
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
-        kernel<<<ctas, 4 * D, SMEM, st>>>(p);
-        return cudaGetLastError();
+        return launch_pdl(kernel, dim3(ctas), dim3(4 * D), SMEM, st, p);
     };
     if (p.keep_u) return p.K == 4 ? go(gdn_rows_kernel<D, true, true>) : go(gdn_rows_kernel<D, true, false>);
     return p.K == 4 ? go(gdn_rows_kernel<D, false, true>) : go(gdn_rows_kernel<D, false, false>);
@@ -589,8 +592,7 @@ template <int D> static cudaError_t drafts_of(const GdnParams& p, cudaStream_t s
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
-        kernel<<<ctas, 4 * D, SMEM, st>>>(p);
-        return cudaGetLastError();
+        return launch_pdl(kernel, dim3(ctas), dim3(4 * D), SMEM, st, p);
     };
     constexpr int MOST = D == 32 ? 4 : DRAFT_ROWS;           // a warp finishes a row
     if (p.rows_per_seq > 4 && MOST > 4) return p.K == 4 ? go(gdn_draft_kernel<D, MOST, true>) : go(gdn_draft_kernel<D, MOST, false>);
@@ -621,12 +623,11 @@ cudaError_t launch_gdn_commit(const GdnParams& p, const int* accepted, cudaStrea
     if (p.n_seqs == 0 || p.rows_per_seq == 0) return cudaSuccess;
     const dim3 grid(p.n_v * (p.d == 128 ? COMMIT_PARTS<128> : 1) + (p.C + 255) / 256, p.n_seqs);
     switch (p.d) {
-        case 32: gdn_commit_kernel<32><<<grid, 256, 0, st>>>(p, accepted); break;
-        case 64: gdn_commit_kernel<64><<<grid, 256, 0, st>>>(p, accepted); break;
-        case 128: gdn_commit_kernel<128><<<grid, 256, 0, st>>>(p, accepted); break;
+        case 32: return launch_pdl(gdn_commit_kernel<32>, grid, dim3(256), 0, st, p, accepted);
+        case 64: return launch_pdl(gdn_commit_kernel<64>, grid, dim3(256), 0, st, p, accepted);
+        case 128: return launch_pdl(gdn_commit_kernel<128>, grid, dim3(256), 0, st, p, accepted);
         default: return cudaErrorNotSupported;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace llm
