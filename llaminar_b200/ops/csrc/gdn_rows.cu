@@ -278,13 +278,16 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
 
 // Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, a quarter each, 32 bytes further than the one before: a
 // column's four threads meet other banks.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
-// them; now 60 us, 15 of them the states' bytes, 1700 clocks a row.)  o comes from the state in front of the row, S^T q = a S0^T q + u (k.q), so that a row has one round of sums.
+// them.)  The state is left alone, so no row needs one of its own: with S in front of the first row, A_r the product of the decays up to row r and w_i = u_i decayed
+// from row i to row r,
+//     a S_r-1^T k_r = A_r S^T k_r + sum_{i<r} w_i (k_i.k_r)       o_r = A_r S^T q_r + sum_{i<=r} w_i (k_i.q_r)
+// All products with S are one pass, and the chain of the rows is one of single numbers.  (Row after row with the state in registers, 1700 clocks a row: 60 us.)
 template <int D, int TB, bool K4>
-__global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) {
+__global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_draft_kernel(const GdnParams p) {
     using namespace tc5;
     constexpr int THREADS = 4 * D, WARPS = THREADS / 32, EPL = D / 32, QUARTER = D / 4, ROW = D + 16, STRIDE = QUARTER * D + 8;
     __shared__ __align__(16) float s_q[TB][ROW], s_k[TB][ROW];
-    __shared__ float s_v[TB][D], s_o[TB][D], s_a[TB], s_b[TB], s_kq[TB];
+    __shared__ float s_v[TB][D], s_o[TB][D], s_a[TB], s_b[TB], s_kk[TB][TB], s_kq[TB][TB];
     __shared__ __align__(8) uint64_t s_bar[2];
     __shared__ int s_abort[2];                               // [1] stays 0 here (tc_common.cuh: restarts the wait clock when set)
     extern __shared__ __align__(16) float s_state[];         // two states of four quarters, STRIDE apart
@@ -408,24 +411,22 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) 
         for (int e = 0; e < EPL; ++e) z[e] = __bfloat162float(now.z[e]);
         if (next < items) load(next, slot1, now);            // on their way from here on
         __syncthreads();
-        // ---- norms and k.q, a warp per row ----
+        // ---- norms, a warp per row ----
         if (warp < n) {
-            float qs = 0.f, ks = 0.f, kq = 0.f, q[EPL], k[EPL];
+            float qs = 0.f, ks = 0.f, q[EPL], k[EPL];
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
                 const int at = e * 32 + lane, to = at + at / QUARTER * 4;
                 q[e] = s_q[warp][to]; k[e] = s_k[warp][to];
-                qs += q[e] * q[e]; ks += k[e] * k[e]; kq += k[e] * q[e];
+                qs += q[e] * q[e]; ks += k[e] * k[e];
             }
             const float rq = rsqrtf(warp_sum(qs) + 1e-6f) * rsqrtf((float)D), rk = rsqrtf(warp_sum(ks) + 1e-6f);
-            kq = warp_sum(kq) * rq * rk;
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
                 const int at = e * 32 + lane, to = at + at / QUARTER * 4;
                 s_q[warp][to] = q[e] * rq; s_k[warp][to] = k[e] * rk;
                 p.keep_k[((size_t)(first + warp) * p.n_v + h) * D + at] = k[e] * rk;
             }
-            if (lane == 0) s_kq[warp] = kq;
         }
         mbar_wait_warp(bars + buffer * 8, phase, abort_flag);
         f32x2 S[QUARTER / 2];
@@ -436,34 +437,69 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_draft_kernel(const GdnParams p) 
         }
         __syncthreads();
         if (abort_flag[0]) break;
-        // ---- the rows ----
-#pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-            const float a = s_a[i];
-            const float4 *k4 = reinterpret_cast<const float4*>(&s_k[i][part * (QUARTER + 4)]), *q4 = reinterpret_cast<const float4*>(&s_q[i][part * (QUARTER + 4)]);
-            f32x2 d0 = pair(0.f, 0.f), d1 = d0, o0 = d0, o1 = d0, k[QUARTER / 2];
+        // ---- k.k and k.q of two rows, a warp per pair ----
+        for (int x = warp; x < n * n; x += WARPS) {
+            const int r = x / n, i = x % n;
+            if (i > r) continue;
+            float kk = 0.f, kq = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                const float ki = s_k[i][to];
+                kk += ki * s_k[r][to];
+                kq += ki * s_q[r][to];
+            }
+            kk = warp_sum(kk);
+            kq = warp_sum(kq);
+            if (lane == 0) { s_kk[r][i] = kk; s_kq[r][i] = kq; }
+        }
+        // ---- S^T k and S^T q of all rows, with the state in front of them ----
+        float dot[TB], o[TB];
+#pragma unroll
+        for (int r = 0; r < TB; ++r) {
+            if (r >= n) break;
+            const float4 *k4 = reinterpret_cast<const float4*>(&s_k[r][part * (QUARTER + 4)]), *q4 = reinterpret_cast<const float4*>(&s_q[r][part * (QUARTER + 4)]);
+            f32x2 d0 = pair(0.f, 0.f), d1 = d0, o0 = d0, o1 = d0;
 #pragma unroll
             for (int e = 0; e < QUARTER / 4; ++e) {
                 const float4 f = k4[e], g = q4[e];
-                k[2 * e] = pair(f.x, f.y); k[2 * e + 1] = pair(f.z, f.w);
-                d0 = fma2(S[2 * e], k[2 * e], d0);
-                d1 = fma2(S[2 * e + 1], k[2 * e + 1], d1);
+                d0 = fma2(S[2 * e], pair(f.x, f.y), d0);
+                d1 = fma2(S[2 * e + 1], pair(f.z, f.w), d1);
                 o0 = fma2(S[2 * e], pair(g.x, g.y), o0);
                 o1 = fma2(S[2 * e + 1], pair(g.z, g.w), o1);
             }
-            const float2 e0 = both(d0), e1 = both(d1), f0 = both(o0), f1 = both(o1);
-            float dot = (e0.x + e0.y) + (e1.x + e1.y), o = (f0.x + f0.y) + (f1.x + f1.y);
-            dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-            o += __shfl_xor_sync(0xffffffffu, o, 1);
-            dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-            o += __shfl_xor_sync(0xffffffffu, o, 2);
-            const float u = s_b[i] * (s_v[i][j] - a * dot);
+            const float2 e0 = both(add2(d0, d1)), f0 = both(add2(o0, o1));
+            dot[r] = e0.x + e0.y;
+            o[r] = f0.x + f0.y;
+        }
 #pragma unroll
-            for (int e = 0; e < QUARTER / 2; ++e) S[e] = fma2(k[e], pair(u, u), mul2(S[e], pair(a, a)));
+        for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+            for (int r = 0; r < TB; ++r) {
+                if (r >= n) break;
+                dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], off);
+                o[r] += __shfl_xor_sync(0xffffffffu, o[r], off);
+            }
+        __syncthreads();
+        // ---- the rows: their corrections, each decayed up to the row at hand, take the place of the states in between ----
+        float w[TB], all = 1.f;
+#pragma unroll
+        for (int r = 0; r < TB; ++r) {
+            if (r >= n) break;
+            const float a = s_a[r];
+            all *= a;
+            float x = all * dot[r], y = all * o[r];
+#pragma unroll
+            for (int i = 0; i < r; ++i) {
+                w[i] *= a;
+                x = fmaf(w[i], s_kk[r][i], x);
+                y = fmaf(w[i], s_kq[r][i], y);
+            }
+            w[r] = s_b[r] * (s_v[r][j] - x);
             if (part == 0) {
-                s_o[i][j] = fmaf(a, o, u * s_kq[i]);
-                const size_t at = (size_t)(first + i) * p.n_v + h;
-                p.keep_u[at * D + j] = u;
+                s_o[r][j] = fmaf(w[r], s_kq[r][r], y);
+                const size_t at = (size_t)(first + r) * p.n_v + h;
+                p.keep_u[at * D + j] = w[r];
                 if (j == 0) p.keep_a[at] = a;
             }
         }
