@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
     int item = blockIdx.x, buffer = 0;
     uint32_t phase = 0;                                      // of both barriers: it turns with every second item
     size_t slot = slot_of(item), slot1 = slot_of(min(item + (int)gridDim.x, items - 1));
-    if (tid == 0) fetch(item, slot, 0);
+    if (tid == THREADS - 1) fetch(item, slot, 0);             // (of the warps with the least to convolve)
     Rows now;
     load(item, slot, now);
     float gain[EPL];
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
     for (int e = 0; e < EPL; ++e) gain[e] = p.norm_w[e * 32 + lane];
     for (; item < items; item += gridDim.x) {
         const int h = item % p.n_v, b = item / p.n_v, first = b * n, next = item + gridDim.x;
-        if (tid == 0 && next < items) fetch(next, slot1, buffer ^ 1);          // (its place was read two barriers ago)
+        if (tid == THREADS - 1 && next < items) fetch(next, slot1, buffer ^ 1);          // (its place was read two barriers ago)
         const size_t slot2 = slot_of(min(next + (int)gridDim.x, items - 1));
         // ---- convolution, SiLU, gates ----
         if (kind < 3) {
@@ -438,9 +438,11 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
         __syncthreads();
         if (abort_flag[0]) break;
         // ---- k.k and k.q of two rows, a warp per pair ----
-        for (int x = warp; x < n * n; x += WARPS) {
-            const int r = x / n, i = x % n;
-            if (i > r) continue;
+        for (int x = warp; x < n * (n + 1) / 2; x += WARPS) {
+            int r = 0;
+#pragma unroll
+            for (int e = 1; e < TB; ++e) r += x >= e * (e + 1) / 2;
+            const int i = x - r * (r + 1) / 2;
             float kk = 0.f, kq = 0.f;
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
