@@ -22,8 +22,8 @@
 //
 // What bounds it: the scan's chain along the state, 7450 clocks a chunk: the state as an operand 1290, S^T k 1070, R 1280, U 500, U as an operand 960, the
 // state's sum 990, the state 530, and 200 for each of four signals.  Operands are in tensor memory since a product of 64 (128) columns takes 41 (71) clocks so and
-// 71 (100) with both in shared memory.  8192 rows of 16 / 48 heads take 609 us (57 by the bytes), five sequences of 900 rows on average 187 (preparation
-// 85, scan 102), 37 rows 31.
+// 71 (100) with both in shared memory.  8192 rows of 16 / 48 heads take 606 us (57 by the bytes), five sequences of 900 rows on average 184 (preparation
+// 85, scan 102), 37 rows 29.
 // Every mbarrier wait is bounded; on a timeout the kernel raises the status word and tears down.
 //
 // (reference: the chunk kernels of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu.)

@@ -276,23 +276,24 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
     }
 }
 
-// Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, a quarter each, 32 bytes further than the one before: a
-// column's four threads meet other banks.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
+// Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, an eighth each, 16 bytes further than the one before: the
+// eight threads of two columns meet other banks.  Two columns a thread since what k and q take of shared memory's bandwidth is the longest phase.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
 // them.)  The state is left alone, so no row needs one of its own: with S in front of the first row, A_r the product of the decays up to row r and w_i = u_i decayed
 // from row i to row r,
 //     a S_r-1^T k_r = A_r S^T k_r + sum_{i<r} w_i (k_i.k_r)       o_r = A_r S^T q_r + sum_{i<=r} w_i (k_i.q_r)
-// All products with S are one pass, and the chain of the rows is one of single numbers.  (Row after row with the state in registers, 1700 clocks a row: 60 us.)
+// All products with S are one pass, and the chain of the rows is one of single numbers.  (Row after row, the state in
+// registers, 1700 clocks a row, 60 us; with a column a thread 51; now 46, 15 of them the states' bytes.)
 template <int D, int TB, bool K4>
 __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_draft_kernel(const GdnParams p) {
     using namespace tc5;
-    constexpr int THREADS = 4 * D, WARPS = THREADS / 32, EPL = D / 32, QUARTER = D / 4, ROW = D + 16, STRIDE = QUARTER * D + 8;
+    constexpr int THREADS = 4 * D, WARPS = THREADS / 32, EPL = D / 32, EIGHTH = D / 8, ROW = D + 32, STRIDE = EIGHTH * D + 4;
     __shared__ __align__(16) float s_q[TB][ROW], s_k[TB][ROW];
     __shared__ float s_v[TB][D], s_o[TB][D], s_a[TB], s_b[TB], s_kk[TB][TB], s_kq[TB][TB];
     __shared__ __align__(8) uint64_t s_bar[2];
     __shared__ int s_abort[2];                               // [1] stays 0 here (tc_common.cuh: restarts the wait clock when set)
-    extern __shared__ __align__(16) float s_state[];         // two states of four quarters, STRIDE apart
+    extern __shared__ __align__(16) float s_state[];         // two states of eight parts, STRIDE apart
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int j = tid >> 2, part = tid & 3;
+    const int j = tid >> 3, part = tid & 7, col = 2 * j + (part & 1);         // two columns, an eighth of their rows; the column whose sums end up here
     const int items = p.n_seqs * p.n_v, K = K4 ? 4 : p.K, n = p.rows_per_seq;
     const uint32_t bars = smem_u32(s_bar);
     volatile int* abort_flag = s_abort;
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
         fence_proxy_async();                                 // what stood there has been read
         mbar_arrive_expect_tx(bars + buffer * 8, D * D * 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bulk_load(smem_u32(s_state + (buffer * 4 + i) * STRIDE), from + i * QUARTER * D, QUARTER * D * 4, bars + buffer * 8);
+        for (int i = 0; i < 8; ++i) bulk_load(smem_u32(s_state + (buffer * 8 + i) * STRIDE), from + i * EIGHTH * D, EIGHTH * D * 4, bars + buffer * 8);
     };
     const int kind = tid / D, i_ch = tid % D;                // this thread's channel: of q, k and v in the first three quarters of the threads
     struct Rows {                                            // an item's, as they were loaded
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
                 if (i >= n) break;
                 const float v = silu(y[i]);
                 if (kind == 2) s_v[i][i_ch] = v;
-                else (kind ? s_k : s_q)[i][i_ch + i_ch / QUARTER * 4] = v;
+                else (kind ? s_k : s_q)[i][i_ch + i_ch / EIGHTH * 4] = v;
                 // the convolution's inputs, for the commit: a channel of q and k by the first value head that reads it
                 if (kind == 2 || (h < p.n_k && p.n_v >= p.n_k)) p.keep_x[((size_t)b * n + i) * p.C + c] = now.x[i];
             }
@@ -416,24 +417,28 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
             float qs = 0.f, ks = 0.f, q[EPL], k[EPL];
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
-                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                const int at = e * 32 + lane, to = at + at / EIGHTH * 4;
                 q[e] = s_q[warp][to]; k[e] = s_k[warp][to];
                 qs += q[e] * q[e]; ks += k[e] * k[e];
             }
             const float rq = rsqrtf(warp_sum(qs) + 1e-6f) * rsqrtf((float)D), rk = rsqrtf(warp_sum(ks) + 1e-6f);
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
-                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                const int at = e * 32 + lane, to = at + at / EIGHTH * 4;
                 s_q[warp][to] = q[e] * rq; s_k[warp][to] = k[e] * rk;
                 p.keep_k[((size_t)(first + warp) * p.n_v + h) * D + at] = k[e] * rk;
             }
         }
         mbar_wait_warp(bars + buffer * 8, phase, abort_flag);
-        f32x2 S[QUARTER / 2];
+        f32x2 S[2][EIGHTH / 2];
         {
-            const float* x = s_state + (buffer * 4 + part) * STRIDE + j;
+            const float* x = s_state + (buffer * 8 + part) * STRIDE + 2 * j;
 #pragma unroll
-            for (int i = 0; i < QUARTER / 2; ++i) S[i] = pair(x[2 * i * D], x[(2 * i + 1) * D]);
+            for (int i = 0; i < EIGHTH / 2; ++i) {
+                const float2 even = *reinterpret_cast<const float2*>(x + 2 * i * D), odd = *reinterpret_cast<const float2*>(x + (2 * i + 1) * D);
+                S[0][i] = pair(even.x, odd.x);
+                S[1][i] = pair(even.y, odd.y);
+            }
         }
         __syncthreads();
         if (abort_flag[0]) break;
@@ -446,7 +451,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
             float kk = 0.f, kq = 0.f;
 #pragma unroll
             for (int e = 0; e < EPL; ++e) {
-                const int at = e * 32 + lane, to = at + at / QUARTER * 4;
+                const int at = e * 32 + lane, to = at + at / EIGHTH * 4;
                 const float ki = s_k[i][to];
                 kk += ki * s_k[r][to];
                 kq += ki * s_q[r][to];
@@ -460,22 +465,25 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
 #pragma unroll
         for (int r = 0; r < TB; ++r) {
             if (r >= n) break;
-            const float4 *k4 = reinterpret_cast<const float4*>(&s_k[r][part * (QUARTER + 4)]), *q4 = reinterpret_cast<const float4*>(&s_q[r][part * (QUARTER + 4)]);
-            f32x2 d0 = pair(0.f, 0.f), d1 = d0, o0 = d0, o1 = d0;
+            const float4 *k4 = reinterpret_cast<const float4*>(&s_k[r][part * (EIGHTH + 4)]), *q4 = reinterpret_cast<const float4*>(&s_q[r][part * (EIGHTH + 4)]);
+            f32x2 d[2] = {pair(0.f, 0.f), pair(0.f, 0.f)}, x[2] = {d[0], d[0]};
 #pragma unroll
-            for (int e = 0; e < QUARTER / 4; ++e) {
+            for (int e = 0; e < EIGHTH / 4; ++e) {
                 const float4 f = k4[e], g = q4[e];
-                d0 = fma2(S[2 * e], pair(f.x, f.y), d0);
-                d1 = fma2(S[2 * e + 1], pair(f.z, f.w), d1);
-                o0 = fma2(S[2 * e], pair(g.x, g.y), o0);
-                o1 = fma2(S[2 * e + 1], pair(g.z, g.w), o1);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    d[c] = fma2(S[c][2 * e + 1], pair(f.z, f.w), fma2(S[c][2 * e], pair(f.x, f.y), d[c]));
+                    x[c] = fma2(S[c][2 * e + 1], pair(g.z, g.w), fma2(S[c][2 * e], pair(g.x, g.y), x[c]));
+                }
             }
-            const float2 e0 = both(add2(d0, d1)), f0 = both(add2(o0, o1));
-            dot[r] = e0.x + e0.y;
-            o[r] = f0.x + f0.y;
+            const float2 d0 = both(d[0]), d1 = both(d[1]), x0 = both(x[0]), x1 = both(x[1]);
+            const bool odd = part & 1;
+            const float ds[2] = {d0.x + d0.y, d1.x + d1.y}, xs[2] = {x0.x + x0.y, x1.x + x1.y};
+            dot[r] = (odd ? ds[1] : ds[0]) + __shfl_xor_sync(0xffffffffu, odd ? ds[0] : ds[1], 1);
+            o[r] = (odd ? xs[1] : xs[0]) + __shfl_xor_sync(0xffffffffu, odd ? xs[0] : xs[1], 1);
         }
 #pragma unroll
-        for (int off = 1; off < 4; off <<= 1)
+        for (int off = 2; off < 8; off <<= 1)
 #pragma unroll
             for (int r = 0; r < TB; ++r) {
                 if (r >= n) break;
@@ -497,12 +505,12 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_dra
                 x = fmaf(w[i], s_kk[r][i], x);
                 y = fmaf(w[i], s_kq[r][i], y);
             }
-            w[r] = s_b[r] * (s_v[r][j] - x);
-            if (part == 0) {
-                s_o[r][j] = fmaf(w[r], s_kq[r][r], y);
+            w[r] = s_b[r] * (s_v[r][col] - x);
+            if (part < 2) {
+                s_o[r][col] = fmaf(w[r], s_kq[r][r], y);
                 const size_t at = (size_t)(first + r) * p.n_v + h;
-                p.keep_u[at * D + j] = w[r];
-                if (j == 0) p.keep_a[at] = a;
+                p.keep_u[at * D + col] = w[r];
+                if (col == 0) p.keep_a[at] = a;
             }
         }
         __syncthreads();
