@@ -276,13 +276,14 @@ __global__ void __launch_bounds__(4 * D, 1) gdn_rows_kernel(const GdnParams p) {
     }
 }
 
-// Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, an eighth each, 16 bytes further than the one before: the
-// eight threads of two columns meet other banks.  Two columns a thread since what k and q take of shared memory's bandwidth is the longest phase.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the barriers waited behind
-// them.)  The state is left alone, so no row needs one of its own: with S in front of the first row, A_r the product of the decays up to row r and w_i = u_i decayed
-// from row i to row r,
+// Drafted rows: at most TB of every sequence, in one block.  The states arrive by bulk copies, two at a time, an eighth each, 16 bytes further than the one before:
+// the eight threads of two columns meet other banks.  (By 16-byte copies of all threads, 73 us at three rows of 32 x 48 heads, the loads in front of the
+// barriers waited behind them.)  The state is left alone, so no row needs one of its own: with S in front of the first row, A_r the product of the decays up to row r
+// and w_i = u_i decayed from row i to row r,
 //     a S_r-1^T k_r = A_r S^T k_r + sum_{i<r} w_i (k_i.k_r)       o_r = A_r S^T q_r + sum_{i<=r} w_i (k_i.q_r)
-// All products with S are one pass, and the chain of the rows is one of single numbers.  (Row after row, the state in
-// registers, 1700 clocks a row, 60 us; with a column a thread 51; now 46, 15 of them the states' bytes.)
+// All products with S are one pass, and the chain of the rows is one of single numbers.  Two columns a thread, since what k and q take of shared memory's
+// bandwidth is the longest phase.  (Row after row, the state in registers, 1700 clocks a row, 60 us; in one pass with a column a thread 51; now 46, 15 of them the
+// states' bytes.)
 template <int D, int TB, bool K4>
 __global__ void __launch_bounds__(4 * D, D == 128 ? 1 : D == 64 ? 2 : 4) gdn_draft_kernel(const GdnParams p) {
     using namespace tc5;
