@@ -13,7 +13,7 @@ D, N_K, N_V = 128, 16, 16
 
 
 class _Call:
-    def __init__(self, lens, pos, seed=5):
+    def __init__(self, lens, pos, seed=5, aligned=False):
         self.lens, self.pos, T = lens, pos, sum(lens)
         self.buf, self.width, self.w, self.conv, self.rec = _rows_problem(seed, T, D, N_K, N_V, 4, len(lens) + 1)
         self.cu = [0]
@@ -23,7 +23,9 @@ class _Call:
         self.positions = it([p + t for n, p in zip(lens, pos) for t in range(n)])
         self.cu_d, self.slots = it(self.cu), it(list(range(len(lens), 0, -1)))
         self.dw = {k: v.to(DEV) if torch.is_tensor(v) else v for k, v in self.w.items()}
-        self.inp = self.buf.to(DEV)[:, :self.width]
+        self.inp = self.buf.to(DEV)[:, :self.width]            # rows an odd number of values apart
+        if aligned:
+            self.inp = self.inp.contiguous()
         self.fresh_state()
 
     def fresh_state(self):
@@ -60,8 +62,9 @@ def test_every_division_into_passes_gives_the_same_bits(monkeypatch, lens, pos):
             assert torch.equal(a, b), chunks
 
 
-def test_a_long_prompt_follows_the_recurrence(monkeypatch):
-    call = _Call([1500], [9])
+@pytest.mark.parametrize("aligned", [False, True])
+def test_a_long_prompt_follows_the_recurrence(monkeypatch, aligned):
+    call = _Call([1500], [9], aligned=aligned)
     _hold(monkeypatch, 12)
     call.run()
     out, conv, rec = call.results()
@@ -112,3 +115,15 @@ def test_two_streams_at_once(monkeypatch):
     for c, want in zip(calls, wants):
         for a, b in zip(c.results(), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lens,pos", [([37], [0]), ([63, 130, 1, 64], [2, 0, 5, 0])])
+def test_rows_on_and_off_their_boundaries_give_the_same_bits(lens, pos):
+    """Four taps in the same order either way."""
+    results = []
+    for aligned in (False, True):
+        call = _Call(lens, pos, aligned=aligned)
+        call.run()
+        results.append(call.results())
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
