@@ -881,6 +881,7 @@ class LLMEngine:
         r.prompt = r.prompt + r.output[r.n_folded:]
         r.n_folded = len(r.output)
         r.state, r.hidden, r.terminal, r.prefix_hit_tokens = "waiting", None, None, 0
+        self._lane_sig = None                          # it may be back, with other pages, before a step without it
         self.waiting.insert(0, r)
         self.stats["preemptions"] += 1
 
@@ -904,17 +905,22 @@ class LLMEngine:
     SHARED_MIN_SAVED = 12300
 
     def _shared_tokens(self, reqs: list[Request]) -> int:
-        """Leading tokens (whole pages) that the sequences have in the same pages, as after a hit of the prefix cache, if taking them once for all pays."""
-        n = min((r.n_tokens - 1) // PAGE_SIZE for r in reqs)
-        first = reqs[0].kv.pages
-        if len(reqs) < 2 or n == 0 or reqs[1].kv.pages[0] != first[0] or self.kv.q8 or not getattr(self.model, "shares_prefixes", bool)():
+        """Leading tokens (whole pages) that the sequences have in the same pages, as after a hit of the prefix cache, if taking them once for all pays.  The same
+        number on every rank that steps together, since the captured step depends on it: page ids are each rank's own, and up to the agreement the answer comes
+        from what all ranks know.  To be asked when the lanes change: the pages in common were there when the sequences were admitted, and tables only grow."""
+        B, most = len(reqs), min(r.n_tokens - 1 for r in reqs) // PAGE_SIZE
+        pays = lambda n: n >= self.SHARED_MIN_TOKENS and n * (B - 1) >= self.SHARED_MIN_SAVED
+        if self.prefix_cache is None or not pays(most * PAGE_SIZE):
             return 0
-        for r in reqs[1:]:
+        n = 0 if self.kv.q8 or not getattr(self.model, "shares_prefixes", bool)() else most
+        head = reqs[0].kv.pages[:n]
+        for r in reqs[1:] if n else ():
             pages = r.kv.pages
-            if pages[:n] != first[:n]:
-                n = next(i for i in range(n) if pages[i] != first[i])
-        n *= PAGE_SIZE
-        return n if n >= self.SHARED_MIN_TOKENS and n * (len(reqs) - 1) >= self.SHARED_MIN_SAVED else 0
+            if pages[:n] != head:
+                n = next(i for i in range(n) if pages[i] != head[i])
+                head = head[:n]
+        n = self._agree_min(n * PAGE_SIZE)
+        return n if pays(n) else 0
 
     def _splits_for(self, bucket: int) -> int:
         if not self.is_cuda:
@@ -976,7 +982,8 @@ class LLMEngine:
                 ln[B:bucket] = 1
                 bt[B:bucket] = 0
                 temp[B:bucket] = 0.0
-        h[v["shared"]] = self._lane_shared = self._shared_tokens(reqs)
+            self._lane_shared = self._shared_tokens(reqs)
+        h[v["shared"]] = self._lane_shared
         for i, r in enumerate(reqs):
             npg = len(r.kv.pages)
             if npg != self._lane_pages[i]:
