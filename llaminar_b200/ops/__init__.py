@@ -78,14 +78,17 @@ class Scratch:
             t.zero_()
 
 
-_scratch: dict[str, Scratch] = {}
+_scratch: dict[torch.device, Scratch] = {}
 
 
 def scratch_for(device) -> Scratch:
-    key = str(device)
-    if key not in _scratch:
-        _scratch[key] = Scratch.create(device)
-    return _scratch[key]
+    """The scratch of a device.  "cuda" is the current device: a tensor on it says "cuda:0", and both have to mean the same status word."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    if device not in _scratch:
+        _scratch[device] = Scratch.create(device)
+    return _scratch[device]
 
 
 def _accum_args(pw: PackedWeight, rows: int, sc: Scratch | None):
