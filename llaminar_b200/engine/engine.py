@@ -1114,7 +1114,8 @@ class LLMEngine:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self._decode_body(bucket, greedy, v, pen, sample)
-        key = (bucket, greedy, pen) if pen else (bucket, greedy) if sample else (bucket, "logits")
+        shared = v.get("max_shared", 0)
+        key = (bucket, greedy, pen, shared) if shared else (bucket, greedy, pen) if pen else (bucket, greedy) if sample else (bucket, "logits")
         self.launches_per_graph[key] = ops.launch_count() - n0
         if self.kv.hybrid is not None:
             self._dec_dev[:v["n"]].copy_(self._dec_host[:v["n"]], non_blocking=True)
