@@ -559,6 +559,22 @@ class CudaModel:
         return (self.stack is None and self.cfg.head_dim in ops.SHARED_HEAD_SIZES and self.n_heads_local % self.n_kv_local == 0
                 and self.n_heads_local // self.n_kv_local * rows_per_seq <= 16)
 
+    # Bytes of K and V of a block that sharing saves a decode step, and sequences of 128-wide ungated heads, from which it pays to take a prefix once
+    PREFIX_MIN_BYTES = 80_000_000
+    PREFIX_MIN_SEQS = 20
+
+    def prefix_pays(self, n_seqs: int, tokens: int) -> bool:
+        """Whether a decode step of ``n_seqs`` sequences that share ``tokens`` leading ones is faster with them taken once.  The second launch and the joining of its
+        parts cost 4 to 8 us a block, and sequences that read the same pages find them in L2, so it takes 80 MB.  Captured, us of a block, each sequence by itself
+        and shared: 24 / 4 gated heads of 256: 16 sequences behind 512 tokens (31 MB) 18 and 21, 16 behind 2048 (126 MB) 31 and 25; 16 / 2 gated heads of 256: 3
+        behind 8192 (34 MB) 21 and 31, 24 behind 2048 (96 MB) 26 and 25; 32 / 8 heads of 128: 4 behind 4096 (50 MB) 21 and 25, 6 behind 4096 (84 MB) 29 and 25;
+        16 / 4 heads of 64: 24 behind 1024 (24 MB) 16 and 18.  Many sequences of 128-wide ungated heads gain or lose little below that: 32 behind 512 of 32 / 8 heads
+        21 and 18, 24 behind 640 of 16 / 2 heads 16 and 21, 24 behind 1024 of 16 / 4 heads 21 and 16."""
+        if not self.shares_prefixes():
+            return False
+        saved = tokens * (n_seqs - 1) * self.n_kv_local * self.cfg.head_dim * 4
+        return saved >= self.PREFIX_MIN_BYTES or (self.cfg.head_dim == 128 and not self.cfg.attn_gate and n_seqs >= self.PREFIX_MIN_SEQS)
+
     def _linear_attention(self, L: CudaLayer, fb: ForwardBatch, inp: torch.Tensor, T: int) -> torch.Tensor:
         """Between the input and output projections of a Gated-DeltaNet block.  Decode steps (one row per sequence) run
         the two step kernels on the sequences' state slots, prefill chunks the chunk-parallel kernels, and a deferred pass (drafts) leaves the

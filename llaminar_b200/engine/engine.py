@@ -898,29 +898,31 @@ class LLMEngine:
                             rows_per_seq=1, n_splits=self._splits_for(B),
                             state_slots=it([r.slot for r in reqs]) if self.kv.hybrid is not None else None)
 
-    # Shared tokens, and tokens that sharing saves a step's sequences, from which a batch takes its prefix once (us of a layer's attention, each sequence by itself and
-    # shared, 32 / 8 heads of 128: 16 sequences behind 512 tokens 11.2 and 10.3, 4 behind 4096 14.7 and 16.4, 8 behind 2048 14.9 and 14.7, 32 behind 2048 35 and 15, 64
-    # behind 8192 235 and 29)
+    # Shared tokens, and tokens that sharing saves a step's sequences, below which a batch takes its prefix with every sequence's own keys whatever its heads are
+    # (`CudaModel.prefix_pays` has the rule on their sizes)
     SHARED_MIN_TOKENS = 512
     SHARED_MIN_SAVED = 12300
 
     def _shared_tokens(self, reqs: list[Request]) -> int:
         """Leading tokens (whole pages) that the sequences have in the same pages, as after a hit of the prefix cache, if taking them once for all pays.  The same
-        number on every rank that steps together, since the captured step depends on it: page ids are each rank's own, and up to the agreement the answer comes
-        from what all ranks know.  To be asked when the lanes change: the pages in common were there when the sequences were admitted, and tables only grow."""
+        number on every rank that steps together, since the captured step depends on it: page ids and heads are each rank's own, and apart from the agreement the
+        answer comes from what all ranks know.  To be asked when the lanes change: the pages in common were there when the sequences were admitted, and tables only
+        grow."""
         B, most = len(reqs), min(r.n_tokens - 1 for r in reqs) // PAGE_SIZE
-        pays = lambda n: n >= self.SHARED_MIN_TOKENS and n * (B - 1) >= self.SHARED_MIN_SAVED
-        if self.prefix_cache is None or not pays(most * PAGE_SIZE):
+        enough = lambda n: n >= self.SHARED_MIN_TOKENS and n * (B - 1) >= self.SHARED_MIN_SAVED
+        if self.prefix_cache is None or not enough(most * PAGE_SIZE):
             return 0
-        n = 0 if self.kv.q8 or not getattr(self.model, "shares_prefixes", bool)() else most
+        pays = getattr(self.model, "prefix_pays", None)
+        n = 0 if self.kv.q8 or pays is None else most
         head = reqs[0].kv.pages[:n]
         for r in reqs[1:] if n else ():
             pages = r.kv.pages
             if pages[:n] != head:
                 n = next(i for i in range(n) if pages[i] != head[i])
                 head = head[:n]
-        n = self._agree_min(n * PAGE_SIZE)
-        return n if pays(n) else 0
+        n *= PAGE_SIZE
+        n = self._agree_min(n if n and pays(B, n) else 0)
+        return n if enough(n) else 0
 
     def _splits_for(self, bucket: int) -> int:
         if not self.is_cuda:

@@ -19,7 +19,7 @@ def _engine(common: int, group=None, shares: bool = True) -> tuple[LLMEngine, li
     e = LLMEngine.__new__(LLMEngine)
     e.max_pages_per_seq, e._agree_group, e.stats, e.device = PAGES, group, {}, torch.device("cpu")
     e.kv = types.SimpleNamespace(hybrid=None, q8=False)
-    e.model = types.SimpleNamespace(shares_prefixes=lambda: shares)
+    e.model = types.SimpleNamespace(prefix_pays=lambda n_seqs, tokens: shares)
     e.prefix_cache = object()
     n = BUCKET * (2 + 1 + PAGES + 3 + 1) + 1
     e._dec_host, e._dec_dev = torch.zeros(n, dtype=torch.int32), torch.zeros(n, dtype=torch.int32)
@@ -87,3 +87,29 @@ def test_without_a_prefix_cache_nothing_is_looked_for():
     e.prefix_cache = None
     e._agree_min = None                                           # not called
     assert _stage(e, reqs) == 0
+
+
+# heads, kv heads, head size, gated, sequences, shared tokens, whether a captured step was faster with the prefix taken once (by more than its spread)
+MEASURED = [
+    (24, 4, 256, True, 16, 512, False), (24, 4, 256, True, 3, 4096, False), (24, 4, 256, True, 16, 2048, True), (24, 4, 256, True, 32, 2048, True),
+    (16, 2, 256, True, 3, 8192, False), (16, 2, 256, True, 16, 1024, False), (16, 2, 256, True, 64, 2048, True), (16, 2, 256, True, 8, 16384, True),
+    (32, 8, 128, False, 4, 4096, False), (32, 8, 128, False, 2, 8192, False), (32, 8, 128, False, 6, 8192, True), (32, 8, 128, False, 32, 512, True),
+    (16, 2, 128, True, 8, 8192, False), (16, 2, 128, True, 32, 1024, False), (16, 2, 128, True, 64, 8192, True),
+    (16, 4, 64, False, 24, 1024, False), (32, 8, 64, False, 24, 512, False), (32, 8, 64, False, 32, 2048, True),
+]
+
+
+def test_a_prefix_is_taken_once_where_that_was_faster():
+    """The rule on the heads' sizes against measured steps of several of them."""
+    from llaminar_b200.engine.cuda_model import CudaModel
+    for H, Hk, D, gated, B, tokens, faster in MEASURED:
+        m = types.SimpleNamespace(cfg=types.SimpleNamespace(head_dim=D, attn_gate=gated), n_heads_local=H, n_kv_local=Hk, stack=None,
+                                  PREFIX_MIN_BYTES=CudaModel.PREFIX_MIN_BYTES, PREFIX_MIN_SEQS=CudaModel.PREFIX_MIN_SEQS)
+        m.shares_prefixes = lambda: CudaModel.shares_prefixes(m)
+        e, reqs = _engine(640)
+        e.model = types.SimpleNamespace(prefix_pays=lambda n, t: CudaModel.prefix_pays(m, n, t))
+        reqs = [Request(rid=i, prompt=[1] * (tokens + 9), params=SamplingParams(temperature=0.0), output=[2], kv=SequenceKV(list(range(1, 1 + tokens // PAGE_SIZE)) + [10000 + i]))
+                for i in range(B)]
+        assert e._shared_tokens(reqs) == (tokens if faster else 0), (H, Hk, D, gated, B, tokens)
+    m.stack = object()                                             # a model whose blocks have attention of their own
+    assert not CudaModel.prefix_pays(m, 64, 8192)
