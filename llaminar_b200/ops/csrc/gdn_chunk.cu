@@ -401,7 +401,9 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                 if (t < ch.n) {
                     const __nv_bfloat16* ab = p.in + (size_t)(ch.row0 + t) * p.in_row + p.ab_off;
                     const float x = __bfloat162float(ab[h]) + dt;
-                    g[e] = a * (x > 20.f ? x : log1pf(expf(x)));
+                    // -10000 is a decay of 0, and differences of sums that hold some of them stay numbers (of two infinities they would not)
+                    const float log_decay = a * (x > 20.f ? x : log1pf(expf(x)));
+                    g[e] = log_decay < -10000.f ? -10000.f : log_decay;
                     b[e] = beta(p, ch, t, h);
                 }
             }
