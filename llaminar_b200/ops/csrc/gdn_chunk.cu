@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             vec[V_ALL / 2 + lane] = make_float2(ea, ea);
         }
         __syncthreads();
-        // ---- A and P, up to the diagonal's blocks: what lies above is not read.  16 rows and 2, 4, 6, 8 units of eight columns for each block of rows ----
+        // ---- A and P, up to the diagonal's blocks.  16 rows and 2, 4, 6, 8 units of eight columns for each block of rows ----
 #pragma unroll 1
         for (int item = tid; item < nh * 320; item += PREP_THREADS) {
             const int hi = item / 320, k = item % 320, tb = (k >= 32) + (k >= 96) + (k >= 192), off = k - 16 * tb * (tb + 1), half = off >> 1;
@@ -467,6 +467,16 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             *reinterpret_cast<uint4*>(A + TRI + at) = al;
             *reinterpret_cast<uint4*>(dst + OFF_PHI + at) = ph;
             *reinterpret_cast<uint4*>(dst + OFF_PLO + at) = pl;
+        }
+        // zeros of P above them: 16 rows and 6, 4, 2 units
+#pragma unroll 1
+        for (int item = tid; item < nh * 192; item += PREP_THREADS) {
+            const int hi = item / 192, k = item % 192, tb = (k >= 96) + (k >= 160);
+            const int row = tb == 0 ? k / 6 : tb == 1 ? (k - 96) >> 2 : (k - 160) >> 1;
+            const int t = 16 * tb + row, unit = 2 * (tb + 1) + (tb == 0 ? k - 6 * row : tb == 1 ? (k - 96) & 3 : (k - 160) & 1);
+            uint8_t* at = head_chunk(cp, u, h0 + hi * p.n_k) + t * 128 + (((unit ^ t) & 7) << 4);
+            *reinterpret_cast<uint4*>(at + OFF_PHI) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(at + OFF_PLO) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
         // ---- the diagonal's blocks of T, in the place of A's: a thread per column ----
@@ -570,6 +580,9 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                 const int t = 16 * i + 8 * (m >> 1) + (lane >> 2);
                 *reinterpret_cast<uint32_t*>(T + t * 128 + (((2 * j + (m & 1)) ^ (t & 7)) << 4) + (lane & 3) * 4) = x[m];
             }
+            __syncwarp();                                   // all lanes have the transpose: zeros above the diagonal
+            const int above = 16 * j + (lane & 15);
+            *reinterpret_cast<uint4*>(T + above * 128 + (((2 * i + (lane >> 4)) ^ (above & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
 #pragma unroll 4
@@ -929,11 +942,12 @@ __global__ void __launch_bounds__(THREADS, 1) gdn_chunk_scan_kernel(const ChunkP
                         mma_f16_ts(tm + d, tm + a + (at + 2 * half) * 8, desc + (k >> 1) * (IMG / 2 / 16) + 2 * (k & 1), idesc(C), !first_one || k > 0 ? 1u : 0u);
                     }
                 };
-                auto with_tri = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {       // [128 columns x 64 rows] times a lower triangle's transpose
+                // [128 columns x 64 rows] times a lower triangle's transpose.  All of one shape and accumulator, zeros above the diagonal included: only such products are
+                // promised to run in the order in which they are issued, and each adds to what the one before left
+                auto with_tri = [&](uint32_t d, uint32_t a, uint32_t img, bool first_one) {
                     const uint64_t desc = smem_desc_sw128(img);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)             // columns in front of the diagonal's block are zero
-                        mma_f16_ts(tm + d + 16 * k, tm + a + k * 8, desc + k * (16 * 128 / 16) + 2 * k, idesc(C - 16 * k), !first_one || k > 0 ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) mma_f16_ts(tm + d, tm + a + k * 8, desc + 2 * k, idesc(C), !first_one || k > 0 ? 1u : 0u);
                 };
                 auto with_keys = [&](uint32_t a, uint32_t img, bool first_one) {                  // [128 columns x 64 rows] [64 rows x d]
                     const uint64_t desc = smem_desc_mn_sw128(img, IMG / 2);
