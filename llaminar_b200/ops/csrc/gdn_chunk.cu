@@ -233,7 +233,7 @@ constexpr int PREP_A = 2 * C * C * 4, PREP_DIAG = PREP_A + PREP_HEADS * 2 * TRI;
 constexpr int PREP_SMEM = PREP_DIAG + PREP_HEADS * C * 16 * 4;                              // and their diagonal blocks in fp32
 static_assert(PREP_DIAG >= KEY_BYTES, "the images");
 constexpr float SX = 1024.f;                                // factor of sum_k A_ik T_kj = -(I + A_ii) T_ij, at most 17
-constexpr int PREP_THREADS = 256;
+constexpr int PREP_THREADS = 256, BAD_HEADS = 64;           // (of a key head's value heads, those 64 apart share a place)
 
 struct ChunkParams {
     GdnParams g;
@@ -250,11 +250,12 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(16) float2 s_G[PREP_HEADS][C];          // a sum as a float and what that leaves of it
     __shared__ float s_b[PREP_HEADS][C];
-    __shared__ int s_chunk[6];
+    __shared__ int s_chunk[6], s_bad[1 + BAD_HEADS];        // first rows whose keys, and whose values of a head, are not finite
     const GdnParams& p = cp.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ks = blockIdx.x, u = blockIdx.y;              // value heads ks, ks + n_k, ... read this key head
     if (cp.first) pdl_wait();
+    if (tid <= BAD_HEADS) s_bad[tid] = C;
     if (warp == 0) {
         int at;
         const int b = sequence_of(p, cp.u0 + u, at);
@@ -312,6 +313,27 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                 const float r = __shfl_sync(0xffffffffu, mine, 4 * i);
                 y[i][0] = mul2(y[i][0], pair(r, r));
                 y[i][1] = mul2(y[i][1], pair(r, r));
+            }
+            // A product of the chunk has all of its rows, those that do not see a row times 0: a key or a value that is not finite would reach the rows in front of
+            // it.  Zeros take its place; from its row on the head's outputs, and its state, are no numbers (the gates, below).
+            if (part > 0) {
+                f32x2 any = pair(0.f, 0.f);                 // not finite if one of them is not (or, looked at again, if products overflow)
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) any = fma2(y[i][0], y[i][1], any);
+                const float2 f = both(any);
+                if (__any_sync(0xffffffffu, (f.x + f.y) * 0.f != 0.f)) {
+                    unsigned rows = 0;
+#pragma unroll
+                    for (int i = 0; i < ROWS; ++i) {
+                        const float2 g = both(fma2(y[i][1], pair(0.f, 0.f), mul2(y[i][0], pair(0.f, 0.f))));
+                        rows |= g.x + g.y != 0.f ? 1u << i : 0u;
+                    }
+                    rows = __reduce_or_sync(0xffffffffu, rows);
+#pragma unroll
+                    for (int i = 0; i < ROWS; ++i)
+                        if (rows >> i & 1) y[i][0] = y[i][1] = pair(0.f, 0.f);
+                    if (lane == 0 && rows) atomicMin(&s_bad[part == 1 ? 0 : 1 + (part - 2) % BAD_HEADS], warp * ROWS + __ffs(rows) - 1);
+                }
             }
             if (part < 2) {
                 uint8_t* img = key_chunk(cp, u, ks);
@@ -386,7 +408,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
     const float* s_kk = reinterpret_cast<const float*>(smem);
     const float* s_qk = s_kk + C * C;
 
-    for (int h0 = ks; h0 < p.n_v; h0 += PREP_HEADS * p.n_k) {
+    for (int h0 = ks, place = 0; h0 < p.n_v; h0 += PREP_HEADS * p.n_k, place += PREP_HEADS) {
         const int nh = min(PREP_HEADS, (p.n_v - h0 + p.n_k - 1) / p.n_k);
         __syncthreads();
         // ---- gates: a warp per head, two rows a lane ----
@@ -407,6 +429,15 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
                     b[e] = beta(p, ch, t, h);
                 }
             }
+            int bad = min(s_bad[0], s_bad[1 + (place + warp) % BAD_HEADS]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const unsigned m = __ballot_sync(0xffffffffu, g[e] * b[e] != g[e] * b[e]);
+                if (m) bad = min(bad, 2 * (__ffs(m) - 1) + e);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (2 * lane + e >= bad) g[e] = b[e] = 0.f;
             // sums in units of ln 2, as exp2 takes them
             const double l0 = (double)g[0] * 1.4426950408889634, l1 = (double)g[1] * 1.4426950408889634;
             double sum = l0 + l1;
@@ -420,9 +451,9 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) gdn_chunk_prep_kernel(const C
             s_G[warp][2 * lane] = make_float2(f0, (float)(G0 - f0)); s_G[warp][2 * lane + 1] = make_float2(f1, (float)(G1 - f1));
             s_b[warp][2 * lane] = b[0]; s_b[warp][2 * lane + 1] = b[1];
             float2* vec = reinterpret_cast<float2*>(head_chunk(cp, u, h) + OFF_VEC);
-            const float e0 = ex2((float)G0), e1 = ex2((float)G1), ea = ex2((float)all);
+            const float e0 = ex2((float)G0), e1 = ex2((float)G1), ea = bad < C ? __int_as_float(0x7fffffff) : ex2((float)all);
             vec[V_BE / 2 + lane] = make_float2(b[0] * e0, b[1] * e1);
-            vec[V_EG / 2 + lane] = make_float2(e0, e1);
+            vec[V_EG / 2 + lane] = make_float2(2 * lane >= bad ? __int_as_float(0x7fffffff) : e0, 2 * lane + 1 >= bad ? __int_as_float(0x7fffffff) : e1);
             vec[V_EL / 2 + lane] = make_float2(ex2((float)(all - G0)), ex2((float)(all - G1)));
             vec[V_ALL / 2 + lane] = make_float2(ea, ea);
         }

@@ -54,7 +54,8 @@ def gdn_prefill(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torc
     Rows cu[b] .. cu[b + 1] of ``inp`` and ``out`` are sequence b's; its state, the slot slots[b] of the layer's fp32 pools conv_state
     [slots, C, K - 1] and rec [slots, n_v, d, d], is advanced in place.  A sequence whose first row has position 0 starts from zeros, whatever
     its slot holds.  Sequences have slots of their own; one without rows keeps its state, and rows outside of all sequences are left as
-    they are.  d is 32, 64 or 128; ssm_a is not positive, so that no decay grows."""
+    they are.  d is 32, 64 or 128; ssm_a is not positive, so that no decay grows.  Values of a row that are not finite reach no row in front of it, no other sequence
+    and no head that does not read them; in chunks all outputs of a head behind such a key, value or gate are NaN, and its state."""
     ws = _gdn_workspace(inp, slots.numel(), n_k, rec.shape[1], rec.shape[-1]) if inp.is_cuda else None
     _count(ext().gdn_prefill(inp, C, z_off, ab_off, conv_w, ssm_a, dt_bias, norm_w, conv_state, rec, positions, cu, slots, out, n_k, v_head_offset, eps,
                              ws, scratch_for(inp.device).status if ws is not None else None))
