@@ -304,12 +304,19 @@ __global__ void __launch_bounds__(Prefix<D, SLOTS>::THREADS, 1) attn_prefix_kern
                 if (!ok) break;
                 tc_fence_after();
                 issue_o(slot, j);
-                if (slot == slots - 1) mma_commit(bar(V_EMPTY + j % X::STAGES));
-                if (j + 2 >= nt) continue;
-                if (slot == 0) ok = scores(j + 2);
-                if (ok) issue_s(slot, j + 2);               // behind the P V that reads P from the same columns
             }
-            if (ok && j + 2 < nt) mma_commit(bar(K_EMPTY + (j + 2) % X::STAGES));
+            if (ok) mma_commit(bar(V_EMPTY + j % X::STAGES));
+            if (j + 2 >= nt) continue;
+            // The scores of tile j + 2 take the columns that P of tile j lies in.  Products of two shapes have no promised order, so P V is waited for; the other
+            // slot's, or the softmax of tile j + 1, is at work meanwhile
+            ok = ok && scores(j + 2);
+            for (int slot = 0; slot < slots && ok; ++slot) {
+                ok = mbar_wait(bar(PV_DONE + slot), j & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                issue_s(slot, j + 2);
+            }
+            if (ok) mma_commit(bar(K_EMPTY + (j + 2) % X::STAGES));
         }
     }
     tc_fence_before();
