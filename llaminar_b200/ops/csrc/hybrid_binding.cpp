@@ -2,6 +2,8 @@
 // nor loads it.  Every argument is checked on the host before a launch.
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cfloat>
+
 #include "binding_util.h"
 #include "hybrid.h"
 #include "launch.h"
@@ -187,6 +189,7 @@ int attn_decode_shared(const Tensor& q, const Tensor& kv, const Tensor& out, con
     TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head size must be 64, 128 or 256");
     TORCH_CHECK(n_kv_heads >= 1 && n_heads >= 1 && n_heads <= 65535 && n_heads % n_kv_heads == 0, "query heads must be a multiple of K/V heads");
     TORCH_CHECK(rows_per_seq >= 1 && n_heads / n_kv_heads * rows_per_seq <= 16, "at most 16 rows x heads of a group per sequence");
+    TORCH_CHECK((float)scale > 0.f && scale <= FLT_MAX, "scale must be positive and finite");
     p.block_table = table_arg(q, block_table, p.n_seqs, p.max_pages);
     TORCH_CHECK(p.n_seqs <= 65535 && (int64_t)p.max_pages * 64 <= INT32_MAX, "more than 65535 sequences, or too many pages");
     TORCH_CHECK(q.numel() == p.n_seqs * rows_per_seq * n_heads * head_dim, "q must be [sequences * rows, heads, head size]");

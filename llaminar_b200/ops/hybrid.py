@@ -114,7 +114,7 @@ def attn_decode_shared(q: torch.Tensor, kv: torch.Tensor, out: torch.Tensor, blo
     int32 on the device), in the pages that block_table[prefix_row] begins with.  Those pages, the last one whole even if the prefix ends in it, stand
     in front of the table of every sequence whose rows all see the prefix; a shorter sequence, or one of no keys, takes nothing from it.  ``max_shared``
     (host; 0: nothing is shared) and ``max_tail`` (most keys of a sequence behind the prefix; 0: unknown) only decide how the keys are shared out.
-    ``gate`` [rows, heads, head size]: its sigmoid multiplies the result.  Head sizes 64, 128 and 256, up to 16 rows x query heads per K/V head."""
+    ``gate`` [rows, heads, head size]: its sigmoid multiplies the result.  ``scale`` is positive.  Head sizes 64, 128 and 256, up to 16 rows x query heads per K/V head."""
     _count(ext().attn_decode_shared(q, kv, out, block_table, seq_lens, shared_len, n_heads, n_kv_heads, head_dim, rows_per_seq, scale, gate, max_shared, max_tail,
                                     prefix_row, scratch.attn_tickets, scratch.status))
 
