@@ -710,13 +710,13 @@ AttnSharedPlan attn_shared_plan(int n_seqs, int rows_per_seq, int n_heads, int n
     if (max_shared > 0 && rows > 0) {
         const int per_cta = head_dim == 256 || rows <= ash::BQ ? ash::BQ : 2 * ash::BQ, bk = ash::PAGE;
         const long long ctas = (rows + per_cta - 1) / per_cta * n_kv_heads, tiles = (max_shared + bk - 1) / bk;
-        long long s = 148 / ctas;
+        long long s = sm_count() / ctas;
         if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
         if (s > ash::MAX_PARTS) s = ash::MAX_PARTS;
         plan.splits = s < 1 ? 1 : (int)s;
     }
     const long long pairs = (long long)n_seqs * n_kv_heads, pages = (max_tail + ash::PAGE - 1) / ash::PAGE;
-    long long t = pairs > 0 ? 148 * (head_dim == 256 ? 1 : head_dim == 128 ? 2 : 4) / pairs : 1;
+    long long t = pairs > 0 ? sm_count() * (head_dim == 256 ? 1 : head_dim == 128 ? 2 : 4) / pairs : 1;
     if (t > (pages + 1) / 2) t = (pages + 1) / 2;
     if (t > ash::MAX_PARTS) t = ash::MAX_PARTS;
     plan.tail_splits = t < 1 || pairs > max_tickets ? 1 : (int)t;

@@ -622,7 +622,7 @@ template <int D> static cudaError_t rows_of(const GdnParams& p, cudaStream_t st)
     constexpr int SMEM = 2 * D * D * 4;
     const long long items = (long long)p.n_v * p.n_seqs;
     if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
-    const unsigned ctas = (unsigned)std::min<long long>(items, 148 * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
+    const unsigned ctas = (unsigned)std::min<long long>(items, sm_count() * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;
@@ -635,7 +635,7 @@ template <int D> static cudaError_t drafts_of(const GdnParams& p, cudaStream_t s
     constexpr int SMEM = 2 * (D * D + 4 * 8) * 4;
     const long long items = (long long)p.n_v * p.n_seqs;
     if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
-    const unsigned ctas = (unsigned)std::min<long long>(items, 148 * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
+    const unsigned ctas = (unsigned)std::min<long long>(items, sm_count() * (D == 128 ? 1 : D == 64 ? 2 : 4));        // as many as fit at once
     auto go = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return e;

@@ -244,7 +244,7 @@ cudaError_t launch_rope_part(const RopePartParams& args, cudaStream_t st) {
     // A warp takes all heads of a token where the tokens give every SM `per_sm` warps, else the heads are shared out; up to eight heads go one at a time.
     const int per_sm = p.head_dim == 256 ? 8 : 16;
     p.parts = 1;
-    while ((long long)p.n_tokens * p.parts < 148 * per_sm && p.parts < heads) p.parts *= 2;
+    while ((long long)p.n_tokens * p.parts < sm_count() * per_sm && p.parts < heads) p.parts *= 2;
     if (p.parts > heads) p.parts = heads;
     const long long ctas = ((long long)p.n_tokens * p.parts + WARPS - 1) / WARPS;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
