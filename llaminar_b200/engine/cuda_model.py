@@ -653,7 +653,7 @@ class CudaModel:
         elif self.torch_attention:
             o3.copy_(self._attention_torch(q.float(), fb, kv_layer, scale))
         elif fb.is_decode:
-            ops.attn_decode(q, kv_layer, o3, fb.block_table, fb.seq_lens, H, Hk, D, fb.rows_per_seq, scale, fb.n_splits, self.scratch)
+            raise ValueError(f"decode steps of {D}-wide heads take up to 16 rows x query heads of a K/V head, not {H // Hk * fb.rows_per_seq}")
         else:
             ops.attn_prefill(q, kv_layer, o3, fb.block_table, fb.cu_q, fb.ctx_lens, H, Hk, D, scale, fb.max_q_len, scratch=self.scratch, max_kv_len=fb.max_kv_len)
         if gate is not None:
