@@ -13,8 +13,11 @@
 //
 // Nothing that a row does not see reaches it: K and V rows of the tiles' ends are masked and zeroed, and the last drafted keys, which some rows of a
 // sequence see and others do not, are taken one by one (a probability of 0 times an infinity would not be 0).
+// Roundings: scores, maxima, sums and O are 32-bit.  Probabilities enter P V as bf16, the type that the tensor cores take beside V: each is off by 2^-8 of itself at
+// most, and the sums are of those that are not rounded.  On outputs of random values that is an error of 2.2e-3 in all, of which 1.7e-3 are the rounding of
+// the outputs themselves; a second product with what is left of P would take it away, and the products bound the prefix already.
 // What bounds it: the prefix, once read, by the tensor pipe and the exponentials from about 200 rows per K/V head on, else by its bytes; the tails by theirs.  61
-// sequences x 2 rows behind 20000 keys of 128 values: prefix 47 us (0.86 PFLOP/s), with the tails 66; a tile of 64 keys takes 1600 clocks of two slots, all of
+// sequences x 2 rows behind 20000 keys of 128 values: 69 us with the tails; a tile of 64 keys takes 1600 clocks of two slots, nearly all of
 // which the products take (a product of 64 columns with both operands in shared memory 71 clocks, of 128 with one in tensor memory 71).  32 behind 8192
 // keys of 256 values 26, the tails beside the prefix; 128 behind 2048 keys of 64 values 20.
 #include "attn_tile.cuh"

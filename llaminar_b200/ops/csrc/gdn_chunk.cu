@@ -21,9 +21,9 @@
 // sum cancels was 2^-7 off behind the gated norm.)  G is summed in 64 bits: differences of sums near -100 would cost a 32-bit one 2^-17.
 //
 // What bounds it: the scan's chain along the state, 7450 clocks a chunk: the state as an operand 1290, S^T k 1070, R 1280, U 500, U as an operand 960, the
-// state's sum 990, the state 530, and 200 for each of four signals.  Operands are in tensor memory since a product of 64 (128) columns takes 41 (71) clocks so and
-// 71 (100) with both in shared memory.  8192 rows of 16 / 48 heads take 606 us (57 by the bytes), five sequences of 900 rows on average 184 (preparation
-// 85, scan 102), 37 rows 29.
+// state's sum 990, the state 530, and 200 for each of four signals (U before its products had all 64 columns: three groups of four at 41 clocks now).  Operands are in tensor memory since a product of 64 (128) columns takes 41 (71) clocks so and
+// 71 (100) with both in shared memory.  8192 rows of 16 / 48 heads take 608 us (57 by the bytes), five sequences of 900 rows on average 188 (preparation
+// 86, scan 102), 37 rows 30.5.
 // Every mbarrier wait is bounded; on a timeout the kernel raises the status word and tears down.
 //
 // (reference: the chunk kernels of src/v2/kernels/cuda/gdn/CUDAGatedDeltaNetKernels.cu.)
@@ -96,7 +96,9 @@ LLM_DEVICE uint2 four(const __nv_bfloat16* x, bool aligned) {
 // sigmoid of a row's second gate
 LLM_DEVICE float beta(const GdnParams& p, const Chunk& ch, int t, int h) { return 1.f / (1.f + expf(-__bfloat162float(p.in[(size_t)(ch.row0 + t) * p.in_row + p.ab_off + p.n_v + h]))); }
 LLM_DEVICE f32x2 two_of(uint32_t w) { return pair(bf16_lo(w), bf16_hi(w)); }
-LLM_DEVICE f32x2 silu2(f32x2 x) {                           // x / (1 + e^-x)
+// x / (1 + e^-x).  The exponential and the reciprocal are the approximate ones, a few 2^-23 off (and the exponent's own rounding, 2^-24 of it), far below the half
+// step of the bf16 outputs, 2^-8.  gdn_rows.cu has the like from other instructions, so the two forms' last bits differ.
+LLM_DEVICE f32x2 silu2(f32x2 x) {
     const float2 e = both(mul2(x, pair(-1.44269504f, -1.44269504f)));
     float2 r = both(add2(pair(ex2(e.x), ex2(e.y)), pair(1.f, 1.f)));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(r.x));
