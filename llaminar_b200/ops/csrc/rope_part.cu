@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(32 * WARPS, ODD ? 1 : D == 256 ? 4 : 6) rope_p
     }
     uint8_t* page = nullptr;
     if (h1 > p.n_heads) {
-        const int seq = LLM_CHECK_INDEX(p.seq_ids[t], p.n_seqs), slot = LLM_CHECK_INDEX(pos / PAGE, p.max_pages);
+        const int seq = LLM_CHECK_INDEX(p.seq_ids[t], p.n_seqs), slot = LLM_CHECK_INDEX(pos >> 6, p.max_pages);          // (a shift: -1 is no page, not the first one)
         page = p.kv + (size_t)LLM_CHECK_INDEX(p.block_table[(size_t)seq * p.max_pages + slot], p.n_pages) * p.page_bytes;
     }
 
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(32 * WARPS, ODD ? 1 : D == 256 ? 4 : 6) rope_p
                     store_raw<N>(p.q_out + ((size_t)t * p.n_heads + h) * D + i0, raw[j]);
                     continue;
                 }
-                const size_t at = ((size_t)(kind - 1) * p.n_kv_heads + (h - p.n_heads - (kind - 1) * p.n_kv_heads)) * PAGE + pos % PAGE;
+                const size_t at = ((size_t)(kind - 1) * p.n_kv_heads + (h - p.n_heads - (kind - 1) * p.n_kv_heads)) * PAGE + (pos & (PAGE - 1));
                 if (!p.q8) {
                     store_raw<N>(reinterpret_cast<__nv_bfloat16*>(page) + at * D + i0, raw[j]);
                     continue;
