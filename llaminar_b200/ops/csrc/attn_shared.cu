@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : D == 128 ? 3 : 1) attn_tail
 #pragma unroll
                 for (int e = 0; e < VPL; ++e) d += x[e] * kx[e];
                 const float score = warp_sum(d) * sl2, top = fmaxf(m, score);
-                if (top == -INFINITY) continue;
+                if (top == -INFINITY && score == -INFINITY) continue;       // (a score that is no number goes on, and makes the row one that is none)
                 const float c = exp2f(m - top), w = exp2f(score - top);
                 m = top;
                 l = l * c + w;
