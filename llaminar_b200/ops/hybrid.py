@@ -63,7 +63,8 @@ def gdn_prefill(inp: torch.Tensor, C: int, z_off: int, ab_off: int, conv_w: torc
 
 @dataclass
 class GdnStash:
-    """What `gdn_verify` keeps for `gdn_commit`: decay, key and correction of every row and head, and the convolution's inputs."""
+    """What `gdn_verify` keeps for `gdn_commit`: decay, key and correction of every row and head, the convolution's inputs, and the sequences' slots (the tensor itself:
+    it still says the same at the commit)."""
     decay: torch.Tensor            # [B, R, n_v]
     key: torch.Tensor              # [B, R, n_v, d]
     correction: torch.Tensor       # [B, R, n_v, d]
